@@ -353,6 +353,104 @@ int kda_gate_fwd(const kda_gate_args* args, void* stream);
 int kda_gate_bwd(const kda_gate_args* args, void* stream);
 
 /* ------------------------------------------------------------------------------------------------
+ * The gated delta rule with ONE decay per token and head (g is [tokens, H]; everywhere else in this header it is one per key column):
+ *
+ *     S_t = exp(g_t) (I - beta_t k_t k_t^T) S_{t-1} + beta_t k_t v_t^T,      o_t = scale * S_t^T q_t
+ *
+ * kda_delta_recurrent_fwd: kda_recurrent_fwd with that g.  The fields of kda_recurrent_args keep their meaning but for these: `g` points to
+ * [tokens, H] of g_raw_dtype and `beta` to [tokens, H] of beta_raw_dtype, whether A_log and beta_sigmoid are given or not; dt_bias is [H].
+ *
+ * kda_delta_chunk_fwd / _bwd: whole sequences in chunks of 64 tokens on the tensor cores, bf16 q, k, v, o.  States, their gradients and every sum are
+ * fp32, and operands that are not inputs are bf16 pairs in the two walks over a sequence: final states and dh0 carry about 1e-5 of their norm.  Rules as
+ * for kda_chunk_fwd / _bwd: the workspace of a forward with save_for_backward goes to the backward untouched; kda_chunk_status reads its status word.
+ * ------------------------------------------------------------------------------------------------ */
+typedef struct kda_delta_args {
+  const void* q;               /* [tokens, HQ, K] bf16 */
+  const void* k;               /* [tokens, HQ, K] bf16 */
+  const void* v;               /* [tokens, H, V]  bf16 */
+  const void* g;               /* [tokens, H] g_dtype, log-decay (<= 0; -inf forgets the state) */
+  const void* beta;            /* [tokens, H] beta_dtype */
+  const float* h0;             /* [N, H, K, V] fp32 or NULL */
+  const int32_t* cu_seqlens;   /* device [N+1], or NULL: N sequences of tokens / N tokens */
+  void* o;                     /* [tokens, H, V] bf16 */
+  float* ht;                   /* [N, H, K, V] fp32 or NULL */
+  /* backward */
+  const void* d_o;             /* [tokens, H, V] bf16 */
+  const float* d_ht;           /* [N, H, K, V] fp32 or NULL */
+  void* dq;                    /* [tokens, HQ, K] bf16, summed over a group's value heads */
+  void* dk;                    /* [tokens, HQ, K] bf16 */
+  void* dv;                    /* [tokens, H, V]  bf16 */
+  void* dg;                    /* [tokens, H] g_dtype */
+  void* dbeta;                 /* [tokens, H] beta_dtype */
+  float* dh0;                  /* [N, H, K, V] fp32 or NULL */
+  void* workspace;             /* >= kda_delta_chunk_workspace_bytes(..), 256-byte aligned */
+  size_t workspace_bytes;
+  void* bwd_workspace;         /* >= kda_delta_chunk_bwd_workspace_bytes(..), 256-byte aligned */
+  size_t bwd_workspace_bytes;
+  int64_t tokens;
+  int32_t N, H, HQ;            /* HQ: heads of q and k (0: H); value head h reads head h / (H / HQ) */
+  int32_t K, V;                /* multiples of 8 up to 128 */
+  int32_t io_dtype;            /* KDA_BF16 */
+  int32_t g_dtype, beta_dtype; /* KDA_BF16 or KDA_FP32 */
+  int32_t use_qk_l2norm;       /* rows of q and k count as x * rsqrt(sum x^2 + 1e-6) */
+  int32_t save_for_backward;
+  int32_t scan_slices;         /* CTAs per (sequence, head) of the walks: 0 = by the number of units and SMs; 1 (backward: 2), 2, 4.  Results do not depend on it
+                                  beyond the order of a product's partial sums. */
+  float scale;
+} kda_delta_args;
+
+size_t kda_delta_chunk_workspace_bytes(int64_t tokens, int32_t N, int32_t H, int32_t K, int32_t V, int32_t save_for_backward);
+size_t kda_delta_chunk_bwd_workspace_bytes(int64_t tokens, int32_t N, int32_t H, int32_t HQ, int32_t K, int32_t V);
+int kda_delta_chunk_fwd(const kda_delta_args* args, void* stream);
+int kda_delta_chunk_bwd(const kda_delta_args* args, void* stream);
+int kda_delta_recurrent_fwd(const kda_recurrent_args* args, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * The norms around a block, over the last dimension of [rows, cols] tensors (rms(x) = sqrt(mean x^2 + eps)):
+ *
+ *     kda_gated_norm:     y = x / rms(x) * weight * act(gate)                        act: sigmoid(z) or z sigmoid(z)
+ *     kda_residual_norm:  b = x, or x / rms(x) * post_weight;   r = residual + scale * b;   y = r / rms(r) * weight
+ *
+ * Sums are fp32, y is computed from r before its rounding, and every tensor is bf16 or fp32 on its own (gradients in their tensor's type).  The backward calls
+ * recompute what they need from the forward's inputs.  Sums over rows (dweight, dpost_weight, dscale) go through the workspace in a fixed order.
+ * cols up to 8192 (KDA_E_LIMIT beyond), any number; multiples of 8 with 16-byte aligned tensors are read 16 bytes at a time.
+ * ------------------------------------------------------------------------------------------------ */
+#define KDA_ACT_SIGMOID 0
+#define KDA_ACT_SILU 1
+typedef struct kda_norm_args {
+  const void* x;               /* [rows, cols] io_dtype */
+  const void* gate;            /* gated: [rows, cols] gate_dtype */
+  const void* residual;        /* residual: [rows, cols] residual_dtype */
+  const void* weight;          /* [cols] weight_dtype; gated: or NULL (1) */
+  const void* post_weight;     /* residual: [cols] post_dtype or NULL (b = x) */
+  const void* scale;           /* residual: [cols] scale_dtype, or NULL: scale_value */
+  void* y;                     /* out, forward: [rows, cols] io_dtype */
+  void* r;                     /* out, forward, residual: [rows, cols] residual_dtype */
+  const void* dy;              /* in, backward: io_dtype; residual: or NULL (zero), not both */
+  const void* dr;              /* in, backward, residual: residual_dtype, or NULL (zero) */
+  void* dx;                    /* out, backward: io_dtype */
+  void* dgate;                 /* out, backward, gated: gate_dtype */
+  void* dresidual;             /* out, backward, residual: residual_dtype, or NULL */
+  void* dweight;               /* out, backward: [cols] of the parameter's type, or NULL (as the next two) */
+  void* dpost_weight;
+  void* dscale;
+  void* workspace;             /* backward with a sum over rows: >= kda_norm_bwd_workspace_bytes(rows, cols, gated: 1, residual: 3) */
+  size_t workspace_bytes;
+  int64_t rows;
+  int32_t cols;
+  int32_t io_dtype, gate_dtype, residual_dtype, weight_dtype, post_dtype, scale_dtype; /* KDA_BF16 or KDA_FP32 */
+  int32_t activation;          /* gated: KDA_ACT_* */
+  float eps;
+  float scale_value;
+} kda_norm_args;
+
+size_t kda_norm_bwd_workspace_bytes(int64_t rows, int32_t cols, int32_t sums);
+int kda_gated_norm_fwd(const kda_norm_args* args, void* stream);
+int kda_gated_norm_bwd(const kda_norm_args* args, void* stream);
+int kda_residual_norm_fwd(const kda_norm_args* args, void* stream);
+int kda_residual_norm_bwd(const kda_norm_args* args, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
  * Strided host <-> device copy for the host-resident pipeline (no counterpart in the Python operator): `rows`
  * rows of `width_bytes`, `spitch` / `dpitch` bytes apart, on `stream` (cudaMemcpy2DAsync, direction inferred from the
  * pointers).  Lets a head range [h0, h1) of a pinned [tokens, H, D] tensor travel as one copy.

@@ -69,6 +69,28 @@ class GateArgs(C.Structure):
     ]
 
 
+class DeltaArgs(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("g", C.c_void_p), ("beta", C.c_void_p),
+        ("h0", C.c_void_p), ("cu_seqlens", C.c_void_p), ("o", C.c_void_p), ("ht", C.c_void_p), ("d_o", C.c_void_p), ("d_ht", C.c_void_p),
+        ("dq", C.c_void_p), ("dk", C.c_void_p), ("dv", C.c_void_p), ("dg", C.c_void_p), ("dbeta", C.c_void_p), ("dh0", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("bwd_workspace", C.c_void_p), ("bwd_workspace_bytes", C.c_size_t),
+        ("tokens", C.c_int64), ("N", C.c_int32), ("H", C.c_int32), ("HQ", C.c_int32), ("K", C.c_int32), ("V", C.c_int32), ("io_dtype", C.c_int32),
+        ("g_dtype", C.c_int32), ("beta_dtype", C.c_int32), ("use_qk_l2norm", C.c_int32), ("save_for_backward", C.c_int32), ("scan_slices", C.c_int32),
+        ("scale", C.c_float),
+    ]
+
+
+class NormArgs(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("gate", C.c_void_p), ("residual", C.c_void_p), ("weight", C.c_void_p), ("post_weight", C.c_void_p), ("scale", C.c_void_p),
+        ("y", C.c_void_p), ("r", C.c_void_p), ("dy", C.c_void_p), ("dr", C.c_void_p), ("dx", C.c_void_p), ("dgate", C.c_void_p), ("dresidual", C.c_void_p),
+        ("dweight", C.c_void_p), ("dpost_weight", C.c_void_p), ("dscale", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+        ("rows", C.c_int64), ("cols", C.c_int32), ("io_dtype", C.c_int32), ("gate_dtype", C.c_int32), ("residual_dtype", C.c_int32),
+        ("weight_dtype", C.c_int32), ("post_dtype", C.c_int32), ("scale_dtype", C.c_int32), ("activation", C.c_int32), ("eps", C.c_float), ("scale_value", C.c_float),
+    ]
+
+
 EXPORTS = (
     "kda_b200_abi_version", "kda_b200_strerror", "kda_recurrent_fwd", "kda_recurrent_status",
     "kda_recurrent_bwd_workspace_bytes", "kda_recurrent_bwd",
@@ -77,6 +99,8 @@ EXPORTS = (
     "kda_chunk_max_chunks", "kda_chunk_workspace_bytes", "kda_chunk_bwd_workspace_bytes",
     "kda_chunk_fwd", "kda_chunk_bwd", "kda_chunk_status", "kda_chunk_fwd_noalloc", "kda_chunk_export_states",
     "kda_gate_bwd_workspace_bytes", "kda_gate_fwd", "kda_gate_bwd",
+    "kda_delta_chunk_workspace_bytes", "kda_delta_chunk_bwd_workspace_bytes", "kda_delta_chunk_fwd", "kda_delta_chunk_bwd", "kda_delta_recurrent_fwd",
+    "kda_norm_bwd_workspace_bytes", "kda_gated_norm_fwd", "kda_gated_norm_bwd", "kda_residual_norm_fwd", "kda_residual_norm_bwd",
     "kda_copy_rows_async", "kda_b200_profile_enable", "kda_b200_profile_read",
 )
 
@@ -136,6 +160,20 @@ def load() -> C.CDLL:
         fn = getattr(lib, name)
         fn.restype = C.c_int
         fn.argtypes = [C.POINTER(GateArgs), C.c_void_p]
+    lib.kda_delta_recurrent_fwd.restype = C.c_int
+    lib.kda_delta_recurrent_fwd.argtypes = [C.POINTER(RecurrentArgs), C.c_void_p]
+    lib.kda_delta_chunk_workspace_bytes.restype = lib.kda_delta_chunk_bwd_workspace_bytes.restype = C.c_size_t
+    lib.kda_delta_chunk_workspace_bytes.argtypes = lib.kda_delta_chunk_bwd_workspace_bytes.argtypes = [C.c_int64] + [C.c_int32] * 5
+    for name in ("kda_delta_chunk_fwd", "kda_delta_chunk_bwd"):
+        fn = getattr(lib, name)
+        fn.restype = C.c_int
+        fn.argtypes = [C.POINTER(DeltaArgs), C.c_void_p]
+    lib.kda_norm_bwd_workspace_bytes.restype = C.c_size_t
+    lib.kda_norm_bwd_workspace_bytes.argtypes = [C.c_int64, C.c_int32, C.c_int32]
+    for name in ("kda_gated_norm_fwd", "kda_gated_norm_bwd", "kda_residual_norm_fwd", "kda_residual_norm_bwd"):
+        fn = getattr(lib, name)
+        fn.restype = C.c_int
+        fn.argtypes = [C.POINTER(NormArgs), C.c_void_p]
     lib.kda_copy_rows_async.restype = C.c_int
     lib.kda_copy_rows_async.argtypes = [C.c_void_p, C.c_size_t, C.c_void_p, C.c_size_t, C.c_size_t, C.c_size_t, C.c_void_p]
     lib.kda_b200_profile_enable.restype = C.c_int

@@ -95,7 +95,8 @@ def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False, 
             if verbose:
                 print(" ".join(cmd), flush=True)
             subprocess.check_call(cmd)
-    if force or _stale(HOST_LIB, [os.path.join(CSRC, "host", "kda_torch.cpp"), os.path.join(ROOT, "include", "kda_b200.h")]):
+    host = [os.path.join(CSRC, "host", f) for f in os.listdir(os.path.join(CSRC, "host"))]
+    if force or _stale(HOST_LIB, host + [os.path.join(ROOT, "include", "kda_b200.h")]):
         cmd = _host_command()
         if verbose:
             print(" ".join(cmd), flush=True)

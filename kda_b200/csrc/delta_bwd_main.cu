@@ -1,0 +1,340 @@
+// Gated delta rule, one decay per token and head: the gradients of a chunk (see delta.cuh), from the state in front of it (HS), the gradient of the
+// state behind it (DH), v_new (VN) and f (DF).
+//
+// A persistent CTA per SM, a tile per (chunk, head).  Stacked operands, rows 0..63 the keys' and 64..127 the queries':
+//   S  = [K; Q] K^T              G2 = [f; dO] VN^T            (128 x 64 x 128)
+//   Y  = [f; dO] HS^T            Z  = VN DH^T                 (128 x 128 x 128; Z: the upper half counts)
+//   E  = rows 0..63 -beta D G2 (j < i), rows 64..127 scale D G2 (j <= i), with the reciprocal norms of both rows; bf16
+//   D4 = E K                     D5 = E^T [K; Q]              (D5: the upper half counts)
+// so that a thread with a key's row has all of dk's terms in its TMEM lane, and one with a query's row all of dq's.  dG comes from the rows' products
+// with k and q, dbeta from f v, k Y and the sums of a row's dA D <k, k>.  The next tile's HS, DH, VN, f, dO, v are fetched once their products are done, its k and q
+// a tile ahead.
+#include <algorithm>
+
+#include "delta.cuh"
+
+namespace kda {
+namespace delta {
+
+namespace {
+
+constexpr int NT = 9 * 32;      // eight warps (TMEM lane quadrant = warp & 3, column half = warp >> 2) and one that issues products and loads
+
+struct MainSmem {
+  unsigned char E[16384];              // [128][64]; as D5's A its second span is what follows, whose rows of the result nobody reads
+  unsigned char KQ[2][2][16384];
+  unsigned char FD[2][16384];          // [128 rows: f, dO][64 v] x 2
+  unsigned char VN[2][8192];           // (Z's lower half reads beyond: the next span, then v)
+  unsigned char V[2][8192];
+  unsigned char HS[2][16384], DH[2][16384];
+  float vec[2][V_LAST + 4];
+  float red[2][3][C], redq[2][C];      // partial sums over the two column halves: k rows: k (row terms), k (column terms), dbeta; q rows: q dq
+  float redz[8], redh[8];
+  uint64_t fullA[2], fullB, ready, eReady, used, mS, mY, mD;
+  uint32_t tmem_slot;
+  volatile int dead;
+};
+static_assert(sizeof(MainSmem) + 1024 <= 227 * 1024, "MainSmem too large");
+constexpr int T_S = 0, T_G2 = 64, T_D4 = 0, T_Y = 128, T_Z = 256, T_D5 = 384;      // TMEM columns: D4 takes the place of S and G2
+
+__device__ __forceinline__ void store_any(void* p, size_t i, int dtype, float x) {
+  if (dtype == KDA_BF16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(x);
+  else static_cast<float*>(p)[i] = x;
+}
+
+}  // namespace
+
+__global__ void __launch_bounds__(NT, 1) delta_bwd_main_kernel(const __grid_constant__ MainParams p, int spans) {
+  chain_point();
+  extern __shared__ unsigned char smem_raw[];
+  MainSmem& s = *reinterpret_cast<MainSmem*>(smem_raw + pad_to_1024(smem_raw));
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, q4 = warp & 3, half = warp >> 2;
+  const long long total = static_cast<long long>(p.map.total()) * p.H;
+  if (tid == 0) {
+    mbar_init(&s.fullA[0], 1);
+    mbar_init(&s.fullA[1], 1);
+    mbar_init(&s.fullB, 1);
+    mbar_init(&s.ready, 8);
+    mbar_init(&s.eReady, 8);
+    mbar_init(&s.used, 8);
+    mbar_init(&s.mS, 1);
+    mbar_init(&s.mY, 1);
+    mbar_init(&s.mD, 1);
+    s.dead = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0) umma::tmem_alloc(&s.tmem_slot, 512);
+  umma::fence_before_sync();
+  __syncthreads();
+  umma::fence_after_sync();
+  const uint32_t tb = s.tmem_slot, tq = tb + (static_cast<uint32_t>(32 * q4) << 16);
+
+  if (warp < 8) {
+    const int t = 32 * (q4 & 1) + lane;      // this thread's token, of k's rows or of q's; its columns 64 half ..
+    const bool krow = q4 < 2;
+    bool ok = true;
+    int n = 0;
+    for (long long tile = blockIdx.x; tile < total; tile += gridDim.x, ++n) {
+      const ChunkInfo ci = p.map.info(static_cast<int>(tile / p.H));
+      const int h = static_cast<int>(tile % p.H);
+      if (__any_sync(0xffffffffu, s.dead != 0)) { ok = false; break; }
+      if (!(ok = warp_wait(&s.fullA[n & 1], (n >> 1) & 1) && warp_wait(&s.fullB, n & 1))) break;
+      if (ci.len < C) {
+        for (int b = 0; b < 4; ++b) clear_rows(s.KQ[n & 1][b >> 1] + (b & 1) * 8192, ci.len, tid, 256);
+        for (int b = 0; b < 2; ++b) clear_rows(s.FD[b] + 8192, ci.len, tid, 256);
+        fence_proxy_async();
+      }
+      warp_arrive(&s.ready, lane);
+      const float* const vec = s.vec[n & 1];
+      const float vb = vec[V_BETA + t], vk = vec[V_KG + t], vw = vec[V_W + t], vq = vec[V_Q + t], rk = vec[V_RK + t], rq = vec[V_RQ + t];
+      const float gh = vec[V_GHI + t], gl = vec[V_GLO + t];
+      // ---- what needs only the tiles: f v, <h, dh'> ----
+      float fv = 0.f;
+      if (krow && half < spans && t < ci.len) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float x[8], y[8];
+          unpack8(*reinterpret_cast<const uint4*>(piece(s.FD[half], t, e)), x);
+          unpack8(*reinterpret_cast<const uint4*>(piece(s.V[half], t, e)), y);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) fv = fmaf(x[j], y[j], fv);
+        }
+      }
+      float hd = 0.f;
+      for (int b = 0; b < spans; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {      // (the same places of both tiles: their order does not matter)
+          float x[8], y[8];
+          unpack8(*reinterpret_cast<const uint4*>(s.HS[b] + (tid + 256 * e) * 16), x);
+          unpack8(*reinterpret_cast<const uint4*>(s.DH[b] + (tid + 256 * e) * 16), y);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) hd = fmaf(x[j], y[j], hd);
+        }
+      hd = warp_sum(hd);
+      if (lane == 0) s.redh[warp] = hd;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s.used);
+      // ---- E ----
+      if (!(ok = warp_wait(&s.mS, n & 1))) break;
+      umma::fence_after_sync();
+      float bsum = 0.f;
+      {
+        float g2[32];
+        umma::tmem_ld16(tq + T_G2 + 32 * half, *reinterpret_cast<float(*)[16]>(&g2[0]));
+        umma::tmem_ld16(tq + T_G2 + 32 * half + 16, *reinterpret_cast<float(*)[16]>(&g2[16]));
+        umma::tmem_ld_wait();
+        const int last = t < ci.len ? (krow ? t - 1 : t) : -1;
+        const float f = krow ? -rk : p.scale * rq;
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          const int j = 32 * half + e;
+          g2[e] = j <= last ? g2[e] * (f * vec[V_RK + j]) * ex2((gh - vec[V_GHI + j]) + (gl - vec[V_GLO + j])) : 0.f;
+        }
+        if (krow) {
+          float x[32];
+          umma::tmem_ld16(tq + T_S + 32 * half, *reinterpret_cast<float(*)[16]>(&x[0]));
+          umma::tmem_ld16(tq + T_S + 32 * half + 16, *reinterpret_cast<float(*)[16]>(&x[16]));
+          umma::tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            bsum = 32 * half + e <= last ? fmaf(g2[e], x[e], bsum) : bsum;
+            g2[e] *= vb;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) *reinterpret_cast<uint4*>(piece(s.E, 64 * (krow ? 0 : 1) + t, 4 * half + e)) = pack8(&g2[8 * e]);
+      }
+      fence_proxy_async();
+      warp_arrive(&s.eReady, lane);
+      // ---- the rows ----
+      if (!(ok = warp_wait(&s.mY, n & 1) && warp_wait(&s.mD, n & 1))) break;
+      umma::fence_after_sync();
+      const unsigned char* const row = s.KQ[n & 1][half] + (krow ? 0 : 8192);
+      float x[64], da = 0.f, db = 0.f, dy = 0.f, dz = 0.f;
+#pragma unroll
+      for (int e = 0; e < 64; e += 16) {
+        float a[16], b[16], in[16];
+        unpack8(*reinterpret_cast<const uint4*>(piece(row, t, e >> 3)), &in[0]);
+        unpack8(*reinterpret_cast<const uint4*>(piece(row, t, (e >> 3) + 1)), &in[8]);
+        umma::tmem_ld16(tq + T_Y + 64 * half + e, a);
+        umma::tmem_ld16(tq + T_D4 + 64 * half + e, b);
+        umma::tmem_ld_wait();
+        if (krow) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            dy = fmaf(in[j], a[j], dy);
+            x[e + j] = fmaf(-vk, a[j], b[j]);
+            da = fmaf(in[j], x[e + j], da);
+          }
+          umma::tmem_ld16(tq + T_Z + 64 * half + e, a);
+          umma::tmem_ld16(tq + T_D5 + 64 * half + e, b);
+          umma::tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            dz = fmaf(in[j], a[j], dz);
+            const float y = fmaf(vw, a[j], b[j]);
+            db = fmaf(in[j], y, db);
+            x[e + j] += y;
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            x[e + j] = fmaf(vq, a[j], b[j]);
+            da = fmaf(in[j], x[e + j], da);
+          }
+        }
+      }
+      if (krow) {
+        s.red[half][0][t] = da;
+        s.red[half][1][t] = db;
+        s.red[half][2][t] = fv + bsum - ex2(gh + gl) * rk * dy;
+        const float z = warp_sum(t < ci.len ? vw * dz : 0.f);
+        if (lane == 0) s.redz[2 * half + q4] = z;
+      } else {
+        s.redq[half][t] = da;
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (p.use_l2norm) {      // through the normalisation: what lies along the row itself falls out
+        const float d = krow ? (s.red[0][0][t] + s.red[1][0][t] + s.red[0][1][t] + s.red[1][1][t]) * rk * rk : (s.redq[0][t] + s.redq[1][t]) * rq * rq;
+#pragma unroll
+        for (int e = 0; e < 64; e += 8) {
+          float in[8];
+          unpack8(*reinterpret_cast<const uint4*>(piece(row, t, e >> 3)), in);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[e + j] = fmaf(-d, in[j], x[e + j]);
+        }
+      }
+      if (t < ci.len) {
+        __nv_bfloat16* const out = (krow ? p.dk : p.dq) + (static_cast<size_t>(ci.tok0 + t) * p.H + h) * p.kc;
+#pragma unroll
+        for (int e = 0; e < 64; e += 8)
+          if (64 * half + e < p.kc) *reinterpret_cast<uint4*>(out + 64 * half + e) = pack8(&x[e]);
+      }
+      if (warp == 0) {      // dg: the sum of dG from a token to the chunk's end, two tokens a lane
+        float tail = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) tail += s.redh[j];
+        tail = tail * vec[V_LAST] + s.redz[0] + s.redz[1] + s.redz[2] + s.redz[3];
+        float d[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int r = 2 * lane + j;
+          d[j] = r < ci.len ? s.redq[0][r] + s.redq[1][r] + s.red[0][0][r] + s.red[1][0][r] - s.red[0][1][r] - s.red[1][1][r] : 0.f;
+        }
+        float sum = d[0] + d[1];
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+          const float y = __shfl_down_sync(0xffffffffu, sum, off);
+          if (lane + off < 32) sum += y;
+        }
+        // sum: over this lane's two tokens and all behind them
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int r = 2 * lane + j;
+          if (r < ci.len) {
+            const size_t at = static_cast<size_t>(ci.tok0 + r) * p.H + h;
+            store_any(p.dg, at, p.g_dtype, (j ? sum - d[0] : sum) + tail);
+            store_any(p.dbeta, at, p.beta_dtype, s.red[0][2][r] + s.red[1][2][r]);
+          }
+        }
+      }
+      umma::fence_before_sync();
+      asm volatile("bar.sync 1, 256;" ::: "memory");      // the sums are read before the next tile's are written
+    }
+    if (!ok) {
+      s.dead = 1;
+      if (lane == 0) atomicOr(p.status, KDA_STATUS_BWD_MAIN_MMA_WAIT);
+    }
+  } else {
+    if (lane == 0) {
+      auto loadA = [&](long long tile, int n) {
+        const ChunkInfo ci = p.map.info(static_cast<int>(tile / p.H));
+        const int h = static_cast<int>(tile % p.H), hq = h / p.grp, tok0 = static_cast<int>(ci.tok0), b = n & 1;
+        mbar_expect_tx(&s.fullA[b], 4 * 8192 + VEC_COPY);
+        for (int x = 0; x < 2; ++x) tma_load_rows(s.KQ[b][x], &p.tm_k, 64 * x, hq, tok0, &s.fullA[b]);
+        for (int x = 0; x < 2; ++x) tma_load_rows(s.KQ[b][x] + 8192, &p.tm_q, 64 * x, hq, tok0, &s.fullA[b]);
+        bulk_g2s(s.vec[b], p.VEC + static_cast<size_t>(tile) * T_VEC, VEC_COPY, &s.fullA[b]);
+      };
+      auto loadB = [&](long long tile) {
+        const ChunkInfo ci = p.map.info(static_cast<int>(tile / p.H));
+        const int h = static_cast<int>(tile % p.H), tok0 = static_cast<int>(ci.tok0);
+        const size_t at = static_cast<size_t>(tile);
+        mbar_expect_tx(&s.fullB, spans * (4 * 8192 + 2 * 16384));
+        for (int x = 0; x < spans; ++x) {
+          bulk_g2s(s.FD[x], p.DF + at * T_VN + x * 8192, 8192, &s.fullB);
+          bulk_g2s(s.VN[x], p.VN + at * T_VN + x * 8192, 8192, &s.fullB);
+          tma_load_rows(s.FD[x] + 8192, &p.tm_do, 64 * x, h, tok0, &s.fullB);
+          tma_load_rows(s.V[x], &p.tm_v, 64 * x, h, tok0, &s.fullB);
+          bulk_g2s(s.HS[x], p.HS + at * T_STATE + x * 16384, 16384, &s.fullB);
+          bulk_g2s(s.DH[x], p.DH + at * T_STATE + x * 16384, 16384, &s.fullB);
+        }
+      };
+      constexpr uint32_t idS = umma::instr_desc(128, 64, false, false), idY = umma::instr_desc(128, 128, false, false),
+                         id4 = umma::instr_desc(128, 128, false, true), id5 = umma::instr_desc(128, 128, true, true);
+      bool ok = true;
+      int n = 0;
+      if (blockIdx.x < total) {
+        loadA(blockIdx.x, 0);
+        loadB(blockIdx.x);
+      }
+      for (long long tile = blockIdx.x; tile < total; tile += gridDim.x, ++n) {
+        const long long next = tile + gridDim.x;
+        const uint32_t aK = smem_u32(s.KQ[n & 1][0]), aE = smem_u32(s.E);
+        if (s.dead || !mbar_wait(&s.fullA[n & 1], (n >> 1) & 1) || !mbar_wait(&s.fullB, n & 1) || !mbar_wait(&s.ready, n & 1)) { ok = false; break; }
+        umma::fence_after_sync();
+#pragma unroll 1
+        for (int b = 0; b < 2; ++b) {
+          const uint64_t d = umma::desc_kmajor(aK + 16384 * b, 0);
+          umma::mma4<umma::KSTEP_KMAJOR, umma::KSTEP_KMAJOR>(tb + T_S, d, d, idS, b);
+        }
+#pragma unroll 1
+        for (int b = 0; b < spans; ++b)
+          umma::mma4<umma::KSTEP_KMAJOR, umma::KSTEP_KMAJOR>(tb + T_G2, umma::desc_kmajor(smem_u32(s.FD[b]), 0), umma::desc_kmajor(smem_u32(s.VN[b]), 0), idS, b);
+        umma::commit(&s.mS);
+#pragma unroll 1
+        for (int b = 0; b < spans; ++b) {
+          umma::mma4<umma::KSTEP_KMAJOR, umma::KSTEP_KMAJOR>(tb + T_Y, umma::desc_kmajor(smem_u32(s.FD[b]), 0), umma::desc_kmajor(smem_u32(s.HS[b]), 0), idY, b);
+          umma::mma4<umma::KSTEP_KMAJOR, umma::KSTEP_KMAJOR>(tb + T_Z, umma::desc_kmajor(smem_u32(s.VN[b]), 0), umma::desc_kmajor(smem_u32(s.DH[b]), 0), idY, b);
+        }
+        umma::commit(&s.mY);
+        if (next < total) loadA(next, n + 1);      // (everybody is past the tile before: `ready`)
+        if (!mbar_wait(&s.eReady, n & 1)) { ok = false; break; }
+        umma::fence_after_sync();
+        umma::mma4<umma::KSTEP_KMAJOR, umma::KSTEP_MNMAJOR>(tb + T_D4, umma::desc_kmajor(aE, 0), umma::desc_mnmajor(aK, 0, 16384), id4, 0);
+#pragma unroll 1
+        for (int b = 0; b < 2; ++b)      // E's rows 0..63 with K's, 64..127 with Q's: one run of 128 rows in both
+          umma::mma4<umma::KSTEP_MNMAJOR, umma::KSTEP_MNMAJOR>(tb + T_D5, umma::desc_mnmajor(aE, 4 * b, 16384), umma::desc_mnmajor(aK, 4 * b, 16384), id5, b);
+        umma::commit(&s.mD);
+        if (next < total) {
+          if (!mbar_wait(&s.mY, n & 1) || !mbar_wait(&s.used, n & 1)) { ok = false; break; }
+          loadB(next);
+        }
+      }
+      if (!ok) {
+        s.dead = 1;
+        atomicOr(p.status, KDA_STATUS_BWD_MAIN_LOAD_WAIT);
+      }
+    }
+    __syncwarp();
+  }
+  __syncthreads();
+  if (tid == 0 && s.dead) {      // somebody gave up: loads and products may still be under way
+    uint64_t* const all[] = {&s.fullA[0], &s.fullA[1], &s.fullB, &s.mS, &s.mY, &s.mD};
+    for (uint64_t* b : all) mbar_drain(b);
+  }
+  umma::fence_before_sync();
+  __syncthreads();
+  if (warp == 0) umma::tmem_dealloc(tb, 512);
+}
+
+int launch_bwd_main(const MainParams& p, long long tiles, int spans, cudaStream_t st) {
+  static DeviceOnce once;
+  const int smem = static_cast<int>(sizeof(MainSmem)) + 1024;
+  const int rc = once.run([&] { return cudaFuncSetAttribute(delta_bwd_main_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
+  if (rc != KDA_OK) return rc;
+  const unsigned grid = static_cast<unsigned>(std::min<long long>(tiles, sm_count()));
+  return static_cast<int>(launch_chained(delta_bwd_main_kernel, grid, NT, smem, st, p, spans));
+}
+
+}  // namespace delta
+}  // namespace kda

@@ -119,7 +119,8 @@ struct Sizes {
   int64_t B, T, HQ, H, K, V;      // H counts value heads; q and k have HQ
 };
 // The operators' common argument checks (types and texts as documented in kda_b200/ops.py).
-Sizes check_common(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& beta, const Tensor& h0, const Tensor& cu) {
+// per_head: one decay per token and head, g [B, T, HV] (the gated delta rule's operators).
+Sizes check_common(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& beta, const Tensor& h0, const Tensor& cu, bool per_head = false) {
   KDA_REQUIRE(q.is_cuda(), PyExc_RuntimeError, "kda_b200 runs on CUDA (sm_100a) tensors only; there is no CPU path");
   KDA_REQUIRE(q.dim() == 4 && v.dim() == 4, PyExc_ValueError, "q, k, v must be [B, T, H, D], got q=", q.sizes(), " v=", v.sizes());
   const Sizes s{q.size(0), q.size(1), q.size(2), v.size(2), q.size(3), v.size(3)};
@@ -128,7 +129,9 @@ Sizes check_common(const Tensor& q, const Tensor& k, const Tensor& v, const Tens
               "), but got HV % H = ", s.HQ > 0 ? s.H % s.HQ : 0);
   KDA_REQUIRE(s.K <= 256, PyExc_AssertionError, "Currently we only support key headdim <=256 for KDA, got ", s.K, ".");
   KDA_REQUIRE(v.size(0) == s.B && v.size(1) == s.T, PyExc_AssertionError, "v must have shape [B, T, HV, V], got ", v.sizes());
-  KDA_REQUIRE((g.sizes() == at::IntArrayRef{s.B, s.T, s.H, s.K}), PyExc_AssertionError, "g must have shape [B, T, HV, K]=[", s.B, ", ", s.T, ", ", s.H, ", ", s.K,
+  if (per_head) {
+    KDA_REQUIRE((g.sizes() == at::IntArrayRef{s.B, s.T, s.H}), PyExc_AssertionError, "g must have shape [B, T, HV]=[", s.B, ", ", s.T, ", ", s.H, "], got ", g.sizes());
+  } else KDA_REQUIRE((g.sizes() == at::IntArrayRef{s.B, s.T, s.H, s.K}), PyExc_AssertionError, "g must have shape [B, T, HV, K]=[", s.B, ", ", s.T, ", ", s.H, ", ", s.K,
               "], got ", g.sizes());
   KDA_REQUIRE((beta.sizes() == at::IntArrayRef{s.B, s.T, s.H}), PyExc_AssertionError, "beta must have shape [B, T, HV]=[", s.B, ", ", s.T, ", ", s.H, "], got ",
               beta.sizes());
@@ -152,43 +155,69 @@ struct RecurrentCall {
   Tensor q, k, v, g, beta, A_log, dt_bias, h0, cu, slots, accepted, out;
   std::optional<double> scale, lower_bound;
   bool output_final = false, inplace = false, l2norm = false, gate = false, beta_sigmoid = false, transposed = false;
+  bool per_head = false;      // one decay per token and head
   bool training = false;      // float32 with gradients: the forward that the backward belongs to,
   Tensor saved;               // and what it leaves for it (undefined: nothing)
 };
 
+// One decay per head: what the kernels take on trust, apart from the numbers in slots and cu_seqlens.
+void check_head_call(const RecurrentCall& c, const Sizes& s) {
+  const at::Device dev = c.q.device();
+  for (const auto& [name, t] : {std::pair{"k", &c.k}, std::pair{"v", &c.v}, std::pair{"g", &c.g}, std::pair{"beta", &c.beta}, std::pair{"initial_state", &c.h0}, std::pair{"out", &c.out}})
+    KDA_REQUIRE(!t->defined() || t->device() == dev, PyExc_ValueError, "kda_b200: `", name, "` is on ", t->device(), ", q on ", dev);
+  const int64_t N = c.cu.defined() ? c.cu.numel() - 1 : s.B, rows = c.transposed ? s.V : s.K, cols = c.transposed ? s.K : s.V;
+  KDA_REQUIRE(s.V % 32 == 0 && (s.K == 32 || s.K == 64 || s.K == 128 || s.K == 256), PyExc_NotImplementedError,
+              "kda_b200: the token-recurrent kernels need K in {32, 64, 128, 256} and V a multiple of 32, got K=", s.K, ", V=", s.V);
+  if (c.h0.defined()) {
+    KDA_REQUIRE(c.h0.scalar_type() == at::kFloat, PyExc_AssertionError, "initial_state must be in float32.");
+    KDA_REQUIRE(c.h0.dim() == 4 && c.h0.size(1) == s.H && c.h0.size(2) == rows && c.h0.size(3) == cols && (c.slots.defined() || c.h0.size(0) == N), PyExc_ValueError,
+                "initial_state must have shape [", c.slots.defined() ? "slots" : "N", ", ", s.H, ", ", rows, ", ", cols, "], got ", c.h0.sizes());
+  }
+  if (c.slots.defined()) {
+    KDA_REQUIRE((c.slots.dim() == 1 || c.slots.dim() == 2) && c.slots.size(0) == N && (c.slots.dim() == 1 || c.cu.defined() || c.slots.size(1) >= s.T), PyExc_ValueError,
+                "ssm_state_indices must be [N] or [N, T], got ", c.slots.sizes());
+    KDA_REQUIRE(!c.cu.defined() || c.slots.dim() == 2, PyExc_ValueError, "ssm_state_indices must be [N, tokens of the longest sequence] with cu_seqlens");
+    KDA_REQUIRE(!c.accepted.defined() || c.accepted.numel() == N, PyExc_ValueError, "num_accepted_tokens must have ", N, " elements");
+  }
+}
+
 std::pair<Tensor, Tensor> recurrent_fwd(RecurrentCall& c) {
-  const Sizes s = check_common(c.q, c.k, c.v, c.g, c.beta, Tensor(), c.cu);
+  const Sizes s = check_common(c.q, c.k, c.v, c.g, c.beta, Tensor(), c.cu, c.per_head);
+  if (c.per_head) check_head_call(c, s);
   KDA_REQUIRE(!c.transposed || s.K == 64 || s.K == 128, PyExc_NotImplementedError, "kda_b200: transpose_state_layout needs K = 64 or 128, got ", s.K);
   const at::Device dev = c.q.device();
   const c10::cuda::CUDAGuard guard(dev);
   kda_recurrent_args a{};
   // the gate activation and the beta sigmoid run inside the recurrent kernels (no separate pass over g and beta)
   Tensor g, beta, A32, b32;
+  if (c.per_head) a.g_raw_dtype = dtype_code(known_dtype(c.g) ? c.g : (c.g = f32(c.g)));
   if (c.gate) {
     KDA_REQUIRE(c.A_log.defined(), PyExc_AssertionError, "A_log must be provided when use_gate_in_kernel=True.");
     g = known_dtype(c.g) ? dense(c.g) : f32(c.g);
     A32 = f32(c.A_log.device() == dev ? c.A_log : c.A_log.to(dev));
     b32 = c.dt_bias.defined() ? f32(c.dt_bias.device() == dev ? c.dt_bias : c.dt_bias.to(dev)) : Tensor();
-    KDA_REQUIRE(A32.numel() == s.H && (!b32.defined() || b32.numel() == s.H * s.K), PyExc_ValueError, "A_log must have ", s.H, " elements and dt_bias ", s.H * s.K);
+    const int64_t biases = c.per_head ? s.H : s.H * s.K;
+    KDA_REQUIRE(A32.numel() == s.H && (!b32.defined() || b32.numel() == biases), PyExc_ValueError, "A_log must have ", s.H, " elements and dt_bias ", biases);
     a.A_log = ptr<float>(A32);
     a.dt_bias = ptr<float>(b32);
     a.g_raw_dtype = dtype_code(g);
     a.lower_bound = static_cast<float>(c.lower_bound.value_or(0.0));
     a.use_lower_bound = c.lower_bound.has_value();
   } else {
-    g = f32(c.g);
+    g = c.per_head ? dense(c.g) : f32(c.g);
   }
-  if (c.beta_sigmoid) {
+  if (c.beta_sigmoid || c.per_head) {
     beta = known_dtype(c.beta) ? dense(c.beta) : f32(c.beta);
-    a.beta_sigmoid = 1;
+    a.beta_sigmoid = c.beta_sigmoid;
     a.beta_raw_dtype = dtype_code(beta);
   } else {
     beta = f32(c.beta);
   }
-  const Tensor q = dense(c.q), k = dense(c.k), v = dense(c.v);
+  g = aligned(g, c.per_head);
+  const Tensor q = aligned(dense(c.q), c.per_head), k = aligned(dense(c.k), c.per_head), v = aligned(dense(c.v), c.per_head);
   const Tensor cu = i32(c.cu, dev);
   const int64_t N = cu.defined() ? cu.numel() - 1 : s.B;
-  const Tensor h0 = dense(c.h0);
+  const Tensor h0 = aligned(dense(c.h0), c.per_head && !c.inplace);
   Tensor ht;
   if (c.inplace) {
     KDA_REQUIRE(c.h0.defined(), PyExc_AssertionError, "inplace_final_state needs an initial_state");
@@ -227,7 +256,8 @@ std::pair<Tensor, Tensor> recurrent_fwd(RecurrentCall& c) {
     else check_rc(kda_recurrent_walk_fwd(&a, stream_of(dev)), "kda_recurrent_walk_fwd");
     return {o, ht};
   }
-  check_rc(kda_recurrent_fwd(&a, stream_of(dev)), "kda_recurrent_fwd");
+  if (c.per_head) check_rc(kda_delta_recurrent_fwd(&a, stream_of(dev)), "kda_delta_recurrent_fwd");
+  else check_rc(kda_recurrent_fwd(&a, stream_of(dev)), "kda_recurrent_fwd");
   if (checked_mode()) {
     uint32_t st = 0;
     check_rc(kda_recurrent_status(&st), "kda_recurrent_status");
@@ -472,6 +502,8 @@ bool chunk_kda(ChunkCall& c, Tensor& o, Tensor& ht) {
   return true;
 }
 
+#include "kda_delta_norm.h"
+
 // ======================================================================================================================
 // CPython functions
 // ======================================================================================================================
@@ -517,7 +549,7 @@ PyObject* wrap(const Tensor& t) {
   }                                                 \
   END_HANDLE_TH_ERRORS
 
-PyObject* py_recurrent_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+PyObject* recurrent_call(PyObject* const* a, Py_ssize_t n, bool per_head) {
   KDA_BEGIN
   KDA_REQUIRE(n == 20 || n == 21, PyExc_TypeError, "recurrent_fwd takes 20 or 21 arguments");
   RecurrentCall c;
@@ -527,6 +559,7 @@ PyObject* py_recurrent_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
   c.slots = tensor_arg(a[12], "ssm_state_indices"); c.accepted = tensor_arg(a[13], "num_accepted_tokens"); c.l2norm = bool_arg(a[14]);
   c.gate = bool_arg(a[15]); c.beta_sigmoid = bool_arg(a[16]); c.lower_bound = double_arg(a[17]); c.out = tensor_arg(a[18], "out");
   c.transposed = bool_arg(a[19]);
+  c.per_head = per_head;
   c.training = n == 21;
   if (c.training) c.saved = tensor_arg(a[20], "saved");
   std::pair<Tensor, Tensor> r;
@@ -536,6 +569,65 @@ PyObject* py_recurrent_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
     r = recurrent_fwd(c);
   }
   return pair(wrap(r.first), wrap(r.second));
+  KDA_END
+}
+
+PyObject* py_recurrent_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) { return recurrent_call(a, n, false); }
+PyObject* py_delta_recurrent_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 20) {
+    PyErr_SetString(PyExc_TypeError, "delta_recurrent_fwd takes 20 arguments");
+    return nullptr;
+  }
+  return recurrent_call(a, n, true);
+}
+
+PyObject* py_chunk_delta(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  KDA_BEGIN
+  KDA_REQUIRE(n == 12, PyExc_TypeError, "chunk_delta takes 12 arguments");
+  DeltaCall c;
+  c.q = need_arg(a[0], "q"); c.k = need_arg(a[1], "k"); c.v = need_arg(a[2], "v"); c.g = need_arg(a[3], "g"); c.beta = need_arg(a[4], "beta");
+  c.h0 = tensor_arg(a[5], "initial_state"); c.scale = double_arg(a[6]); c.output_final = bool_arg(a[7]); c.cu = tensor_arg(a[8], "cu_seqlens");
+  c.l2norm = bool_arg(a[9]); c.transposed = bool_arg(a[10]); c.slices = static_cast<int>(double_arg(a[11]).value_or(0));
+  Tensor o, ht;
+  bool done;
+  {
+    GilRelease nogil;
+    done = chunk_delta(c, o, ht);
+  }
+  if (!done) Py_RETURN_NONE;
+  return pair(wrap(o), wrap(ht));
+  KDA_END
+}
+
+PyObject* py_gated_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  KDA_BEGIN
+  KDA_REQUIRE(n == 5, PyExc_TypeError, "gated_norm takes 5 arguments");
+  const Tensor x = need_arg(a[0], "x"), gate = need_arg(a[1], "gate"), weight = tensor_arg(a[2], "weight");
+  const double eps = double_arg(a[3]).value_or(0), act = double_arg(a[4]).value_or(0);
+  Tensor y;
+  {
+    GilRelease nogil;
+    y = gated_norm(x, gate, weight, eps, static_cast<int>(act));
+  }
+  return wrap(y);
+  KDA_END
+}
+
+PyObject* py_residual_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  KDA_BEGIN
+  KDA_REQUIRE(n == 6, PyExc_TypeError, "residual_norm takes 6 arguments");
+  const Tensor x = need_arg(a[0], "x"), residual = need_arg(a[1], "residual"), weight = need_arg(a[2], "weight"), post = tensor_arg(a[4], "post_weight");
+  Tensor scale;
+  double value = 1.0;
+  if (THPVariable_Check(a[3])) scale = THPVariable_Unpack(a[3]);
+  else value = double_arg(a[3]).value_or(1.0);
+  const double eps = double_arg(a[5]).value_or(0);
+  Tensor y, r;
+  {
+    GilRelease nogil;
+    std::tie(y, r) = residual_norm(x, residual, weight, scale, value, post, eps);
+  }
+  return pair(wrap(y), wrap(r));
   KDA_END
 }
 
@@ -572,6 +664,10 @@ PyObject* py_set_errors(PyObject*, PyObject* args) {
 PyMethodDef methods[] = {
     {"recurrent_fwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_recurrent_fwd)), METH_FASTCALL, "decode / token-recurrent forward"},
     {"chunk_kda", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_chunk_kda)), METH_FASTCALL, "chunked forward with autograd; None: not this path"},
+    {"delta_recurrent_fwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_delta_recurrent_fwd)), METH_FASTCALL, "the same, one decay per head"},
+    {"chunk_delta", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_chunk_delta)), METH_FASTCALL, "chunked gated delta rule, one decay per head; None: not this path"},
+    {"gated_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_gated_norm)), METH_FASTCALL, "RMS norm with a gate"},
+    {"residual_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_residual_norm)), METH_FASTCALL, "scaled sum at the residual stream, with norms"},
     {"set_errors", py_set_errors, METH_VARARGS, "exception type and status reporter of kda_b200._lib"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_kda_torch", "host path of the kda_b200 operators", -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -127,6 +127,9 @@ inline ChunkMap chunk_map(const ChunkWs& w, const int32_t* cu, int64_t tokens, i
   return m;
 }
 
+// fills the tables of a packed call and its status word (kda_chunk_fwd.cu)
+void launch_tables(const int32_t* cu, int N, int64_t tokens, int max_chunks, int* off, int* seq, int* order, unsigned* status, cudaStream_t st);
+
 // byte offset of element (v, k) of a [128 v][128 k] state tile: span k/64, then the 128-byte-row swizzle
 __device__ __forceinline__ uint32_t vk_off(int v, int k) { return (static_cast<uint32_t>(k >> 6) << 14) + swz<128>(v, k & 63); }
 

@@ -141,8 +141,8 @@ int validate_chunk_args(const kda_chunk_args& a, bool backward) {
   return KDA_OK;
 }
 
-static void launch_tables(const kda_chunk_args& a, int max_chunks, int* off, int* seq, int* order, unsigned* status, cudaStream_t st) {
-  kda_chunk_tables_kernel<<<1, 1024, 0, st>>>(a.cu_seqlens, a.N, a.tokens, max_chunks, off, seq, order, status);
+void launch_tables(const int32_t* cu, int N, int64_t tokens, int max_chunks, int* off, int* seq, int* order, unsigned* status, cudaStream_t st) {
+  kda_chunk_tables_kernel<<<1, 1024, 0, st>>>(cu, N, tokens, max_chunks, off, seq, order, status);
 }
 
 }  // namespace kda
@@ -182,7 +182,7 @@ extern "C" int kda_chunk_fwd(const kda_chunk_args* args, void* stream) {
   ProfCall* prof = prof_begin(st);
   const ChunkMap map = chunk_map(w, a.cu_seqlens, a.tokens, a.N);
   if (a.cu_seqlens) {
-    launch_tables(a, NTmax, w.seq_chunk_off, w.chunk_seq, w.seq_order, w.status, st);
+    launch_tables(a.cu_seqlens, a.N, a.tokens, NTmax, w.seq_chunk_off, w.chunk_seq, w.seq_order, w.status, st);
     if ((e = cudaGetLastError()) != cudaSuccess) return static_cast<int>(e);
   }
   prof_mark(prof, KDA_STAGE_TABLES, st);

@@ -66,6 +66,19 @@ __device__ __forceinline__ float recurrent_beta(const kda_recurrent_args& a, siz
   return a.beta_sigmoid ? sigmoid_fast(load_raw(a.beta, row, a.beta_raw_dtype)) : a.beta[row];
 }
 
+// the same with one decay per token and head
+__device__ __forceinline__ float recurrent_head_decay(const kda_recurrent_args& a, size_t row, int h) {
+  float x = load_raw(a.g, row, a.g_raw_dtype);
+  if (!a.A_log) return x;
+  if (a.dt_bias) x += a.dt_bias[h];
+  const float al = __expf(a.A_log[h]);
+  return a.use_lower_bound ? a.lower_bound * sigmoid_fast(al * x) : -al * softplus_fast(x);
+}
+__device__ __forceinline__ float recurrent_head_beta(const kda_recurrent_args& a, size_t row) {
+  const float x = load_raw(a.beta, row, a.beta_raw_dtype);
+  return a.beta_sigmoid ? sigmoid_fast(x) : x;
+}
+
 // ---- tensor-core primitives (warp-level, bf16 in / fp32 accumulate) ------------------------------
 // D(16x8) += A(16x16, row) * B(16x8, col).  Fragment ownership (gid = lane/4, tig = lane%4):
 //   a0:(gid, 2tig..+1) a1:(gid+8, 2tig..) a2:(gid, 2tig+8..) a3:(gid+8, 2tig+8..)

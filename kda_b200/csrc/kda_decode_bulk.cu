@@ -96,7 +96,8 @@ struct Pos {
 // TR: the states are [slots, H, V, K] (fla's transpose_state_layout): a unit is HV contiguous value rows, a warp owns 16 of them and a
 // lane four key columns, so both sums over K stay inside the warp (two butterflies).
 // GATE: g and / or beta are the raw layer outputs and are activated here (see kda_recurrent_args::A_log, beta_sigmoid).
-template <typename IO, bool TR, bool GATE, int HV>
+// HEAD (with GATE): one decay per token and head, g and beta of either type (kda_delta_recurrent_fwd).
+template <typename IO, bool TR, bool GATE, int HV, bool HEAD>
 __global__ void __launch_bounds__(HV * 2 + 32, 128 / HV) kda_decode_bulk_kernel(const __grid_constant__ DecParams p) {
   chain_point();
   extern __shared__ unsigned char smem_raw[];
@@ -225,10 +226,10 @@ __global__ void __launch_bounds__(HV * 2 + 32, 128 / HV) kda_decode_bulk_kernel(
     }
     if (has_gv) {
       if constexpr (GATE) {
-        r.x[RG] = ld_bits(a.g, row * DK + e, a.A_log && a.g_raw_dtype == KDA_BF16);
+        r.x[RG] = ld_bits(a.g, HEAD ? row : row * DK + e, (HEAD || a.A_log) && a.g_raw_dtype == KDA_BF16);
         if (a.A_log) {
           r.x[RA] = __float_as_uint(a.A_log[q.h]);
-          r.x[RBIAS] = a.dt_bias ? __float_as_uint(a.dt_bias[static_cast<size_t>(q.h) * DK + e]) : 0u;
+          r.x[RBIAS] = a.dt_bias ? __float_as_uint(a.dt_bias[HEAD ? q.h : static_cast<size_t>(q.h) * DK + e]) : 0u;
         }
       } else {
         r.x[RG] = __float_as_uint(a.g[row * DK + e]);
@@ -236,7 +237,7 @@ __global__ void __launch_bounds__(HV * 2 + 32, 128 / HV) kda_decode_bulk_kernel(
       if (e < HV) r.x[RV] = ld_bits(a.v, row * DV + half * HV + e, IO16);
     }
     if (tid == 0) {
-      if constexpr (GATE) r.x[RB] = ld_bits(a.beta, row, a.beta_sigmoid && a.beta_raw_dtype == KDA_BF16);
+      if constexpr (GATE) r.x[RB] = ld_bits(a.beta, row, (HEAD || a.beta_sigmoid) && a.beta_raw_dtype == KDA_BF16);
       else r.x[RB] = __float_as_uint(a.beta[row]);
     }
   };
@@ -254,7 +255,7 @@ __global__ void __launch_bounds__(HV * 2 + 32, 128 / HV) kda_decode_bulk_kernel(
       }
     }
     if (has_gv) {
-      float g = __uint_as_float(r.x[RG]);
+      float g = to_float(r.x[RG], HEAD && a.g_raw_dtype == KDA_BF16);
       if constexpr (GATE) {
         if (a.A_log) {
           const float x = to_float(r.x[RG], a.g_raw_dtype == KDA_BF16) + __uint_as_float(r.x[RBIAS]);
@@ -266,7 +267,7 @@ __global__ void __launch_bounds__(HV * 2 + 32, 128 / HV) kda_decode_bulk_kernel(
       if (e < HV) s.vv[buf][e] = to_float(r.x[RV], IO16);
     }
     if (tid == 0) {
-      float b = __uint_as_float(r.x[RB]);
+      float b = to_float(r.x[RB], HEAD && a.beta_raw_dtype == KDA_BF16);
       if constexpr (GATE) {
         if (a.beta_sigmoid) b = sigmoid_fast(to_float(r.x[RB], a.beta_raw_dtype == KDA_BF16));
       }
@@ -440,12 +441,12 @@ __global__ void __launch_bounds__(HV * 2 + 32, 128 / HV) kda_decode_bulk_kernel(
 
 namespace {
 
-template <typename IO, bool TR, bool GATE, int HV>
+template <typename IO, bool TR, bool GATE, int HV, bool HEAD>
 int launch_hv(const kda_recurrent_args& a, cudaStream_t st) {
   const int smem = static_cast<int>(sizeof(DecSmem<HV>)) + 128;
   static DeviceOnce once;      // per template variant, per device
   const int rc = once.run([&] {
-    return cudaFuncSetAttribute(kda_decode_bulk_kernel<IO, TR, GATE, HV>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    return cudaFuncSetAttribute(kda_decode_bulk_kernel<IO, TR, GATE, HV, HEAD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   });
   if (rc != KDA_OK) return rc;
   constexpr int PARTS = DV / HV;
@@ -456,15 +457,15 @@ int launch_hv(const kda_recurrent_args& a, cudaStream_t st) {
   p.dn = p.step / PARTS / a.H;
   p.dh = p.step / PARTS % a.H;
   if (!TR && HV != DV && (make_states_tmap(&p.tm_in, a.h0, DV, HV, DK) || make_states_tmap(&p.tm_out, a.ht, DV, HV, DK))) return KDA_E_TMAP;
-  return static_cast<int>(launch_chained(kda_decode_bulk_kernel<IO, TR, GATE, HV>, static_cast<unsigned>(p.step), HV * 2 + 32, smem, st, p));
+  return static_cast<int>(launch_chained(kda_decode_bulk_kernel<IO, TR, GATE, HV, HEAD>, static_cast<unsigned>(p.step), HV * 2 + 32, smem, st, p));
 }
 
-template <typename IO, bool TR, bool GATE>
+template <typename IO, bool TR, bool GATE, bool HEAD = false>
 int launch(const kda_recurrent_args& a, cudaStream_t st) {
   if constexpr (TR || GATE) {
-    if (a.T == 1) return launch_hv<IO, TR, GATE, 128>(a, st);
+    if (a.T == 1) return launch_hv<IO, TR, GATE, 128, HEAD>(a, st);
   }
-  return launch_hv<IO, TR, GATE, 64>(a, st);
+  return launch_hv<IO, TR, GATE, 64, HEAD>(a, st);
 }
 
 }  // namespace
@@ -482,7 +483,11 @@ bool decode_bulk_covers(const kda_recurrent_args& a) {
   return states >= KDA_DECODE_BULK_MIN_UNITS_PER_SM * static_cast<long long>(sm_count()) && states <= 0x3fffffff;
 }
 
-int decode_bulk_launch(const kda_recurrent_args& a, cudaStream_t st) {
+int decode_bulk_launch(const kda_recurrent_args& a, bool per_head, cudaStream_t st) {
+  if (per_head) {
+    if (a.io_dtype == KDA_BF16) return a.transpose_state ? launch<__nv_bfloat16, true, true, true>(a, st) : launch<__nv_bfloat16, false, true, true>(a, st);
+    return a.transpose_state ? launch<float, true, true, true>(a, st) : launch<float, false, true, true>(a, st);
+  }
   // One token, states [K, V]: the variant with gates also serves the calls without.  At the copy rate it is when the loads and stores of the SMs
   // meet in DRAM that decides, and that variant's steps fall better (without gates, us, its own variant | this one: 148 sequences x 32 heads
   // 102.0 | 100.5, 512: 340 | 334, 1,024: 666 | 657, 1,500: 978 | 962).  States [V, K]: its own is better (1,024: 655 | 680).

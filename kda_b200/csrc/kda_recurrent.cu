@@ -88,7 +88,8 @@ struct RowBits {
 
 // A token's vectors are fetched while the token before is worked on: with one warp per slice there is nobody else to hide
 // their latency (one sequence of four draft tokens: 14.2 us when each token fetched its own, 8.0 us so).
-template <typename IO, int K, int VS>
+// HEAD: one decay per token and head (kda_delta_recurrent_fwd).
+template <typename IO, int K, int VS, bool HEAD>
 __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_kernel(const kda_recurrent_args a) {
   chain_point();
   constexpr int CL = VS / 4;      // lanes across the V slice (4 columns each)
@@ -98,7 +99,7 @@ __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_kernel(const kda
   constexpr bool IO16 = sizeof(IO) == 2;
   static_assert(K % RG == 0 && K % 32 == 0, "unsupported K");
 
-  __shared__ float s_k[REC_WARPS][K], s_q[REC_WARPS][K], s_eg[REC_WARPS][K];
+  __shared__ float s_k[REC_WARPS][K], s_q[REC_WARPS][K], s_eg[REC_WARPS][HEAD ? 1 : K];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int nvs = a.V / VS;
@@ -120,9 +121,11 @@ __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_kernel(const kda
     bos = static_cast<long long>(n) * a.T;
     eos = bos + a.T;
   }
-  const bool g16 = a.A_log && a.g_raw_dtype == KDA_BF16, b16 = a.beta_sigmoid && a.beta_raw_dtype == KDA_BF16;
+  const bool g16 = (HEAD || a.A_log) && a.g_raw_dtype == KDA_BF16, b16 = (HEAD || a.beta_sigmoid) && a.beta_raw_dtype == KDA_BF16;
+  constexpr int EG = HEAD ? 1 : E;      // g elements per lane
   struct Token {
-    RowBits<E> q, k, g;
+    RowBits<E> q, k;
+    RowBits<EG> g;
     RowBits<4> v;
     RowBits<1> b;
   };
@@ -131,7 +134,7 @@ __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_kernel(const kda
     const size_t row = static_cast<size_t>(t) * a.H + h;
     x.q.load(a.q, rowq, IO16);
     x.k.load(a.k, rowq, IO16);
-    x.g.load(a.g, row * K + lane * E, g16);
+    x.g.load(a.g, HEAD ? row : row * K + lane * E, g16);
     x.b.load(a.beta, row, b16);
     x.v.load(a.v, row * a.V + col, IO16);
   };
@@ -140,9 +143,9 @@ __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_kernel(const kda
   const long long slot = slots ? slots[a.num_accepted_tokens ? a.num_accepted_tokens[n] - 1 : 0] : n;
   Token cur, nxt;
   if (bos < eos) fetch(bos, cur);
-  float bias[E], al = 0.f;
+  float bias[EG], al = 0.f, decay = 1.f;
 #pragma unroll
-  for (int e = 0; e < E; ++e) bias[e] = a.dt_bias ? a.dt_bias[static_cast<size_t>(h) * K + lane * E + e] : 0.f;
+  for (int e = 0; e < EG; ++e) bias[e] = a.dt_bias ? a.dt_bias[HEAD ? h : static_cast<size_t>(h) * K + lane * E + e] : 0.f;
   if (a.A_log) al = __expf(a.A_log[h]);
   const size_t sbase = (static_cast<size_t>(slot) * a.H + h) * K * a.V + col;
 
@@ -164,12 +167,14 @@ __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_kernel(const kda
     for (int e = 0; e < E; ++e) {
       qf[e] = cur.q.get(e, IO16);
       kf[e] = cur.k.get(e, IO16);
-      float g = cur.g.get(e, g16);
+      if (HEAD && e > 0) continue;
+      float g = cur.g.get(HEAD ? 0 : e, g16);
       if (a.A_log) {
-        g += bias[e];
+        g += bias[HEAD ? 0 : e];
         g = a.use_lower_bound ? a.lower_bound * sigmoid_fast(al * g) : -al * softplus_fast(g);
       }
-      s_eg[warp][lane * E + e] = expf(g);
+      if constexpr (HEAD) decay = expf(g);
+      else s_eg[warp][lane * E + e] = expf(g);
     }
     float qs = a.scale;
     if (a.use_qk_l2norm) {
@@ -200,7 +205,7 @@ __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_kernel(const kda
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       const int r = rg + RG * i;
-      const float eg = s_eg[warp][r], kk = s_k[warp][r];
+      const float eg = HEAD ? decay : s_eg[warp][r], kk = s_k[warp][r];
       S[i].x *= eg; S[i].y *= eg; S[i].z *= eg; S[i].w *= eg;
       hk.x += kk * S[i].x; hk.y += kk * S[i].y; hk.z += kk * S[i].z; hk.w += kk * S[i].w;
     }
@@ -266,7 +271,7 @@ __device__ __forceinline__ void st_row(float* p, const float (&d)[E]) {
 // lane*(K/32) .. of those rows, so every state access is again contiguous over the warp.  The two reductions over K
 // are per-lane partial dot products summed over the lanes 32 values at a time by a butterfly (lane L ends up with
 // the total of value row L); the delta-rule update needs every row's dv in every lane: one shuffle per row.
-template <typename IO, int K>
+template <typename IO, int K, bool HEAD>
 __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_t_kernel(const kda_recurrent_args a) {
   constexpr int E = K / 32;       // key columns per lane
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -313,7 +318,8 @@ __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_t_kernel(const k
     for (int e = 0; e < E; ++e) {
       qf[e] = IoTraits<IO>::ld(qp + rowq + e);
       kf[e] = IoTraits<IO>::ld(kp + rowq + e);
-      eg[e] = expf(recurrent_log_decay(a, static_cast<size_t>(t) * a.H + h, h, lane * E + e, K));
+      if constexpr (HEAD) eg[e] = e == 0 ? expf(recurrent_head_decay(a, static_cast<size_t>(t) * a.H + h, h)) : eg[0];
+      else eg[e] = expf(recurrent_log_decay(a, static_cast<size_t>(t) * a.H + h, h, lane * E + e, K));
     }
     float qs = a.scale;
     if (a.use_qk_l2norm) {
@@ -332,7 +338,7 @@ __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_t_kernel(const k
     }
 #pragma unroll
     for (int e = 0; e < E; ++e) qf[e] *= qs;
-    const float beta = recurrent_beta(a, static_cast<size_t>(t) * a.H + h);
+    const float beta = HEAD ? recurrent_head_beta(a, static_cast<size_t>(t) * a.H + h) : recurrent_beta(a, static_cast<size_t>(t) * a.H + h);
     const float vt = IoTraits<IO>::ld(vp + (static_cast<size_t>(t) * a.H + h) * a.V + vs * 32 + lane);      // value row `lane`
     float part[32];
 #pragma unroll
@@ -374,51 +380,51 @@ __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_t_kernel(const k
   }
 }
 
-template <typename IO, int K>
+template <typename IO, int K, bool HEAD>
 static int launch_rec_t(const kda_recurrent_args& a, cudaStream_t st) {
   const long long total = static_cast<long long>(a.N) * a.H * (a.V / 32);
   const long long blocks = (total + REC_WARPS - 1) / REC_WARPS;
   if (blocks <= 0) return KDA_OK;
   if (blocks > 0x7fffffffLL) return KDA_E_SHAPE;
-  kda_recurrent_t_kernel<IO, K><<<static_cast<unsigned>(blocks), REC_WARPS * 32, 0, st>>>(a);
+  kda_recurrent_t_kernel<IO, K, HEAD><<<static_cast<unsigned>(blocks), REC_WARPS * 32, 0, st>>>(a);
   return static_cast<int>(cudaGetLastError());
 }
 
-template <typename IO, int K, int VS>
+template <typename IO, int K, int VS, bool HEAD>
 static int launch_rec(const kda_recurrent_args& a, cudaStream_t st) {
   const long long total = static_cast<long long>(a.N) * a.H * (a.V / VS);
   const long long blocks = (total + REC_WARPS - 1) / REC_WARPS;
   if (blocks <= 0) return KDA_OK;
   if (blocks > 0x7fffffffLL) return KDA_E_SHAPE;
-  return static_cast<int>(launch_chained(kda_recurrent_kernel<IO, K, VS>, static_cast<unsigned>(blocks), REC_WARPS * 32, 0, st, a));
+  return static_cast<int>(launch_chained(kda_recurrent_kernel<IO, K, VS, HEAD>, static_cast<unsigned>(blocks), REC_WARPS * 32, 0, st, a));
 }
 
-template <typename IO>
+template <typename IO, bool HEAD>
 static int dispatch_rec(const kda_recurrent_args& a, cudaStream_t st) {
   if (a.transpose_state) {
     switch (a.K) {
-      case 64: return launch_rec_t<IO, 64>(a, st);
-      case 128: return launch_rec_t<IO, 128>(a, st);
+      case 64: return launch_rec_t<IO, 64, HEAD>(a, st);
+      case 128: return launch_rec_t<IO, 128, HEAD>(a, st);
       default: return KDA_E_SHAPE;
     }
   }
   switch (a.K) {
-    case 32: return launch_rec<IO, 32, 32>(a, st);
-    case 64: return launch_rec<IO, 64, 32>(a, st);
+    case 32: return launch_rec<IO, 32, 32, HEAD>(a, st);
+    case 64: return launch_rec<IO, 64, 32, HEAD>(a, st);
     // one or two sequences leave most SMs idle: twice as many warps with half the columns each (one sequence x 32 heads, one token: 3.4
     // instead of 4.3 us; from half a state per SM on the wider slices win: 96 states 4.3 against 4.5 us)
-    case 128: return 2LL * a.N * a.H <= sm_count() ? launch_rec<IO, 128, 16>(a, st) : launch_rec<IO, 128, 32>(a, st);
-    case 256: return (a.V % 32 == 0) ? launch_rec<IO, 256, 16>(a, st) : KDA_E_SHAPE;
+    case 128: return 2LL * a.N * a.H <= sm_count() ? launch_rec<IO, 128, 16, HEAD>(a, st) : launch_rec<IO, 128, 32, HEAD>(a, st);
+    case 256: return (a.V % 32 == 0) ? launch_rec<IO, 256, 16, HEAD>(a, st) : KDA_E_SHAPE;
     default: return KDA_E_SHAPE;
   }
 }
 
 bool decode_bulk_covers(const kda_recurrent_args& a);                    // kda_decode_bulk.cu
-int decode_bulk_launch(const kda_recurrent_args& a, cudaStream_t st);
+int decode_bulk_launch(const kda_recurrent_args& a, bool per_head, cudaStream_t st);
 
 }  // namespace kda
 
-extern "C" int kda_recurrent_fwd(const kda_recurrent_args* args, void* stream) {
+static int recurrent_fwd(const kda_recurrent_args* args, bool per_head, void* stream) {
   if (!args) return KDA_E_NULL;
   kda_recurrent_args a = *args;
   if (a.state_indices) {
@@ -447,8 +453,16 @@ extern "C" int kda_recurrent_fwd(const kda_recurrent_args* args, void* stream) {
                          reinterpret_cast<uintptr_t>(a.ht);
   if (bits & 15u) return KDA_E_ALIGN;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (kda::decode_bulk_covers(a)) return kda::decode_bulk_launch(a, st);
-  if (a.io_dtype == KDA_BF16) return kda::dispatch_rec<__nv_bfloat16>(a, st);
-  if (a.io_dtype == KDA_FP32) return kda::dispatch_rec<float>(a, st);
+  if (kda::decode_bulk_covers(a)) return kda::decode_bulk_launch(a, per_head, st);
+  if (a.io_dtype == KDA_BF16) return per_head ? kda::dispatch_rec<__nv_bfloat16, true>(a, st) : kda::dispatch_rec<__nv_bfloat16, false>(a, st);
+  if (a.io_dtype == KDA_FP32) return per_head ? kda::dispatch_rec<float, true>(a, st) : kda::dispatch_rec<float, false>(a, st);
   return KDA_E_DTYPE;
+}
+
+extern "C" int kda_recurrent_fwd(const kda_recurrent_args* args, void* stream) { return recurrent_fwd(args, false, stream); }
+
+extern "C" int kda_delta_recurrent_fwd(const kda_recurrent_args* args, void* stream) {
+  if (args && ((args->g_raw_dtype != KDA_BF16 && args->g_raw_dtype != KDA_FP32) || (args->beta_raw_dtype != KDA_BF16 && args->beta_raw_dtype != KDA_FP32)))
+    return KDA_E_DTYPE;
+  return recurrent_fwd(args, true, stream);
 }

@@ -98,7 +98,7 @@ struct ScanParams {
   __nv_bfloat16* o;
   unsigned* status;
   int H, grp, kc, vc;
-  alignas(64) CUtensorMap tm_q, tm_k, tm_v;
+  alignas(64) CUtensorMap tm_q, tm_k, tm_v, tm_o;
 };
 struct RScanParams {
   ChunkMap map;
@@ -109,7 +109,7 @@ struct RScanParams {
   __nv_bfloat16* dv;
   unsigned* status;
   int H, grp, kc, vc;
-  alignas(64) CUtensorMap tm_q, tm_k, tm_do;
+  alignas(64) CUtensorMap tm_q, tm_k, tm_do, tm_dv;
 };
 struct MainParams {
   ChunkMap map;
@@ -120,7 +120,7 @@ struct MainParams {
   unsigned* status;
   int H, grp, kc, use_l2norm;
   float scale;
-  alignas(64) CUtensorMap tm_q, tm_k, tm_v, tm_do;
+  alignas(64) CUtensorMap tm_q, tm_k, tm_v, tm_do, tm_dq, tm_dk;
 };
 
 int launch_prepare(const PrepParams& p, long long tiles, cudaStream_t st);

@@ -107,7 +107,7 @@ extern "C" int kda_delta_chunk_fwd(const kda_delta_args* args, void* stream) {
   PrepParams pp{};
   ScanParams sp{};
   if (make_rows_tmap(&pp.tm_q, a.q, false, a.tokens, HQ, a.K, 64, 64, true) || make_rows_tmap(&pp.tm_k, a.k, false, a.tokens, HQ, a.K, 64, 64, true) ||
-      make_rows_tmap(&sp.tm_v, a.v, false, a.tokens, a.H, a.V, 64, 64, true))
+      make_rows_tmap(&sp.tm_v, a.v, false, a.tokens, a.H, a.V, 64, 64, true) || make_rows_tmap(&sp.tm_o, a.o, false, a.tokens, a.H, a.V, 64, 64, true))
     return KDA_E_TMAP;
   sp.tm_q = pp.tm_q; sp.tm_k = pp.tm_k;
   ProfCall* const prof = prof_begin(st);
@@ -155,8 +155,12 @@ extern "C" int kda_delta_chunk_bwd(const kda_delta_args* args, void* stream) {
   const ChunkMap map = chunk_map(cw, a.cu_seqlens, a.tokens, a.N);
   RScanParams rp{};
   MainParams mp{};
+  mp.dq = grp > 1 ? w.DQH : static_cast<__nv_bfloat16*>(a.dq);
+  mp.dk = grp > 1 ? w.DKH : static_cast<__nv_bfloat16*>(a.dk);
   if (make_rows_tmap(&mp.tm_q, a.q, false, a.tokens, HQ, a.K, 64, 64, true) || make_rows_tmap(&mp.tm_k, a.k, false, a.tokens, HQ, a.K, 64, 64, true) ||
-      make_rows_tmap(&mp.tm_v, a.v, false, a.tokens, a.H, a.V, 64, 64, true) || make_rows_tmap(&mp.tm_do, a.d_o, false, a.tokens, a.H, a.V, 64, 64, true))
+      make_rows_tmap(&mp.tm_v, a.v, false, a.tokens, a.H, a.V, 64, 64, true) || make_rows_tmap(&mp.tm_do, a.d_o, false, a.tokens, a.H, a.V, 64, 64, true) ||
+      make_rows_tmap(&mp.tm_dq, mp.dq, false, a.tokens, a.H, a.K, 64, 64, true) || make_rows_tmap(&mp.tm_dk, mp.dk, false, a.tokens, a.H, a.K, 64, 64, true) ||
+      make_rows_tmap(&rp.tm_dv, a.dv, false, a.tokens, a.H, a.V, 64, 64, true))
     return KDA_E_TMAP;
   rp.tm_q = mp.tm_q; rp.tm_k = mp.tm_k; rp.tm_do = mp.tm_do;
   ProfCall* const prof = prof_begin(st);
@@ -165,7 +169,6 @@ extern "C" int kda_delta_chunk_bwd(const kda_delta_args* args, void* stream) {
   if ((rc = delta::launch_bwd_scan(rp, a.N * a.H, a.scan_slices, st)) != KDA_OK) return rc;
   prof_mark(prof, KDA_STAGE_BWD_SCAN, st);
   mp.map = map; mp.VEC = w.VEC; mp.HS = w.HS; mp.VN = w.VN; mp.DH = w.DH; mp.DF = w.DF;
-  mp.dq = grp > 1 ? w.DQH : static_cast<__nv_bfloat16*>(a.dq); mp.dk = grp > 1 ? w.DKH : static_cast<__nv_bfloat16*>(a.dk);
   mp.dg = a.dg; mp.dbeta = a.dbeta; mp.g_dtype = a.g_dtype; mp.beta_dtype = a.beta_dtype; mp.status = w.status; mp.H = a.H; mp.grp = grp; mp.kc = a.K;
   mp.use_l2norm = a.use_qk_l2norm; mp.scale = a.scale;
   const long long chunks = map.T > 0 ? static_cast<long long>(a.N) * map.per_seq : most;

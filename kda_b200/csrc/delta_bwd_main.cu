@@ -8,7 +8,7 @@
 //   D4 = E K                     D5 = E^T [K; Q]              (D5: the upper half counts)
 // so that a thread with a key's row has all of dk's terms in its TMEM lane, and one with a query's row all of dq's.  dG comes from the rows' products
 // with k and q, dbeta from f v, k Y and the sums of a row's dA D <k, k>.  The next tile's HS, DH, VN, f, dO, v are fetched once their products are done, its k and q
-// a tile ahead.
+// a tile ahead; dk and dq of a full chunk leave by TMA from k's and q's rows, which they overwrite.
 #include <algorithm>
 
 #include "delta.cuh"
@@ -204,7 +204,11 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_main_kernel(const __grid_cons
           for (int j = 0; j < 8; ++j) x[e + j] = fmaf(-d, in[j], x[e + j]);
         }
       }
-      if (t < ci.len) {
+      if (ci.len == C) {
+#pragma unroll
+        for (int e = 0; e < 64; e += 8) *reinterpret_cast<uint4*>(const_cast<unsigned char*>(piece(row, t, e >> 3))) = pack8(&x[e]);
+        fence_proxy_async();
+      } else if (t < ci.len) {
         __nv_bfloat16* const out = (krow ? p.dk : p.dq) + (static_cast<size_t>(ci.tok0 + t) * p.H + h) * p.kc;
 #pragma unroll
         for (int e = 0; e < 64; e += 8)
@@ -241,6 +245,7 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_main_kernel(const __grid_cons
       umma::fence_before_sync();
       asm volatile("bar.sync 1, 256;" ::: "memory");      // the sums are read before the next tile's are written
     }
+    if (ok) warp_arrive(&s.ready, lane);                  // the last tile's rows stand in shared memory
     if (!ok) {
       s.dead = 1;
       if (lane == 0) atomicOr(p.status, KDA_STATUS_BWD_MAIN_MMA_WAIT);
@@ -271,6 +276,16 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_main_kernel(const __grid_cons
       };
       constexpr uint32_t idS = umma::instr_desc(128, 64, false, false), idY = umma::instr_desc(128, 128, false, false),
                          id4 = umma::instr_desc(128, 128, false, true), id5 = umma::instr_desc(128, 128, true, true);
+      auto store = [&](long long tile, int n) {      // dk, dq of a full chunk
+        const ChunkInfo ci = p.map.info(static_cast<int>(tile / p.H));
+        if (ci.len < C) return;
+        const int h = static_cast<int>(tile % p.H), tok0 = static_cast<int>(ci.tok0);
+        for (int x = 0; x < 2 && 64 * x < p.kc; ++x) {
+          tma_store_rows(&p.tm_dk, 64 * x, h, tok0, s.KQ[n & 1][x]);
+          tma_store_rows(&p.tm_dq, 64 * x, h, tok0, s.KQ[n & 1][x] + 8192);
+        }
+        bulk_commit();
+      };
       bool ok = true;
       int n = 0;
       if (blockIdx.x < total) {
@@ -297,7 +312,11 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_main_kernel(const __grid_cons
           umma::mma4<umma::KSTEP_KMAJOR, umma::KSTEP_KMAJOR>(tb + T_Z, umma::desc_kmajor(smem_u32(s.VN[b]), 0), umma::desc_kmajor(smem_u32(s.DH[b]), 0), idY, b);
         }
         umma::commit(&s.mY);
-        if (next < total) loadA(next, n + 1);      // (everybody is past the tile before: `ready`)
+        if (n > 0) store(tile - gridDim.x, n - 1);      // everybody is past the tile before: `ready`
+        if (next < total) {
+          bulk_wait_read<0>();
+          loadA(next, n + 1);
+        }
         if (!mbar_wait(&s.eReady, n & 1)) { ok = false; break; }
         umma::fence_after_sync();
         umma::mma4<umma::KSTEP_KMAJOR, umma::KSTEP_MNMAJOR>(tb + T_D4, umma::desc_kmajor(aE, 0), umma::desc_mnmajor(aK, 0, 16384), id4, 0);
@@ -310,10 +329,15 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_main_kernel(const __grid_cons
           loadB(next);
         }
       }
+      if (ok && n > 0) {
+        ok = mbar_wait(&s.ready, n & 1);
+        if (ok) store(blockIdx.x + static_cast<long long>(n - 1) * gridDim.x, n - 1);
+      }
       if (!ok) {
         s.dead = 1;
         atomicOr(p.status, KDA_STATUS_BWD_MAIN_LOAD_WAIT);
       }
+      bulk_wait_read<0>();      // the stores read shared memory that goes with the CTA
     }
     __syncwarp();
   }

@@ -6,6 +6,7 @@
 //   2   Tm^T x                    (M = 64, K = 64;   f = that + Pt^T dO)
 //   3   K^T y                     (M = 128, K = 64;  y = -beta exp(G) f;  dh = exp(G_last) dh' + that + Q^T (scale exp(G) dO))
 // Pt^T dO and Q^T (..) depend on dO alone and run beside the chain.  dh', x, y and the scaled dO are bf16 pairs, hi and lo side by side in one operand.
+// With 64 columns the tiles and full chunks of dv leave by bulk copies: DH from the operand dh', f and dv through operands that are done (dO's tile, the scaled dO's).
 #include "delta.cuh"
 
 namespace kda {
@@ -25,7 +26,7 @@ struct RSmem {
   unsigned char Os[VC == 32 ? 1 : 2][8192];    // scale exp(G) dO: [64 t][hi, lo]
   float vec[2][VEC_COPY / 4];
   uint64_t fullA[2], freeA[2], fullB, freeB;
-  uint64_t hReady, dReady, xReady, yReady, m1, m2, m3;
+  uint64_t hReady, dReady, xReady, yReady, oReady, m1, m2, m3;
   uint32_t tmem_slot;
   volatile int dead;
 };
@@ -49,6 +50,7 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_scan_kernel(const __grid_cons
   chain_point();
   using Smem = RSmem<VC>;
   constexpr int HC = VC / 2, QC = VC / 4;
+  constexpr bool BULK = VC == 64;
   constexpr int D1 = 0, D2 = 2 * VC, D3 = 4 * VC, DO = 6 * VC;
   constexpr uint32_t TM = VC == 32 ? 256 : 512;
   extern __shared__ unsigned char smem_raw[];
@@ -71,6 +73,7 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_scan_kernel(const __grid_cons
     mbar_init(&s.dReady, 8);
     mbar_init(&s.xReady, 8);
     mbar_init(&s.yReady, 8);
+    mbar_init(&s.oReady, 8);
     mbar_init(&s.m1, 1);
     mbar_init(&s.m2, 1);
     mbar_init(&s.m3, 1);
@@ -116,7 +119,7 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_scan_kernel(const __grid_cons
         const Split x = split8(&S[e]);
         put<VC>(s.H[0], 128, key, col + e, x);
         const int v = v0 + col + e;
-        *reinterpret_cast<uint4*>(piece(p.DH + tile * T_STATE + (v >> 6) * 16384, key, (v & 63) >> 3)) = x.hi;
+        if constexpr (!BULK) *reinterpret_cast<uint4*>(piece(p.DH + tile * T_STATE + (v >> 6) * 16384, key, (v & 63) >> 3)) = x.hi;
       }
       if (!(ok = warp_wait(&s.fullA[i & 1], (i >> 1) & 1))) break;
       const float* const vec = s.vec[i & 1];
@@ -186,12 +189,23 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_scan_kernel(const __grid_cons
       }
       fence_proxy_async();
       warp_arrive(&s.yReady, lane);
-      if (has) {
+      if constexpr (BULK) {
+        if (has) {
+#pragma unroll
+          for (int e = 0; e < HC / 8; ++e) {
+            *reinterpret_cast<uint4*>(piece(s.dO, t, (col >> 3) + e)) = kf[e];
+            if (len == C) *reinterpret_cast<uint4*>(piece(s.Os[0], t, (col >> 3) + e)) = kv[e];
+          }
+        }
+        fence_proxy_async();
+        warp_arrive(&s.oReady, lane);
+      }
+      if (has && (!BULK || len < C)) {
         __nv_bfloat16* const dv = p.dv + (static_cast<size_t>(tok0 + t) * p.H + h) * p.vc + v0 + col;
 #pragma unroll
         for (int e = 0; e < HC / 8; ++e) {
           const int v = v0 + col + 8 * e;
-          *reinterpret_cast<uint4*>(piece(p.DF + tile * T_VN + (v >> 6) * 8192, t, (v & 63) >> 3)) = kf[e];
+          if constexpr (!BULK) *reinterpret_cast<uint4*>(piece(p.DF + tile * T_VN + (v >> 6) * 8192, t, (v & 63) >> 3)) = kf[e];
           if (t < len && v < p.vc) *reinterpret_cast<uint4*>(dv + 8 * e) = kv[e];
         }
       }
@@ -231,6 +245,10 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_scan_kernel(const __grid_cons
         for (int b = 0; b < 2; ++b)
           umma::mma4<umma::KSTEP_KMAJOR, umma::KSTEP_MNMAJOR>(tb + D1, umma::desc_kmajor(aK + 16384 * b, 0), dH + 4ull * b * umma::KSTEP_MNMAJOR, id1, b);
         umma::commit(&s.m1);
+        if constexpr (BULK) {
+          bulk_s2g(p.DH + (static_cast<size_t>(c0 + nchunks - 1 - i) * p.H + h) * T_STATE + (v0 / 64) * 16384, s.H[0], 16384);
+          bulk_commit();
+        }
         if (!mbar_wait(&s.fullB, i & 1) || !mbar_wait(&s.dReady, i & 1)) { ok = false; break; }
         umma::fence_after_sync();
         umma::mma4<umma::KSTEP_MNMAJOR, umma::KSTEP_MNMAJOR>(tb + DO, umma::desc_mnmajor(aT + 8192, 0, 8192), dO, idTl, 0);
@@ -245,6 +263,7 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_scan_kernel(const __grid_cons
         if (!mbar_wait(&s.yReady, i & 1)) { ok = false; break; }
         umma::fence_after_sync();
         umma::mma4<umma::KSTEP_MNMAJOR, umma::KSTEP_MNMAJOR>(tb + D3, umma::desc_mnmajor(aK, 0, 16384), dX, id3, 1);
+        if constexpr (BULK) bulk_wait_read<0>();      // m3 also says that dh' may be overwritten
         umma::commit(&s.m3);
         umma::commit(&s.freeA[i & 1]);
       }
@@ -252,29 +271,55 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_scan_kernel(const __grid_cons
         s.dead = 1;
         atomicOr(p.status, KDA_STATUS_BWD_SCAN_MMA_WAIT);
       }
+      if constexpr (BULK) bulk_wait_read<0>();
     }
     __syncwarp();
   } else {
     if (lane == 0) {
       const int hq = h / p.grp;
-      bool ok = true;
-      for (int i = 0; i < nchunks && ok; ++i) {
-        const int b = i & 1, c = nchunks - 1 - i, tok0 = static_cast<int>(tok_begin + static_cast<long long>(c) * C);
-        const size_t tile = static_cast<size_t>(c0 + c) * p.H + h;
-        if (s.dead || (i >= 2 && !mbar_wait(&s.freeA[b], ((i - 2) >> 1) & 1))) { ok = false; break; }
+      auto first = [&](int i) { return static_cast<int>(tok_begin + static_cast<long long>(nchunks - 1 - i) * C); };
+      auto tile_of = [&](int i) { return static_cast<size_t>(c0 + nchunks - 1 - i) * p.H + h; };
+      auto loadA = [&](int i) {
+        const int b = i & 1, tok0 = first(i);
         mbar_expect_tx(&s.fullA[b], 4 * 8192 + VEC_COPY);
         for (int x = 0; x < 2; ++x) tma_load_rows(s.KQ[b][x], &p.tm_k, 64 * x, hq, tok0, &s.fullA[b]);
         for (int x = 0; x < 2; ++x) tma_load_rows(s.KQ[b][x] + 8192, &p.tm_q, 64 * x, hq, tok0, &s.fullA[b]);
-        bulk_g2s(s.vec[b], p.VEC + tile * T_VEC, VEC_COPY, &s.fullA[b]);
-        if (s.dead || (i >= 1 && !mbar_wait(&s.freeB, (i - 1) & 1))) { ok = false; break; }
+        bulk_g2s(s.vec[b], p.VEC + tile_of(i) * T_VEC, VEC_COPY, &s.fullA[b]);
+      };
+      auto loadB = [&](int i) {
         mbar_expect_tx(&s.fullB, 2 * 16384 + 8192);
-        tma_load_rows(s.dO, &p.tm_do, v0 & ~63, h, tok0, &s.fullB);
-        bulk_g2s(s.TP[0], p.TP + tile * T_TP, 32768, &s.fullB);
+        tma_load_rows(s.dO, &p.tm_do, v0 & ~63, h, first(i), &s.fullB);
+        bulk_g2s(s.TP[0], p.TP + tile_of(i) * T_TP, 32768, &s.fullB);
+      };
+      bool ok = true;
+      if (nchunks > 0) {
+        loadA(0);
+        loadB(0);
+        if (nchunks > 1) loadA(1);
+      }
+      for (int i = 0; i < nchunks; ++i) {
+        if (s.dead) { ok = false; break; }
+        if constexpr (BULK) {      // f stands in dO's tile, dv in the scaled dO's
+          if (!mbar_wait(&s.oReady, i & 1)) { ok = false; break; }
+          bulk_s2g(p.DF + tile_of(i) * T_VN + (v0 / 64) * 8192, s.dO, 8192);
+          if (tok_end - first(i) >= C) tma_store_rows(&p.tm_dv, v0, h, first(i), s.Os[0]);
+          bulk_commit();
+          bulk_wait_read<0>();
+        }
+        if (i + 1 < nchunks) {
+          if (!mbar_wait(&s.freeB, i & 1)) { ok = false; break; }
+          loadB(i + 1);
+        }
+        if (i + 2 < nchunks) {
+          if (!mbar_wait(&s.freeA[i & 1], (i >> 1) & 1)) { ok = false; break; }
+          loadA(i + 2);
+        }
       }
       if (!ok) {
         s.dead = 1;
         atomicOr(p.status, KDA_STATUS_BWD_SCAN_LOAD_WAIT);
       }
+      if constexpr (BULK) bulk_wait_read<0>();      // the stores read shared memory that goes with the CTA
     }
     __syncwarp();
   }

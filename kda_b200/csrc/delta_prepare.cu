@@ -1,10 +1,12 @@
 // Gated delta rule, one decay per token and head: what a chunk needs that does not depend on the state (see delta.cuh).
 //
-// One CTA per (chunk, head).  [K; Q] K^T is one product (128 x 64 x 128, its operands the input rows themselves); the decays, norms and beta multiply its
-// fp32 result.  Tm = (I + A)^-1: the four 16 x 16 diagonal blocks by substitution in fp32, then two merges
-// (T21 = -T2 A21 T1, at 16 and 32 rows), also in fp32: a merge by split bf16 products would take six dependent rounds on the tensor core.
-// Pt = P Tm is a product again, in hi + lo parts, whose A operand's upper half is Tm's own tile (the rows it adds are not read).
+// One CTA per (chunk, head), three of them on an SM.  [K; Q] K^T is one product (128 x 64 x 128, its operands the input rows themselves); the decays, norms and
+// beta multiply its fp32 result.  Tm = (I + A)^-1: the four 16 x 16 diagonal blocks by substitution in fp32, then two merges
+// T21 = -(T2 A21) T1, at 16 and 32 rows, by mma.sync on bf16 pairs: T2 A21 leaves the first product in the layout that the second takes its A in.
+// Pt = P Tm is a product of the tensor core again, in pairs, whose A operand's upper half is Tm's own tile (the rows it adds are not read).
 // G is summed in double and kept as two floats: after a strong decay early in a chunk one float leaves 1e-5 in every later D_ij.
+// Bound by instruction issue and shared memory (with the merges as fp32 sums over shared memory 25 k warp instructions and 5.8 k wavefronts a tile: 578 us for
+// 16,384 tiles).
 #include "delta.cuh"
 
 namespace kda {
@@ -15,7 +17,13 @@ namespace {
 constexpr int PT = 256;      // 8 warps: TMEM lane quadrant = warp & 3, column half = warp >> 2
 
 struct PrepSmem {
-  unsigned char KQ[2][16384];      // [128 rows: k, then q][64 columns] x 2; once read, A and T (below)
+  union {
+    unsigned char KQ[2][16384];    // [128 rows: k, then q][64 columns] x 2
+    struct {                       // once those are read:
+      unsigned char Ah[8192], Al[8192];      // A as bf16 pairs, [64][64]
+      float D[4][16][20];                    // its diagonal blocks in fp32
+    };
+  };
   unsigned char TPh[16384], TPl[16384];
   double gs[2];
   float ghi[C], glo[C], beta[C], rk[C], rq[C], q2[2][C];
@@ -24,11 +32,39 @@ struct PrepSmem {
 };
 static_assert(sizeof(PrepSmem) + 1024 <= 75 * 1024, "three CTAs per SM");
 
-// element (i, j) of a 64 x 64 fp32 matrix; groups of four columns are permuted by the row so that a column of threads writes without conflicts
-__device__ __forceinline__ int at(int i, int j) { return i * 64 + ((((j >> 2) ^ i) & 15) << 2) + (j & 3); }
-__device__ __forceinline__ float4 at4(const float* m, int i, int j4) { return *reinterpret_cast<const float4*>(m + i * 64 + (((j4 ^ i) & 15) << 2)); }
-__device__ __forceinline__ void axpy4(float4& y, float a, const float4& x) {
-  y.x = fmaf(a, x.x, y.x); y.y = fmaf(a, x.y, y.y); y.z = fmaf(a, x.z, y.z); y.w = fmaf(a, x.w, y.w);
+// a pair of neighbours (row, col), (row, col + 1) as bf16 pairs
+__device__ __forceinline__ void put2(unsigned char* hi, unsigned char* lo, int row, int col, float a, float b) {
+  uint32_t h, l;
+  split2(a, b, h, l);
+  *reinterpret_cast<uint32_t*>(hi + umma::sw128(row, col)) = h;
+  *reinterpret_cast<uint32_t*>(lo + umma::sw128(row, col)) = l;
+}
+// The 16 x 16 block at (row, col) of a tile as an A operand; the 16 x 16 block as a B operand of two products of eight columns.
+__device__ __forceinline__ void frag_a(uint32_t (&f)[4], const unsigned char* tile, int row, int col, int lane) {
+  ldsm_x4(f, smem_u32(tile) + umma::sw128(row + (lane & 15), col + 8 * (lane >> 4)));
+}
+__device__ __forceinline__ void frag_b(uint32_t (&f)[4], const unsigned char* tile, int row, int col, int lane) {
+  ldsm_x4_t(f, smem_u32(tile) + umma::sw128(row + (lane & 15), col + 8 * (lane >> 4)));
+}
+struct FragPair { uint32_t h[4], l[4]; };
+// c (16 x 16: two accumulators) += a b in pairs, without the product of the low parts
+__device__ __forceinline__ void mma_pair(float (&c)[2][4], const FragPair& a, const FragPair& b) {
+#pragma unroll
+  for (int n = 0; n < 2; ++n) {
+    mma16816(c[n], a.l, b.h[2 * n], b.h[2 * n + 1]);
+    mma16816(c[n], a.h, b.l[2 * n], b.l[2 * n + 1]);
+    mma16816(c[n], a.h, b.h[2 * n], b.h[2 * n + 1]);
+  }
+}
+// an accumulated 16 x 16 block as the A operand of the next product: the accumulator's layout is the operand's
+__device__ __forceinline__ FragPair as_a(const float (&c)[2][4]) {
+  FragPair f;
+#pragma unroll
+  for (int n = 0; n < 2; ++n) {
+    split2(c[n][0], c[n][1], f.h[2 * n], f.l[2 * n]);
+    split2(c[n][2], c[n][3], f.h[2 * n + 1], f.l[2 * n + 1]);
+  }
+  return f;
 }
 
 }  // namespace
@@ -125,46 +161,87 @@ __global__ void __launch_bounds__(PT, 3) delta_prepare_kernel(const __grid_const
   if (tid < C) s.rq[tid] = p.use_l2norm ? rsqrtf(s.q2[0][tid] + s.q2[1][tid] + L2NORM_EPS) : 1.f;
   __syncthreads();
   if (ok) {
-    float* const A = reinterpret_cast<float*>(s.KQ[0]);
-    float* const T = reinterpret_cast<float*>(s.KQ[1]);
-    {
+    // ---- A and P: rows times decays ------------------------------------------------------------------------------------------------------------------
+    const bool above = half > (q4 & 1);      // this warp's columns lie above the diagonal block row: zero
+    if (!above) {
       const float gh = s.ghi[i], gl = s.glo[i], f = q4 < 2 ? s.beta[i] * s.rk[i] : p.scale * s.rq[i];
       const int last = i < ci.len ? (q4 < 2 ? i - 1 : i) : -1;      // columns beyond it are zero, whatever stands in the rows' products
 #pragma unroll
-      for (int e = 0; e < 32; ++e) {
+      for (int e = 0; e < 32; e += 4) {
         const int j = 32 * half + e;
-        S[e] = j <= last ? S[e] * (f * s.rk[j]) * ex2((gh - s.ghi[j]) + (gl - s.glo[j])) : 0.f;
+        const float4 h4 = *reinterpret_cast<const float4*>(&s.ghi[j]), l4 = *reinterpret_cast<const float4*>(&s.glo[j]), r4 = *reinterpret_cast<const float4*>(&s.rk[j]);
+        S[e] = j <= last ? S[e] * (f * r4.x) * ex2((gh - h4.x) + (gl - l4.x)) : 0.f;
+        S[e + 1] = j + 1 <= last ? S[e + 1] * (f * r4.y) * ex2((gh - h4.y) + (gl - l4.y)) : 0.f;
+        S[e + 2] = j + 2 <= last ? S[e + 2] * (f * r4.z) * ex2((gh - h4.z) + (gl - l4.z)) : 0.f;
+        S[e + 3] = j + 3 <= last ? S[e + 3] * (f * r4.w) * ex2((gh - h4.w) + (gl - l4.w)) : 0.f;
       }
-    }
-    if (q4 < 2) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) *reinterpret_cast<float4*>(&A[at(i, 32 * half + 4 * e)]) = make_float4(S[4 * e], S[4 * e + 1], S[4 * e + 2], S[4 * e + 3]);
     } else {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) S[e] = 0.f;
+    }
+    {
+      unsigned char* const hi = q4 < 2 ? s.Ah : s.TPh + 8192;
+      unsigned char* const lo = q4 < 2 ? s.Al : s.TPl + 8192;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const Split x = split8(&S[8 * e]);
-        *reinterpret_cast<uint4*>(piece(s.TPh, 64 + i, 4 * half + e)) = x.hi;
-        *reinterpret_cast<uint4*>(piece(s.TPl, 64 + i, 4 * half + e)) = x.lo;
+        *reinterpret_cast<uint4*>(piece(hi, i, 4 * half + e)) = x.hi;
+        *reinterpret_cast<uint4*>(piece(lo, i, 4 * half + e)) = x.lo;
+        if (q4 < 2) {      // Tm begins as zeros: what stays so is its part above the diagonal
+          *reinterpret_cast<uint4*>(piece(s.TPh, i, 4 * half + e)) = make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(piece(s.TPl, i, 4 * half + e)) = make_uint4(0, 0, 0, 0);
+        }
+      }
+      if (q4 < 2 && half == q4) {
+        const int b = lane >> 4;      // the diagonal block of this row begins at column 16 b of its half
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          *reinterpret_cast<float4*>(&s.D[i >> 4][i & 15][4 * e]) = b ? make_float4(S[16 + 4 * e], S[17 + 4 * e], S[18 + 4 * e], S[19 + 4 * e])
+                                                                       : make_float4(S[4 * e], S[4 * e + 1], S[4 * e + 2], S[4 * e + 3]);
       }
     }
     __syncthreads();
-    // ---- Tm: diagonal blocks by substitution, a column per thread; meanwhile the others write VEC ------------------------------------------------
+    // ---- Tm: diagonal blocks by substitution, a column per thread; meanwhile others write VEC ----------------------------------------------------------
     if (tid < 64) {
-      const int b = tid & ~15, col = tid & 15;
+      const int b = tid >> 4, col = tid & 15;
       float x[16];
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         float acc = r == col ? 1.f : 0.f;
 #pragma unroll
         for (int j4 = 0; j4 < (r + 3) / 4; ++j4) {
-          const float4 a = at4(A, b + r, (b >> 2) + j4);
+          const float4 a = *reinterpret_cast<const float4*>(&s.D[b][r][4 * j4]);
           if (4 * j4 < r) acc = fmaf(-a.x, x[4 * j4], acc);
           if (4 * j4 + 1 < r) acc = fmaf(-a.y, x[4 * j4 + 1], acc);
           if (4 * j4 + 2 < r) acc = fmaf(-a.z, x[4 * j4 + 2], acc);
           if (4 * j4 + 3 < r) acc = fmaf(-a.w, x[4 * j4 + 3], acc);
         }
         x[r] = acc;
-        T[at(b + r, b + col)] = acc;
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const __nv_bfloat16 hi = __float2bfloat16_rn(x[r]);
+        const uint32_t off = umma::sw128(16 * b + r, 16 * b + col);
+        *reinterpret_cast<__nv_bfloat16*>(s.TPh + off) = hi;
+        *reinterpret_cast<__nv_bfloat16*>(s.TPl + off) = __float2bfloat16_rn(x[r] - __bfloat162float(hi));
+      }
+      __syncwarp();
+      // ---- merge of 16: each of the two warps has written both diagonal blocks of its pair -------------------------------------------------------------
+      const int r0 = 32 * warp;
+      FragPair t2, a21, t1;
+      frag_a(t2.h, s.TPh, r0 + 16, r0 + 16, lane);
+      frag_a(t2.l, s.TPl, r0 + 16, r0 + 16, lane);
+      frag_b(a21.h, s.Ah, r0 + 16, r0, lane);
+      frag_b(a21.l, s.Al, r0 + 16, r0, lane);
+      frag_b(t1.h, s.TPh, r0, r0, lane);
+      frag_b(t1.l, s.TPl, r0, r0, lane);
+      float y[2][4] = {}, z[2][4] = {};
+      mma_pair(y, t2, a21);
+      mma_pair(z, as_a(y), t1);
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        put2(s.TPh, s.TPl, r0 + 16 + (lane >> 2), r0 + 8 * n + 2 * (lane & 3), -z[n][0], -z[n][1]);
+        put2(s.TPh, s.TPl, r0 + 24 + (lane >> 2), r0 + 8 * n + 2 * (lane & 3), -z[n][2], -z[n][3]);
       }
     } else if (tid >= 128 && tid < 192) {
       const int t = tid - 128;
@@ -182,73 +259,35 @@ __global__ void __launch_bounds__(PT, 3) delta_prepare_kernel(const __grid_const
       if (t < 4) v[V_LAST + t] = ex2(lh + ll);
     }
     __syncthreads();
-    // ---- merges: X = A21 T1 into the unused upper right of T, then T21 = -T2 X ---------------------------------------------------------------------
-    {
-      const int b = 32 * (tid >> 7), r = (tid >> 3) & 15, c4 = tid & 3, m0 = (tid & 4) ? 8 : 0;      // eight terms of four columns per thread, two threads a sum
-      auto pairsum = [](float4 x) {
-        x.x += __shfl_xor_sync(0xffffffffu, x.x, 4);
-        x.y += __shfl_xor_sync(0xffffffffu, x.y, 4);
-        x.z += __shfl_xor_sync(0xffffffffu, x.z, 4);
-        x.w += __shfl_xor_sync(0xffffffffu, x.w, 4);
-        return x;
-      };
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    // ---- merge of 32: warps 0..3, 16 rows and 16 of the 32 columns each ----------------------------------------------------------------------------------
+    if (warp < 4) {
+      const int rb = warp & 1, n0 = 16 * (warp >> 1), r0 = 32 + 16 * rb;
+      float y[2][2][4] = {}, z[2][4] = {};      // T2 A21: 16 rows, 32 columns
 #pragma unroll
-      for (int m = 0; m < 8; ++m) {      // T1 above its diagonal is not written: zero
-        float4 t = at4(T, b + m0 + m, (b >> 2) + c4);
-        const int d = m0 + m - 4 * c4;
-        if (d < 0) t.x = 0.f;
-        if (d < 1) t.y = 0.f;
-        if (d < 2) t.z = 0.f;
-        if (d < 3) t.w = 0.f;
-        axpy4(acc, A[at(b + 16 + r, b + m0 + m)], t);
+      for (int m = 0; m < 2; ++m) {
+        if (m > rb) break;                       // T2's upper right block is zero
+        FragPair t2;
+        frag_a(t2.h, s.TPh, r0, 32 + 16 * m, lane);
+        frag_a(t2.l, s.TPl, r0, 32 + 16 * m, lane);
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          FragPair a21;
+          frag_b(a21.h, s.Ah, 32 + 16 * m, 16 * n, lane);
+          frag_b(a21.l, s.Al, 32 + 16 * m, 16 * n, lane);
+          mma_pair(y[n], t2, a21);
+        }
       }
-      acc = pairsum(acc);
-      if (!(tid & 4)) *reinterpret_cast<float4*>(&T[at(b + r, b + 16 + 4 * c4)]) = acc;
-      __syncthreads();
-      acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int m = 0; m < 8; ++m)
-        if (m0 + m <= r) axpy4(acc, -T[at(b + 16 + r, b + 16 + m0 + m)], at4(T, b + m0 + m, (b >> 2) + 4 + c4));
-      acc = pairsum(acc);
-      if (!(tid & 4)) *reinterpret_cast<float4*>(&T[at(b + 16 + r, b + 4 * c4)]) = acc;
-    }
-    __syncthreads();
-    {
-      const int r = tid >> 3, c4 = tid & 7;
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-      for (int m = 0; m < 32; ++m) {
-        float4 t = at4(T, m, c4);
-        const int d = m - 4 * c4;
-        if (d < 0) t.x = 0.f;
-        if (d < 1) t.y = 0.f;
-        if (d < 2) t.z = 0.f;
-        if (d < 3) t.w = 0.f;
-        axpy4(acc, A[at(32 + r, m)], t);
+      for (int m = 0; m < 2; ++m) {
+        FragPair t1;
+        frag_b(t1.h, s.TPh, 16 * m, n0, lane);
+        frag_b(t1.l, s.TPl, 16 * m, n0, lane);
+        mma_pair(z, as_a(y[m]), t1);
       }
-      *reinterpret_cast<float4*>(&T[at(r, 32 + 4 * c4)]) = acc;
-      __syncthreads();
-      acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-      for (int m = 0; m < 32; ++m)
-        if (m <= r) axpy4(acc, -T[at(32 + r, 32 + m)], at4(T, m, 8 + c4));
-      *reinterpret_cast<float4*>(&T[at(32 + r, 4 * c4)]) = acc;
-    }
-    __syncthreads();
-    {      // Tm as an operand
-      const int r = tid >> 2, c0 = 16 * (tid & 3);
-      float x[16];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) *reinterpret_cast<float4*>(&x[4 * e]) = at4(T, r, (c0 >> 2) + e);
-#pragma unroll
-      for (int e = 0; e < 16; ++e)
-        if (c0 + e > r) x[e] = 0.f;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const Split y = split8(&x[8 * e]);
-        *reinterpret_cast<uint4*>(piece(s.TPh, r, (c0 >> 3) + e)) = y.hi;
-        *reinterpret_cast<uint4*>(piece(s.TPl, r, (c0 >> 3) + e)) = y.lo;
+      for (int n = 0; n < 2; ++n) {
+        put2(s.TPh, s.TPl, r0 + (lane >> 2), n0 + 8 * n + 2 * (lane & 3), -z[n][0], -z[n][1]);
+        put2(s.TPh, s.TPl, r0 + 8 + (lane >> 2), n0 + 8 * n + 2 * (lane & 3), -z[n][2], -z[n][3]);
       }
     }
     fence_proxy_async();
@@ -287,7 +326,7 @@ __global__ void __launch_bounds__(PT, 3) delta_prepare_kernel(const __grid_const
       bulk_s2g(p.TP + tile * T_TP, s.TPh, 16384);
       bulk_s2g(p.TP + tile * T_TP + 16384, s.TPl, 16384);
       bulk_commit();
-      bulk_wait<0>();
+      bulk_wait_read<0>();      // shared memory may go; the writes are complete with the kernel
     }
   }
   if (!ok && tid == 0) {      // a wait gave up: loads and products may still be under way

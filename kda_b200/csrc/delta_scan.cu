@@ -9,6 +9,8 @@
 // epilogue adds the two accumulators: the products are bound by reading operands from shared memory, and A is the larger one.
 // With 128 columns there is no room in tensor memory for that; they accumulate one behind the other.
 // The warps meet through mbarriers only; warp 8 issues the products, warp 9 the loads.
+// From 64 columns on tiles leave by bulk copies, HS from the operand h, v_new and o through operands that are done (v's tile, q's rows): stored by the threads
+// that have them, 32 rows at a time, they took the load/store unit 4 k cycles a chunk (8 x 4096 x 32 in training: 816 us).
 #include "delta.cuh"
 
 namespace kda {
@@ -29,7 +31,7 @@ struct ScanSmem {
   unsigned char R[SPANS][8192];                              // [64 t][..] the same of r, then of w v_new
   float vec[2][VEC_COPY / 4];
   uint64_t fullA[2], freeA[2], fullB, freeB;                 // k, q, VEC; TP, v
-  uint64_t hReady, rReady, uReady, m1, m2, m3;
+  uint64_t hReady, rReady, uReady, oReady, m1, m2, m3;
   uint32_t tmem_slot;
   volatile int dead;
 };
@@ -54,7 +56,7 @@ template <int VC, bool TRAIN>
 __global__ void __launch_bounds__(NT, 1) delta_scan_kernel(const __grid_constant__ ScanParams p) {
   chain_point();
   using Smem = ScanSmem<VC>;
-  constexpr bool CAT = Smem::CAT;
+  constexpr bool CAT = Smem::CAT, BULK = VC >= 64;      // BULK: tiles and full chunks of o leave by bulk copies
   constexpr int HC = VC / 2, DW = CAT ? 2 * VC : VC;
   constexpr int D1 = 0, D2 = DW, D3 = 2 * DW;
   constexpr uint32_t TM = 3 * DW <= 256 ? 256 : 512;
@@ -77,6 +79,7 @@ __global__ void __launch_bounds__(NT, 1) delta_scan_kernel(const __grid_constant
     mbar_init(&s.hReady, 8);
     mbar_init(&s.rReady, 4);
     mbar_init(&s.uReady, 4);
+    mbar_init(&s.oReady, 4);
     mbar_init(&s.m1, 1);
     mbar_init(&s.m2, 1);
     mbar_init(&s.m3, 1);
@@ -125,7 +128,7 @@ __global__ void __launch_bounds__(NT, 1) delta_scan_kernel(const __grid_constant
       for (int e = 0; e < HC; e += 8) {
         const Split x = split8(&S[e]);
         put<VC>(s.H[0], 128, key, col + e, x);
-        if constexpr (TRAIN) {
+        if constexpr (TRAIN && !BULK) {
           const int v = v0 + col + e;
           *reinterpret_cast<uint4*>(piece(p.HS + tile * T_STATE + (v >> 6) * 16384, key, (v & 63) >> 3)) = x.hi;
         }
@@ -162,14 +165,21 @@ __global__ void __launch_bounds__(NT, 1) delta_scan_kernel(const __grid_constant
         warp_arrive(&s.rReady, lane);
         if (!(ok = warp_wait(&s.m2, i & 1))) break;
         umma::fence_after_sync();
-        uint4 keep[TRAIN ? HC / 8 : 1];
+        uint4 keep[TRAIN && !BULK ? HC / 8 : 1];
 #pragma unroll
         for (int e = 0; e < HC; e += 16) {
           float x[16];
           load(D2, e, x);
           if constexpr (TRAIN) {
-            keep[e / 8] = pack8(&x[0]);
-            keep[e / 8 + 1] = pack8(&x[8]);
+            const uint4 a = pack8(&x[0]), b = pack8(&x[8]);
+            if constexpr (BULK) {      // into v's tile: the same places
+              const int c = col + e;
+              *reinterpret_cast<uint4*>(piece(s.V[c >> 6], t, (c & 63) >> 3)) = a;
+              *reinterpret_cast<uint4*>(piece(s.V[c >> 6], t, ((c & 63) >> 3) + 1)) = b;
+            } else {
+              keep[e / 8] = a;
+              keep[e / 8 + 1] = b;
+            }
           }
 #pragma unroll
           for (int j = 0; j < 16; ++j) x[j] *= vw;
@@ -178,7 +188,7 @@ __global__ void __launch_bounds__(NT, 1) delta_scan_kernel(const __grid_constant
         }
         fence_proxy_async();
         warp_arrive(&s.uReady, lane);
-        if constexpr (TRAIN) {
+        if constexpr (TRAIN && !BULK) {
 #pragma unroll
           for (int e = 0; e < HC / 8; ++e) {
             const int v = v0 + col + 8 * e;
@@ -197,8 +207,19 @@ __global__ void __launch_bounds__(NT, 1) delta_scan_kernel(const __grid_constant
           load(D2, e, y);
 #pragma unroll
           for (int j = 0; j < 16; ++j) y[j] = fmaf(vq, x[j], y[j]);
+          if (BULK && len == C) {      // into q's rows, which product 1 has read
+            const int c = col + e;
+            unsigned char* const out = s.KQ[i & 1][c >> 6] + 8192;
+            *reinterpret_cast<uint4*>(piece(out, t, (c & 63) >> 3)) = pack8(&y[0]);
+            *reinterpret_cast<uint4*>(piece(out, t, ((c & 63) >> 3) + 1)) = pack8(&y[8]);
+            continue;
+          }
           if (t < len && v0 + col + e < p.vc) *reinterpret_cast<uint4*>(o + e) = pack8(&y[0]);
           if (t < len && v0 + col + e + 8 < p.vc) *reinterpret_cast<uint4*>(o + e + 8) = pack8(&y[8]);
+        }
+        if constexpr (BULK) {
+          fence_proxy_async();
+          warp_arrive(&s.oReady, lane);
         }
       }
       if (!(ok = warp_wait(&s.m3, i & 1))) break;
@@ -240,6 +261,11 @@ __global__ void __launch_bounds__(NT, 1) delta_scan_kernel(const __grid_constant
             umma::mma4<umma::KSTEP_KMAJOR, umma::KSTEP_MNMAJOR>(tb + D1, umma::desc_kmajor(aK + 16384 * b, 0),
                                                                 umma::desc_mnmajor(aH + x * LO * HS_, 4 * b, HS_), id1, x + b > 0);
         umma::commit(&s.m1);
+        if constexpr (TRAIN && BULK) {
+#pragma unroll
+          for (int x = 0; x < VC / 64; ++x) bulk_s2g(p.HS + (static_cast<size_t>(c0 + i) * p.H + h) * T_STATE + (v0 / 64 + x) * 16384, s.H[x], 16384);
+          bulk_commit();
+        }
         if (!mbar_wait(&s.fullB, i & 1) || !mbar_wait(&s.rReady, i & 1)) { ok = false; break; }
         umma::fence_after_sync();
         umma::mma4<umma::KSTEP_KMAJOR, umma::KSTEP_MNMAJOR>(tb + D2, umma::desc_kmajor(aT, 0), umma::desc_mnmajor(aR, 0, RS_), id1, 0);
@@ -253,6 +279,7 @@ __global__ void __launch_bounds__(NT, 1) delta_scan_kernel(const __grid_constant
 #pragma unroll
         for (int x = 0; x < (CAT ? 1 : 2); ++x)
           umma::mma4<umma::KSTEP_MNMAJOR, umma::KSTEP_MNMAJOR>(tb + D3, umma::desc_mnmajor(aK, 0, 16384), umma::desc_mnmajor(aR + x * LO * RS_, 0, RS_), id3, x);
+        if constexpr (TRAIN && BULK) bulk_wait_read<0>();      // m3 also says that h may be overwritten
         umma::commit(&s.m3);
         umma::commit(&s.freeA[i & 1]);
       }
@@ -260,6 +287,7 @@ __global__ void __launch_bounds__(NT, 1) delta_scan_kernel(const __grid_constant
         s.dead = 1;
         atomicOr(p.status, KDA_STATUS_SCAN_MMA_WAIT);
       }
+      if constexpr (TRAIN && BULK) bulk_wait_read<0>();
     }
     __syncwarp();
   } else {
@@ -279,17 +307,45 @@ __global__ void __launch_bounds__(NT, 1) delta_scan_kernel(const __grid_constant
         bulk_g2s(s.TP[0], p.TP + (static_cast<size_t>(c0 + i) * p.H + h) * T_TP, 32768, &s.fullB);
       };
       bool ok = true;
-      int i = 0;
-      for (; i < nchunks && ok; ++i) {
-        if (s.dead || (i >= 2 && !mbar_wait(&s.freeA[i & 1], ((i - 2) >> 1) & 1))) { ok = false; break; }
-        loadA(i);
-        if (s.dead || (i >= 1 && !mbar_wait(&s.freeB, (i - 1) & 1))) { ok = false; break; }
-        loadB(i);
+      if (nchunks > 0) {
+        loadA(0);
+        loadB(0);
+        if (nchunks > 1) loadA(1);
+      }
+      for (int i = 0; i < nchunks; ++i) {
+        if (s.dead) { ok = false; break; }
+        if constexpr (TRAIN && BULK) {      // v_new stands in v's tile
+          if (!mbar_wait(&s.uReady, i & 1)) { ok = false; break; }
+#pragma unroll
+          for (int x = 0; x < VC / 64; ++x) bulk_s2g(p.VN + (static_cast<size_t>(c0 + i) * p.H + h) * T_VN + (v0 / 64 + x) * 8192, s.V[x], 8192);
+          bulk_commit();
+          bulk_wait_read<0>();
+        }
+        if (i + 1 < nchunks) {
+          if (!mbar_wait(&s.freeB, i & 1)) { ok = false; break; }
+          loadB(i + 1);
+        }
+        if constexpr (BULK) {               // o in q's rows
+          if (!mbar_wait(&s.oReady, i & 1)) { ok = false; break; }
+          const long long tok0 = tok_begin + static_cast<long long>(i) * C;
+          if (tok_end - tok0 >= C) {
+#pragma unroll
+            for (int x = 0; x < VC / 64; ++x)
+              if (v0 + 64 * x < p.vc) tma_store_rows(&p.tm_o, v0 + 64 * x, h, static_cast<int>(tok0), s.KQ[i & 1][x] + 8192);
+            bulk_commit();
+            bulk_wait_read<0>();
+          }
+        }
+        if (i + 2 < nchunks) {
+          if (!mbar_wait(&s.freeA[i & 1], (i >> 1) & 1)) { ok = false; break; }
+          loadA(i + 2);
+        }
       }
       if (!ok) {
         s.dead = 1;
         atomicOr(p.status, KDA_STATUS_SCAN_LOAD_WAIT);
       }
+      if constexpr (BULK) bulk_wait_read<0>();      // the stores read shared memory that goes with the CTA
     }
     __syncwarp();
   }

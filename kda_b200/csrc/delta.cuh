@@ -124,8 +124,11 @@ struct MainParams {
 };
 
 int launch_prepare(const PrepParams& p, long long tiles, cudaStream_t st);
+// The walks: `slices` CTAs per (sequence, head) unit (1, 2 or 4; 0: by the number of units and SMs).  The forms with one CTA are in files of their own.
 int launch_scan(const ScanParams& p, int units, int slices, cudaStream_t st);
+int launch_scan_t(const ScanParams& p, int units, cudaStream_t st);
 int launch_bwd_scan(const RScanParams& p, int units, int slices, cudaStream_t st);
+int launch_bwd_scan_t(const RScanParams& p, int units, cudaStream_t st);
 int launch_bwd_main(const MainParams& p, long long tiles, int spans, cudaStream_t st);   // spans of 64 value columns
 
 // x = hi + lo to 17 bits: eight neighbours at a time, as the two 16-byte pieces of an operand row

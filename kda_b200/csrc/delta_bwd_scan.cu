@@ -298,6 +298,16 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_scan_kernel(const __grid_cons
         if (nchunks > 1) loadA(1);
       }
       for (int i = 0; i < nchunks; ++i) {
+        if (i + 3 < nchunks) {     // into L2, ahead of the loads: from DRAM a stage takes longer than a chunk
+          if (v0 == 0) {           // what the slices of a unit share
+            for (int x = 0; x < 2 && 64 * x < p.kc; ++x) {
+              tma_prefetch_rows(&p.tm_k, 64 * x, hq, first(i + 3));
+              tma_prefetch_rows(&p.tm_q, 64 * x, hq, first(i + 3));
+            }
+            bulk_prefetch(p.TP + tile_of(i + 3) * T_TP, 32768);
+          }
+          if ((v0 & 63) == 0) tma_prefetch_rows(&p.tm_do, v0, h, first(i + 3));
+        }
         if (s.dead) { ok = false; break; }
         if constexpr (BULK) {      // f stands in dO's tile, dv in the scaled dO's
           if (!mbar_wait(&s.oReady, i & 1)) { ok = false; break; }
@@ -343,8 +353,8 @@ static int launch_vc(const RScanParams& p, int units, cudaStream_t st) {
 }
 
 int launch_bwd_scan(const RScanParams& p, int units, int slices, cudaStream_t st) {
-  if (slices == 0) slices = 4 * units <= sm_count() ? 4 : 2;
-  return slices == 4 ? launch_vc<32>(p, units, st) : launch_vc<64>(p, units, st);
+  if (slices == 0) slices = 4 * units <= sm_count() ? 4 : 2 * units <= sm_count() ? 2 : 1;
+  return slices == 4 ? launch_vc<32>(p, units, st) : slices == 2 ? launch_vc<64>(p, units, st) : launch_bwd_scan_t(p, units, st);
 }
 
 }  // namespace delta

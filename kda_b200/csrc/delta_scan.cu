@@ -1,16 +1,15 @@
 // Gated delta rule, one decay per token and head: the forward walk over a sequence's chunks (see delta.cuh).
 //
-// A CTA walks the chunks of one (sequence, head) with VC of the value columns; the recurrence is independent per column.  The state is fp32 in registers
-// (TMEM lane = key row, a thread holds half of a row's columns).  Per chunk, three dependent products:
+// A CTA walks the chunks of one (sequence, head) with VC = 32 or 64 of the value columns, for calls that have fewer units than SMs (delta_scan_t.cu: all
+// columns); the recurrence is independent per column.  The state is fp32 in registers (TMEM lane = key row, a thread holds half of a row's columns).  Per
+// chunk, three dependent products:
 //   1   [K; Q] h             (M = 128: the keys' rows and the queries' in one, K = 128)
 //   2   [Tm; Pt] r           (r = beta V - beta exp(G) K h; gives v_new and the chunk's own part of o, K = 64)
 //   3   K^T (w v_new)        (added to the state that the registers decay, K = 64)
-// h, r and w v_new are bf16 pairs.  Up to 64 columns hi and lo stand side by side in one operand, so that a product reads A once for both and the
-// epilogue adds the two accumulators: the products are bound by reading operands from shared memory, and A is the larger one.
-// With 128 columns there is no room in tensor memory for that; they accumulate one behind the other.
+// h, r and w v_new are bf16 pairs, hi and lo side by side in one operand, so that a product reads A once for both and the epilogue adds the two
+// accumulators: the products are bound by reading operands from shared memory, and A is the larger one.
 // The warps meet through mbarriers only; warp 8 issues the products, warp 9 the loads.
-// From 64 columns on tiles leave by bulk copies, HS from the operand h, v_new and o through operands that are done (v's tile, q's rows): stored by the threads
-// that have them, 32 rows at a time, they took the load/store unit 4 k cycles a chunk (8 x 4096 x 32 in training: 816 us).
+// With 64 columns tiles leave by bulk copies, HS from the operand h, v_new and o through operands that are done (v's tile, q's rows).
 #include "delta.cuh"
 
 namespace kda {
@@ -22,12 +21,11 @@ constexpr int NW = 10, NT = NW * 32, W_ISSUE = 8;
 
 template <int VC>
 struct ScanSmem {
-  static constexpr bool CAT = VC <= 64;                      // hi and lo side by side
-  static constexpr int SPANS = VC == 32 ? 1 : VC / 32;       // 128-byte-wide spans of an operand of VC columns, hi and lo together
+  static constexpr int SPANS = VC / 32;                      // 128-byte-wide spans of an operand of VC columns, hi and lo together
   unsigned char KQ[2][2][16384];                             // two stages of [128 rows: k, then q][64 key columns] x 2
   unsigned char TP[2][16384];                                // hi, lo
-  unsigned char V[VC <= 64 ? 1 : 2][8192];                   // [64 t][64 v]
-  unsigned char H[SPANS][16384];                             // [128 keys][64 columns] spans: hi, then lo (VC = 32: 32 of each in one span)
+  unsigned char V[8192];                   // [64 t][64 v]
+  unsigned char H[SPANS][16384];                             // [128 keys][64 columns]: hi, then lo (VC = 32: 32 of each in one span)
   unsigned char R[SPANS][8192];                              // [64 t][..] the same of r, then of w v_new
   float vec[2][VEC_COPY / 4];
   uint64_t fullA[2], freeA[2], fullB, freeB;                 // k, q, VEC; TP, v
@@ -35,7 +33,7 @@ struct ScanSmem {
   uint32_t tmem_slot;
   volatile int dead;
 };
-static_assert(sizeof(ScanSmem<128>) + 1024 <= 227 * 1024, "ScanSmem too large");
+static_assert(sizeof(ScanSmem<64>) + 1024 <= 227 * 1024, "ScanSmem too large");
 
 // where eight columns (col a multiple of 8) of a row stand in an operand of VC columns as bf16 pairs
 template <int VC>
@@ -44,9 +42,8 @@ __device__ __forceinline__ void put(unsigned char* tile, int rows, int row, int 
     *reinterpret_cast<uint4*>(piece(tile, row, col >> 3)) = x.hi;
     *reinterpret_cast<uint4*>(piece(tile, row, 4 + (col >> 3))) = x.lo;
   } else {
-    unsigned char* const t = tile + (col >> 6) * rows * 128;
-    *reinterpret_cast<uint4*>(piece(t, row, (col & 63) >> 3)) = x.hi;
-    *reinterpret_cast<uint4*>(piece(t + (VC / 64) * rows * 128, row, (col & 63) >> 3)) = x.lo;
+    *reinterpret_cast<uint4*>(piece(tile, row, col >> 3)) = x.hi;
+    *reinterpret_cast<uint4*>(piece(tile + rows * 128, row, col >> 3)) = x.lo;
   }
 }
 
@@ -56,14 +53,14 @@ template <int VC, bool TRAIN>
 __global__ void __launch_bounds__(NT, 1) delta_scan_kernel(const __grid_constant__ ScanParams p) {
   chain_point();
   using Smem = ScanSmem<VC>;
-  constexpr bool CAT = Smem::CAT, BULK = VC >= 64;      // BULK: tiles and full chunks of o leave by bulk copies
-  constexpr int HC = VC / 2, DW = CAT ? 2 * VC : VC;
+  constexpr bool BULK = VC == 64;      // tiles and full chunks of o leave by bulk copies
+  constexpr int HC = VC / 2, DW = 2 * VC;
   constexpr int D1 = 0, D2 = DW, D3 = 2 * DW;
   constexpr uint32_t TM = 3 * DW <= 256 ? 256 : 512;
   extern __shared__ unsigned char smem_raw[];
   Smem& s = *reinterpret_cast<Smem*>(smem_raw + pad_to_1024(smem_raw));
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, q4 = warp & 3, half = (warp >> 2) & 1;
-  const int slices = (((p.vc + 63) & ~63) + VC - 1) / VC;    // narrow heads: whole spans of 64 columns, as the tiles have them
+  const int slices = ((p.vc + 63) & ~63) / VC;               // narrow heads: whole spans of 64 columns, as the tiles have them
   const int unit = blockIdx.x / slices, v0 = (blockIdx.x % slices) * VC;
   const int seq = p.map.started(unit / p.H), h = unit % p.H;
   const int c0 = p.map.first_chunk(seq), nchunks = p.map.first_chunk(seq + 1) - c0;
@@ -104,18 +101,13 @@ __global__ void __launch_bounds__(NT, 1) delta_scan_kernel(const __grid_constant
       const float4 f = p.h0 && key < p.kc && v0 + col + e < p.vc ? *reinterpret_cast<const float4*>(p.h0 + sb + e) : make_float4(0.f, 0.f, 0.f, 0.f);
       S[e] = f.x; S[e + 1] = f.y; S[e + 2] = f.z; S[e + 3] = f.w;
     }
-    // sums hi and lo where they are two accumulators
-    auto load = [&](int d, int e, float (&x)[16]) {
+    auto load = [&](int d, int e, float (&x)[16]) {      // hi's and lo's sums
+      float y[16];
       umma::tmem_ld16(tq + d + col + e, x);
-      if constexpr (CAT) {
-        float y[16];
-        umma::tmem_ld16(tq + d + VC + col + e, y);
-        umma::tmem_ld_wait();
+      umma::tmem_ld16(tq + d + VC + col + e, y);
+      umma::tmem_ld_wait();
 #pragma unroll
-        for (int j = 0; j < 16; ++j) x[j] += y[j];
-      } else {
-        umma::tmem_ld_wait();
-      }
+      for (int j = 0; j < 16; ++j) x[j] += y[j];
     };
     bool ok = true;
     for (int i = 0; i < nchunks; ++i) {
@@ -152,10 +144,9 @@ __global__ void __launch_bounds__(NT, 1) delta_scan_kernel(const __grid_constant
         for (int e = 0; e < HC; e += 16) {
           float x[16], v[16];
           load(D1, e, x);
-          const int c = (VC == 32 ? v0 & 63 : 0) + col + e;
-          const unsigned char* const vt = s.V[VC == 32 ? 0 : c >> 6];
-          unpack8(*reinterpret_cast<const uint4*>(piece(vt, t, (c & 63) >> 3)), &v[0]);
-          unpack8(*reinterpret_cast<const uint4*>(piece(vt, t, ((c & 63) >> 3) + 1)), &v[8]);
+          const int c = ((VC == 32 ? v0 & 63 : 0) + col + e) >> 3;
+          unpack8(*reinterpret_cast<const uint4*>(piece(s.V, t, c)), &v[0]);
+          unpack8(*reinterpret_cast<const uint4*>(piece(s.V, t, c + 1)), &v[8]);
 #pragma unroll
           for (int j = 0; j < 16; ++j) x[j] = t < len ? fmaf(vb, v[j], -vk * x[j]) : 0.f;
           put<VC>(s.R[0], 64, t, col + e, split8(&x[0]));
@@ -173,9 +164,8 @@ __global__ void __launch_bounds__(NT, 1) delta_scan_kernel(const __grid_constant
           if constexpr (TRAIN) {
             const uint4 a = pack8(&x[0]), b = pack8(&x[8]);
             if constexpr (BULK) {      // into v's tile: the same places
-              const int c = col + e;
-              *reinterpret_cast<uint4*>(piece(s.V[c >> 6], t, (c & 63) >> 3)) = a;
-              *reinterpret_cast<uint4*>(piece(s.V[c >> 6], t, ((c & 63) >> 3) + 1)) = b;
+              *reinterpret_cast<uint4*>(piece(s.V, t, (col + e) >> 3)) = a;
+              *reinterpret_cast<uint4*>(piece(s.V, t, ((col + e) >> 3) + 1)) = b;
             } else {
               keep[e / 8] = a;
               keep[e / 8 + 1] = b;
@@ -208,10 +198,8 @@ __global__ void __launch_bounds__(NT, 1) delta_scan_kernel(const __grid_constant
 #pragma unroll
           for (int j = 0; j < 16; ++j) y[j] = fmaf(vq, x[j], y[j]);
           if (BULK && len == C) {      // into q's rows, which product 1 has read
-            const int c = col + e;
-            unsigned char* const out = s.KQ[i & 1][c >> 6] + 8192;
-            *reinterpret_cast<uint4*>(piece(out, t, (c & 63) >> 3)) = pack8(&y[0]);
-            *reinterpret_cast<uint4*>(piece(out, t, ((c & 63) >> 3) + 1)) = pack8(&y[8]);
+            *reinterpret_cast<uint4*>(piece(s.KQ[i & 1][0] + 8192, t, (col + e) >> 3)) = pack8(&y[0]);
+            *reinterpret_cast<uint4*>(piece(s.KQ[i & 1][0] + 8192, t, ((col + e) >> 3) + 1)) = pack8(&y[8]);
             continue;
           }
           if (t < len && v0 + col + e < p.vc) *reinterpret_cast<uint4*>(o + e) = pack8(&y[0]);
@@ -244,41 +232,32 @@ __global__ void __launch_bounds__(NT, 1) delta_scan_kernel(const __grid_constant
   } else if (warp == W_ISSUE) {
     if (lane == 0) {
       // N of a product with hi and lo side by side (or of one of them), and with hi alone
-      constexpr int N = CAT ? 2 * VC : VC;
+      constexpr int N = 2 * VC;
       constexpr uint32_t id1 = umma::instr_desc(128, N, false, true), id2l = umma::instr_desc(128, VC, false, true), id3 = umma::instr_desc(128, N, true, true);
       constexpr uint32_t HS_ = 16384, RS_ = 8192;            // strides of the spans
       const uint32_t aH = smem_u32(s.H[0]), aR = smem_u32(s.R[0]), aT = smem_u32(s.TP[0]);
-      constexpr int LO = VC / 64;                            // !CAT: spans of hi in front of those of lo
       bool ok = true;
       for (int i = 0; i < nchunks && ok; ++i) {
         const uint32_t aK = smem_u32(s.KQ[i & 1][0]);
         if (s.dead || !mbar_wait(&s.fullA[i & 1], (i >> 1) & 1) || !mbar_wait(&s.hReady, i & 1)) { ok = false; break; }
         umma::fence_after_sync();
 #pragma unroll
-        for (int x = 0; x < (CAT ? 1 : 2); ++x)
-#pragma unroll
-          for (int b = 0; b < 2; ++b)
-            umma::mma4<umma::KSTEP_KMAJOR, umma::KSTEP_MNMAJOR>(tb + D1, umma::desc_kmajor(aK + 16384 * b, 0),
-                                                                umma::desc_mnmajor(aH + x * LO * HS_, 4 * b, HS_), id1, x + b > 0);
+        for (int b = 0; b < 2; ++b)
+          umma::mma4<umma::KSTEP_KMAJOR, umma::KSTEP_MNMAJOR>(tb + D1, umma::desc_kmajor(aK + 16384 * b, 0), umma::desc_mnmajor(aH, 4 * b, HS_), id1, b);
         umma::commit(&s.m1);
         if constexpr (TRAIN && BULK) {
-#pragma unroll
-          for (int x = 0; x < VC / 64; ++x) bulk_s2g(p.HS + (static_cast<size_t>(c0 + i) * p.H + h) * T_STATE + (v0 / 64 + x) * 16384, s.H[x], 16384);
+          bulk_s2g(p.HS + (static_cast<size_t>(c0 + i) * p.H + h) * T_STATE + (v0 / 64) * 16384, s.H[0], 16384);
           bulk_commit();
         }
         if (!mbar_wait(&s.fullB, i & 1) || !mbar_wait(&s.rReady, i & 1)) { ok = false; break; }
         umma::fence_after_sync();
         umma::mma4<umma::KSTEP_KMAJOR, umma::KSTEP_MNMAJOR>(tb + D2, umma::desc_kmajor(aT, 0), umma::desc_mnmajor(aR, 0, RS_), id1, 0);
-        if constexpr (!CAT)
-          umma::mma4<umma::KSTEP_KMAJOR, umma::KSTEP_MNMAJOR>(tb + D2, umma::desc_kmajor(aT, 0), umma::desc_mnmajor(aR + LO * RS_, 0, RS_), id1, 1);
         umma::mma4<umma::KSTEP_KMAJOR, umma::KSTEP_MNMAJOR>(tb + D2, umma::desc_kmajor(aT + 16384, 0), umma::desc_mnmajor(aR, 0, RS_), id2l, 1);
         umma::commit(&s.m2);
         umma::commit(&s.freeB);
         if (!mbar_wait(&s.uReady, i & 1)) { ok = false; break; }
         umma::fence_after_sync();
-#pragma unroll
-        for (int x = 0; x < (CAT ? 1 : 2); ++x)
-          umma::mma4<umma::KSTEP_MNMAJOR, umma::KSTEP_MNMAJOR>(tb + D3, umma::desc_mnmajor(aK, 0, 16384), umma::desc_mnmajor(aR + x * LO * RS_, 0, RS_), id3, x);
+        umma::mma4<umma::KSTEP_MNMAJOR, umma::KSTEP_MNMAJOR>(tb + D3, umma::desc_mnmajor(aK, 0, 16384), umma::desc_mnmajor(aR, 0, RS_), id3, 0);
         if constexpr (TRAIN && BULK) bulk_wait_read<0>();      // m3 also says that h may be overwritten
         umma::commit(&s.m3);
         umma::commit(&s.freeA[i & 1]);
@@ -302,8 +281,8 @@ __global__ void __launch_bounds__(NT, 1) delta_scan_kernel(const __grid_constant
       };
       auto loadB = [&](int i) {
         const int tok0 = static_cast<int>(tok_begin + static_cast<long long>(i) * C);
-        mbar_expect_tx(&s.fullB, 2 * 16384 + sizeof(s.V));
-        for (int x = 0; x < static_cast<int>(sizeof(s.V) / 8192); ++x) tma_load_rows(s.V[x], &p.tm_v, (v0 & ~63) + 64 * x, h, tok0, &s.fullB);
+        mbar_expect_tx(&s.fullB, 2 * 16384 + 8192);
+        tma_load_rows(s.V, &p.tm_v, v0 & ~63, h, tok0, &s.fullB);
         bulk_g2s(s.TP[0], p.TP + (static_cast<size_t>(c0 + i) * p.H + h) * T_TP, 32768, &s.fullB);
       };
       bool ok = true;
@@ -313,11 +292,21 @@ __global__ void __launch_bounds__(NT, 1) delta_scan_kernel(const __grid_constant
         if (nchunks > 1) loadA(1);
       }
       for (int i = 0; i < nchunks; ++i) {
+        if (i + 3 < nchunks) {                // into L2, ahead of the loads: from DRAM a stage takes longer than a chunk
+          const int tok0 = static_cast<int>(tok_begin + static_cast<long long>(i + 3) * C);
+          if (v0 == 0) {                      // what the slices of a unit share
+            for (int x = 0; x < 2 && 64 * x < p.kc; ++x) {
+              tma_prefetch_rows(&p.tm_k, 64 * x, hq, tok0);
+              tma_prefetch_rows(&p.tm_q, 64 * x, hq, tok0);
+            }
+            bulk_prefetch(p.TP + (static_cast<size_t>(c0 + i + 3) * p.H + h) * T_TP, 32768);
+          }
+          if ((v0 & 63) == 0) tma_prefetch_rows(&p.tm_v, v0, h, tok0);
+        }
         if (s.dead) { ok = false; break; }
         if constexpr (TRAIN && BULK) {      // v_new stands in v's tile
           if (!mbar_wait(&s.uReady, i & 1)) { ok = false; break; }
-#pragma unroll
-          for (int x = 0; x < VC / 64; ++x) bulk_s2g(p.VN + (static_cast<size_t>(c0 + i) * p.H + h) * T_VN + (v0 / 64 + x) * 8192, s.V[x], 8192);
+          bulk_s2g(p.VN + (static_cast<size_t>(c0 + i) * p.H + h) * T_VN + (v0 / 64) * 8192, s.V, 8192);
           bulk_commit();
           bulk_wait_read<0>();
         }
@@ -329,9 +318,7 @@ __global__ void __launch_bounds__(NT, 1) delta_scan_kernel(const __grid_constant
           if (!mbar_wait(&s.oReady, i & 1)) { ok = false; break; }
           const long long tok0 = tok_begin + static_cast<long long>(i) * C;
           if (tok_end - tok0 >= C) {
-#pragma unroll
-            for (int x = 0; x < VC / 64; ++x)
-              if (v0 + 64 * x < p.vc) tma_store_rows(&p.tm_o, v0 + 64 * x, h, static_cast<int>(tok0), s.KQ[i & 1][x] + 8192);
+            tma_store_rows(&p.tm_o, v0, h, static_cast<int>(tok0), s.KQ[i & 1][0] + 8192);
             bulk_commit();
             bulk_wait_read<0>();
           }
@@ -365,16 +352,16 @@ static int launch_vc(const ScanParams& p, int units, cudaStream_t st) {
   const int smem = static_cast<int>(sizeof(ScanSmem<VC>)) + 1024;
   const int rc = once.run([&] { return cudaFuncSetAttribute(delta_scan_kernel<VC, TRAIN>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
   if (rc != KDA_OK) return rc;
-  return static_cast<int>(launch_chained(delta_scan_kernel<VC, TRAIN>, static_cast<unsigned>(units) * ((((p.vc + 63) & ~63) + VC - 1) / VC), NT, smem, st, p));
+  return static_cast<int>(launch_chained(delta_scan_kernel<VC, TRAIN>, static_cast<unsigned>(units) * (((p.vc + 63) & ~63) / VC), NT, smem, st, p));
 }
 
-// Few (sequence, head) units leave SMs idle: their value columns are spread over up to four CTAs, which shortens a chunk's products.
+// Few (sequence, head) units leave SMs idle: their value columns are spread over two or four CTAs, which shortens a chunk's products.
 int launch_scan(const ScanParams& p, int units, int slices, cudaStream_t st) {
   if (slices == 0) slices = 4 * units <= sm_count() ? 4 : 2 * units <= sm_count() ? 2 : 1;
   const bool train = p.HS != nullptr;
   if (slices == 4) return train ? launch_vc<32, true>(p, units, st) : launch_vc<32, false>(p, units, st);
   if (slices == 2) return train ? launch_vc<64, true>(p, units, st) : launch_vc<64, false>(p, units, st);
-  return train ? launch_vc<128, true>(p, units, st) : launch_vc<128, false>(p, units, st);
+  return launch_scan_t(p, units, st);
 }
 
 }  // namespace delta

@@ -24,7 +24,7 @@
 // Tiles in the workspace, per (chunk, head), bf16 rows of 128 bytes, swizzled (umma::sw128), each a tcgen05 operand as it lies in memory:
 //   TP      [128][64] hi, then lo: rows 0..63 Tm, rows 64..127 Pt
 //   VEC     fp32 rows of 64: see the V_ constants; then exp(G_last)
-//   HS, DH  [128 keys][64 v] x 2: state in front of the chunk, gradient of the state behind it
+//   HS, DH  [128 v][64 keys] x 2: state in front of the chunk, gradient of the state behind it, both transposed
 //   VN, DF  [64 t][64 v] x 2: v_new and f
 #pragma once
 
@@ -161,6 +161,28 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) {
   umma::fence_before_sync();
   __syncwarp();
   if (lane == 0) mbar_arrive(bar);
+}
+// One value column of a [64 t][64 v] tile in shared memory, two bytes a row: `at` from column_at for a first row that is a multiple of eight, `j` rows further.
+__device__ __forceinline__ uint32_t column_at(const unsigned char* tile, int row, int v) { return smem_u32(tile) + umma::sw128(row, v); }
+__device__ __forceinline__ uint32_t column_get(uint32_t at, int j) {
+  unsigned short x;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(x) : "r"((at ^ ((j & 7) << 4)) + j * 128) : "memory");
+  return x;
+}
+__device__ __forceinline__ void column_put(uint32_t at, int j, float x) {
+  asm volatile("st.shared.b16 [%0], %1;" ::"r"((at ^ ((j & 7) << 4)) + j * 128), "h"(__bfloat16_as_ushort(__float2bfloat16_rn(x))) : "memory");
+}
+// sixteen neighbours of VEC
+__device__ __forceinline__ void row16(const float* p, float (&x)[16]) {
+#pragma unroll
+  for (int e = 0; e < 16; e += 4) *reinterpret_cast<float4*>(&x[e]) = *reinterpret_cast<const float4*>(p + e);
+}
+// eight value columns of a state's row `key`, as bf16, into a [128 v][64 keys] x 2 tile in global memory: the lanes of a warp are neighbouring keys
+__device__ __forceinline__ void leave_state(unsigned char* tile, int key, int v, const uint4& x) {
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    *reinterpret_cast<uint16_t*>(tile + (key >> 6) * 16384 + umma::sw128(v + j, key & 63)) = static_cast<uint16_t>(j & 1 ? w[j / 2] >> 16 : w[j / 2]);
 }
 // rows len..63 of the [64][64] boxes at `tile` and `tile + stride` (a sequence's last chunk): what a load found there belongs to the next sequence
 __device__ __forceinline__ void clear_rows(unsigned char* tile, int len, int tid, int nthreads) {

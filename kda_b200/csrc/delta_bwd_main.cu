@@ -101,9 +101,9 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_main_kernel(const __grid_cons
         }
       }
       float hd = 0.f;
-      for (int b = 0; b < spans; ++b)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {      // (the same places of both tiles: their order does not matter)
+      for (int b = 0; b < 2; ++b)
+        for (int e = 0; e < 2 * spans; ++e) {      // (the same places of both tiles: their order does not matter)
           float x[8], y[8];
           unpack8(*reinterpret_cast<const uint4*>(s.HS[b] + (tid + 256 * e) * 16), x);
           unpack8(*reinterpret_cast<const uint4*>(s.DH[b] + (tid + 256 * e) * 16), y);
@@ -270,12 +270,14 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_main_kernel(const __grid_cons
           bulk_g2s(s.VN[x], p.VN + at * T_VN + x * 8192, 8192, &s.fullB);
           tma_load_rows(s.FD[x] + 8192, &p.tm_do, 64 * x, h, tok0, &s.fullB);
           tma_load_rows(s.V[x], &p.tm_v, 64 * x, h, tok0, &s.fullB);
-          bulk_g2s(s.HS[x], p.HS + at * T_STATE + x * 16384, 16384, &s.fullB);
-          bulk_g2s(s.DH[x], p.DH + at * T_STATE + x * 16384, 16384, &s.fullB);
+        }
+        for (int x = 0; x < 2; ++x) {      // spans of 64 keys: the rows of the value columns that there are
+          bulk_g2s(s.HS[x], p.HS + at * T_STATE + x * 16384, spans * 8192, &s.fullB);
+          bulk_g2s(s.DH[x], p.DH + at * T_STATE + x * 16384, spans * 8192, &s.fullB);
         }
       };
-      constexpr uint32_t idS = umma::instr_desc(128, 64, false, false), idY = umma::instr_desc(128, 128, false, false),
-                         id4 = umma::instr_desc(128, 128, false, true), id5 = umma::instr_desc(128, 128, true, true);
+      constexpr uint32_t idS = umma::instr_desc(128, 64, false, false),
+                         id4 = umma::instr_desc(128, 128, false, true) /* Y and Z too: the states' rows are value columns */, id5 = umma::instr_desc(128, 128, true, true);
       auto store = [&](long long tile, int n) {      // dk, dq of a full chunk
         const ChunkInfo ci = p.map.info(static_cast<int>(tile / p.H));
         if (ci.len < C) return;
@@ -308,8 +310,8 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_main_kernel(const __grid_cons
         umma::commit(&s.mS);
 #pragma unroll 1
         for (int b = 0; b < spans; ++b) {
-          umma::mma4<umma::KSTEP_KMAJOR, umma::KSTEP_KMAJOR>(tb + T_Y, umma::desc_kmajor(smem_u32(s.FD[b]), 0), umma::desc_kmajor(smem_u32(s.HS[b]), 0), idY, b);
-          umma::mma4<umma::KSTEP_KMAJOR, umma::KSTEP_KMAJOR>(tb + T_Z, umma::desc_kmajor(smem_u32(s.VN[b]), 0), umma::desc_kmajor(smem_u32(s.DH[b]), 0), idY, b);
+          umma::mma4<umma::KSTEP_KMAJOR, umma::KSTEP_MNMAJOR>(tb + T_Y, umma::desc_kmajor(smem_u32(s.FD[b]), 0), umma::desc_mnmajor(smem_u32(s.HS[0]), 4 * b, 16384), id4, b);
+          umma::mma4<umma::KSTEP_KMAJOR, umma::KSTEP_MNMAJOR>(tb + T_Z, umma::desc_kmajor(smem_u32(s.VN[b]), 0), umma::desc_mnmajor(smem_u32(s.DH[0]), 4 * b, 16384), id4, b);
         }
         umma::commit(&s.mY);
         if (n > 0) store(tile - gridDim.x, n - 1);      // everybody is past the tile before: `ready`

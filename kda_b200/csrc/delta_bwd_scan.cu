@@ -6,7 +6,7 @@
 //   2   Tm^T x                    (M = 64, K = 64;   f = that + Pt^T dO)
 //   3   K^T y                     (M = 128, K = 64;  y = -beta exp(G) f;  dh = exp(G_last) dh' + that + Q^T (scale exp(G) dO))
 // Pt^T dO and Q^T (..) depend on dO alone and run beside the chain.  dh', x, y and the scaled dO are bf16 pairs, hi and lo side by side in one operand.
-// With 64 columns the tiles and full chunks of dv leave by bulk copies: DH from the operand dh', f and dv through operands that are done (dO's tile, the scaled dO's).
+// With 64 columns f and dv leave by bulk copies, through operands that are done (dO's tile, the scaled dO's).
 #include "delta.cuh"
 
 namespace kda {
@@ -118,8 +118,7 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_scan_kernel(const __grid_cons
       for (int e = 0; e < HC; e += 8) {
         const Split x = split8(&S[e]);
         put<VC>(s.H[0], 128, key, col + e, x);
-        const int v = v0 + col + e;
-        if constexpr (!BULK) *reinterpret_cast<uint4*>(piece(p.DH + tile * T_STATE + (v >> 6) * 16384, key, (v & 63) >> 3)) = x.hi;
+        leave_state(p.DH + tile * T_STATE, key, v0 + col + e, x.hi);
       }
       if (!(ok = warp_wait(&s.fullA[i & 1], (i >> 1) & 1))) break;
       const float* const vec = s.vec[i & 1];
@@ -245,10 +244,6 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_scan_kernel(const __grid_cons
         for (int b = 0; b < 2; ++b)
           umma::mma4<umma::KSTEP_KMAJOR, umma::KSTEP_MNMAJOR>(tb + D1, umma::desc_kmajor(aK + 16384 * b, 0), dH + 4ull * b * umma::KSTEP_MNMAJOR, id1, b);
         umma::commit(&s.m1);
-        if constexpr (BULK) {
-          bulk_s2g(p.DH + (static_cast<size_t>(c0 + nchunks - 1 - i) * p.H + h) * T_STATE + (v0 / 64) * 16384, s.H[0], 16384);
-          bulk_commit();
-        }
         if (!mbar_wait(&s.fullB, i & 1) || !mbar_wait(&s.dReady, i & 1)) { ok = false; break; }
         umma::fence_after_sync();
         umma::mma4<umma::KSTEP_MNMAJOR, umma::KSTEP_MNMAJOR>(tb + DO, umma::desc_mnmajor(aT + 8192, 0, 8192), dO, idTl, 0);
@@ -263,7 +258,6 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_scan_kernel(const __grid_cons
         if (!mbar_wait(&s.yReady, i & 1)) { ok = false; break; }
         umma::fence_after_sync();
         umma::mma4<umma::KSTEP_MNMAJOR, umma::KSTEP_MNMAJOR>(tb + D3, umma::desc_mnmajor(aK, 0, 16384), dX, id3, 1);
-        if constexpr (BULK) bulk_wait_read<0>();      // m3 also says that dh' may be overwritten
         umma::commit(&s.m3);
         umma::commit(&s.freeA[i & 1]);
       }
@@ -271,7 +265,6 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_scan_kernel(const __grid_cons
         s.dead = 1;
         atomicOr(p.status, KDA_STATUS_BWD_SCAN_MMA_WAIT);
       }
-      if constexpr (BULK) bulk_wait_read<0>();
     }
     __syncwarp();
   } else {

@@ -16,11 +16,11 @@ namespace {
 constexpr int CW = 16, NT = (CW + 2) * 32, W_ISSUE = CW;
 
 struct RTSmem {
-  unsigned char KQ[2][2][16384];
+  unsigned char KQ[2][2][16384];        // two stages, of dO and of what leaves as dv too
+  unsigned char dO[2][2][8192];         // [64 t][64 v] x 2
+  unsigned char dV[2][2][8192];
   unsigned char TP[2][16384];
-  unsigned char dO[2][8192];            // [64 t][64 v] x 2
-  unsigned char dV[2][8192];
-  unsigned char H[2][16384];            // dh' as it leaves: [128 keys][64 v] x 2
+  unsigned char H[2][16384];            // dh' as it leaves: [128 v][64 keys] x 2
   alignas(16) float vec[2][VEC_COPY / 4];
   uint64_t fullA[2], freeA[2], fullB, freeB;
   uint64_t hReady, dReady, xReady, yReady, oReady, m1, m2, m3;
@@ -31,12 +31,6 @@ static_assert(sizeof(RTSmem) + 1024 <= 227 * 1024, "RTSmem too large");
 
 // TMEM columns: dh' hi, lo; product 1, then x or y (16 columns per group of tokens: eight hi, eight lo); scaled dO hi, lo; dO; products 2 and 3
 constexpr int AH = 0, AL = 64, D1 = 128, OH = 192, OL = 224, DO = 256, D2 = 288, D3 = 352;
-
-// sixteen neighbours of VEC
-__device__ __forceinline__ void row16(const float* p, float (&x)[16]) {
-#pragma unroll
-  for (int e = 0; e < 16; e += 4) *reinterpret_cast<float4*>(&x[e]) = *reinterpret_cast<const float4*>(p + e);
-}
 
 }  // namespace
 
@@ -90,10 +84,8 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_scan_t_kernel(const __grid_co
         const Split a = split8(&S[e]), b = split8(&S[e + 8]);
         umma::tmem_st8(tq + AH + (k0 + e) / 2, a.hi, b.hi);
         umma::tmem_st8(tq + AL + (k0 + e) / 2, a.lo, b.lo);
-        const uint32_t w[8] = {a.hi.x, a.hi.y, a.hi.z, a.hi.w, b.hi.x, b.hi.y, b.hi.z, b.hi.w};
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          *reinterpret_cast<uint16_t*>(s.H[v >> 6] + umma::sw128(k0 + e + j, v & 63)) = static_cast<uint16_t>(j & 1 ? w[j / 2] >> 16 : w[j / 2]);
+        *reinterpret_cast<uint4*>(piece(s.H[g >> 1], v, 4 * (g & 1) + e / 8)) = a.hi;
+        *reinterpret_cast<uint4*>(piece(s.H[g >> 1], v, 4 * (g & 1) + e / 8 + 1)) = b.hi;
       }
       umma::tmem_st_wait();
       if (!(ok = warp_wait(&s.fullA[i & 1], (i >> 1) & 1))) break;
@@ -108,14 +100,14 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_scan_t_kernel(const __grid_co
 #pragma unroll
       for (int e = 0; e < 32; ++e) S[e] *= last;
       // ---- beside product 1: dO and scaled dO as operands ----
-      if (!(ok = warp_wait(&s.fullB, i & 1))) break;
+      const uint32_t at_o = column_at(s.dO[i & 1][v >> 6], t0, v & 63), at_v = column_at(s.dV[i & 1][v >> 6], t0, v & 63);
       {
         float d[16], q[16];
         uint32_t w[8];
         row16(vec + V_Q + t0, q);
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-          const uint32_t x = t0 + j < len ? *reinterpret_cast<const uint16_t*>(s.dO[v >> 6] + umma::sw128(t0 + j, v & 63)) : 0u;
+          const uint32_t x = t0 + j < len ? column_get(at_o, j) : 0u;
           w[j / 2] = j & 1 ? w[j / 2] | x << 16 : x;
           d[j] = __uint_as_float(x << 16) * q[j];
         }
@@ -159,10 +151,10 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_scan_t_kernel(const __grid_co
       warp_arrive(&s.yReady, lane);
       row16(vec + V_BETA + t0, w);
 #pragma unroll
-      for (int j = 0; j < 16; ++j) *reinterpret_cast<__nv_bfloat16*>(s.dO[v >> 6] + umma::sw128(t0 + j, v & 63)) = __float2bfloat16_rn(f[j]);
+      for (int j = 0; j < 16; ++j) column_put(at_o, j, f[j]);
       if (len == C) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) *reinterpret_cast<__nv_bfloat16*>(s.dV[v >> 6] + umma::sw128(t0 + j, v & 63)) = __float2bfloat16_rn(w[j] * f[j]);
+        for (int j = 0; j < 16; ++j) column_put(at_v, j, w[j] * f[j]);
       } else if (v < p.vc) {
 #pragma unroll
         for (int j = 0; j < 16; ++j)
@@ -259,14 +251,14 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_scan_t_kernel(const __grid_co
       auto tile_of = [&](int i) { return static_cast<size_t>(c0 + nchunks - 1 - i) * p.H + h; };
       auto loadA = [&](int i) {
         const int b = i & 1, tok0 = first(i);
-        mbar_expect_tx(&s.fullA[b], 4 * 8192 + VEC_COPY);
+        mbar_expect_tx(&s.fullA[b], 6 * 8192 + VEC_COPY);
         for (int x = 0; x < 2; ++x) tma_load_rows(s.KQ[b][x], &p.tm_k, 64 * x, hq, tok0, &s.fullA[b]);
         for (int x = 0; x < 2; ++x) tma_load_rows(s.KQ[b][x] + 8192, &p.tm_q, 64 * x, hq, tok0, &s.fullA[b]);
+        for (int x = 0; x < 2; ++x) tma_load_rows(s.dO[b][x], &p.tm_do, 64 * x, h, tok0, &s.fullA[b]);
         bulk_g2s(s.vec[b], p.VEC + tile_of(i) * T_VEC, VEC_COPY, &s.fullA[b]);
       };
       auto loadB = [&](int i) {
-        mbar_expect_tx(&s.fullB, 2 * 16384 + 2 * 8192);
-        for (int x = 0; x < 2; ++x) tma_load_rows(s.dO[x], &p.tm_do, 64 * x, h, first(i), &s.fullB);
+        mbar_expect_tx(&s.fullB, 2 * 16384);
         bulk_g2s(s.TP[0], p.TP + tile_of(i) * T_TP, 32768, &s.fullB);
       };
       bool ok = true;
@@ -276,28 +268,21 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_scan_t_kernel(const __grid_co
         if (nchunks > 1) loadA(1);
       }
       for (int i = 0; i < nchunks; ++i) {
-        if (i + 3 < nchunks) {                 // into L2, ahead of the loads: from DRAM a stage takes longer than a chunk
-          for (int x = 0; x < 2; ++x) {
-            if (64 * x < p.kc) tma_prefetch_rows(&p.tm_k, 64 * x, hq, first(i + 3));
-            if (64 * x < p.kc) tma_prefetch_rows(&p.tm_q, 64 * x, hq, first(i + 3));
-            if (64 * x < p.vc) tma_prefetch_rows(&p.tm_do, 64 * x, h, first(i + 3));
-          }
-          bulk_prefetch(p.TP + tile_of(i + 3) * T_TP, 32768);
+        if (i + 2 < nchunks) bulk_prefetch(p.TP + tile_of(i + 2) * T_TP, 32768);      // into L2
+        if (i + 1 < nchunks) {
+          if (s.dead || !mbar_wait(&s.freeB, i & 1)) { ok = false; break; }
+          loadB(i + 1);
         }
         if (s.dead || !mbar_wait(&s.oReady, i & 1)) { ok = false; break; }
 #pragma unroll
-        for (int x = 0; x < 2; ++x) bulk_s2g(p.DF + tile_of(i) * T_VN + x * 8192, s.dO[x], 8192);
+        for (int x = 0; x < 2; ++x) bulk_s2g(p.DF + tile_of(i) * T_VN + x * 8192, s.dO[i & 1][x], 8192);
         if (tok_end - first(i) >= C) {
-          for (int x = 0; x < 2 && 64 * x < p.vc; ++x) tma_store_rows(&p.tm_dv, 64 * x, h, first(i), s.dV[x]);
+          for (int x = 0; x < 2 && 64 * x < p.vc; ++x) tma_store_rows(&p.tm_dv, 64 * x, h, first(i), s.dV[i & 1][x]);
         }
         bulk_commit();
-        if (i + 1 < nchunks) {                 // (dv's tile is written again behind the next dO's arrival)
-          if (!mbar_wait(&s.freeB, i & 1)) { ok = false; break; }
-          bulk_wait_read<0>();
-          loadB(i + 1);
-        }
         if (i + 2 < nchunks) {
           if (!mbar_wait(&s.freeA[i & 1], (i >> 1) & 1)) { ok = false; break; }
+          bulk_wait_read<0>();
           loadA(i + 2);
         }
       }

@@ -9,7 +9,7 @@
 // h, r and w v_new are bf16 pairs, hi and lo side by side in one operand, so that a product reads A once for both and the epilogue adds the two
 // accumulators: the products are bound by reading operands from shared memory, and A is the larger one.
 // The warps meet through mbarriers only; warp 8 issues the products, warp 9 the loads.
-// With 64 columns tiles leave by bulk copies, HS from the operand h, v_new and o through operands that are done (v's tile, q's rows).
+// With 64 columns v_new and o leave by bulk copies, through operands that are done (v's tile, q's rows).
 #include "delta.cuh"
 
 namespace kda {
@@ -120,10 +120,7 @@ __global__ void __launch_bounds__(NT, 1) delta_scan_kernel(const __grid_constant
       for (int e = 0; e < HC; e += 8) {
         const Split x = split8(&S[e]);
         put<VC>(s.H[0], 128, key, col + e, x);
-        if constexpr (TRAIN && !BULK) {
-          const int v = v0 + col + e;
-          *reinterpret_cast<uint4*>(piece(p.HS + tile * T_STATE + (v >> 6) * 16384, key, (v & 63) >> 3)) = x.hi;
-        }
+        if constexpr (TRAIN) leave_state(p.HS + tile * T_STATE, key, v0 + col + e, x.hi);
       }
       if (!(ok = warp_wait(&s.fullA[i & 1], (i >> 1) & 1))) break;
       const float* const vec = s.vec[i & 1];
@@ -245,10 +242,6 @@ __global__ void __launch_bounds__(NT, 1) delta_scan_kernel(const __grid_constant
         for (int b = 0; b < 2; ++b)
           umma::mma4<umma::KSTEP_KMAJOR, umma::KSTEP_MNMAJOR>(tb + D1, umma::desc_kmajor(aK + 16384 * b, 0), umma::desc_mnmajor(aH, 4 * b, HS_), id1, b);
         umma::commit(&s.m1);
-        if constexpr (TRAIN && BULK) {
-          bulk_s2g(p.HS + (static_cast<size_t>(c0 + i) * p.H + h) * T_STATE + (v0 / 64) * 16384, s.H[0], 16384);
-          bulk_commit();
-        }
         if (!mbar_wait(&s.fullB, i & 1) || !mbar_wait(&s.rReady, i & 1)) { ok = false; break; }
         umma::fence_after_sync();
         umma::mma4<umma::KSTEP_KMAJOR, umma::KSTEP_MNMAJOR>(tb + D2, umma::desc_kmajor(aT, 0), umma::desc_mnmajor(aR, 0, RS_), id1, 0);
@@ -258,7 +251,6 @@ __global__ void __launch_bounds__(NT, 1) delta_scan_kernel(const __grid_constant
         if (!mbar_wait(&s.uReady, i & 1)) { ok = false; break; }
         umma::fence_after_sync();
         umma::mma4<umma::KSTEP_MNMAJOR, umma::KSTEP_MNMAJOR>(tb + D3, umma::desc_mnmajor(aK, 0, 16384), umma::desc_mnmajor(aR, 0, RS_), id3, 0);
-        if constexpr (TRAIN && BULK) bulk_wait_read<0>();      // m3 also says that h may be overwritten
         umma::commit(&s.m3);
         umma::commit(&s.freeA[i & 1]);
       }
@@ -266,7 +258,6 @@ __global__ void __launch_bounds__(NT, 1) delta_scan_kernel(const __grid_constant
         s.dead = 1;
         atomicOr(p.status, KDA_STATUS_SCAN_MMA_WAIT);
       }
-      if constexpr (TRAIN && BULK) bulk_wait_read<0>();
     }
     __syncwarp();
   } else {

@@ -20,9 +20,9 @@ constexpr int CW = 16, NT = (CW + 2) * 32, W_ISSUE = CW;
 template <bool TRAIN>
 struct TSmem {
   unsigned char KQ[2][2][16384];             // two stages of [128 rows: k, then q][64 key columns] x 2
+  unsigned char V[2][2][8192];               // and of [64 t][64 v] x 2
   unsigned char TP[2][16384];                // hi, lo
-  unsigned char V[2][8192];                  // [64 t][64 v] x 2
-  unsigned char H[TRAIN ? 2 : 1][TRAIN ? 16384 : 16];      // h as it leaves: [128 keys][64 v] x 2
+  unsigned char H[TRAIN ? 2 : 1][TRAIN ? 16384 : 16];      // h as it leaves: [128 v][64 keys] x 2
   alignas(16) float vec[2][VEC_COPY / 4];
   uint64_t fullA[2], freeA[2], fullB, freeB;
   uint64_t hReady, rReady, uReady, oReady, m1, m2, m3;
@@ -33,12 +33,6 @@ static_assert(sizeof(TSmem<true>) + 1024 <= 227 * 1024, "TSmem too large");
 
 // TMEM columns: h hi, lo; r (then w v_new) hi, lo; the three products (3 takes the place of 1)
 constexpr int AH = 0, AL = 64, RH = 128, RL = 160, D1 = 192, D2 = 320, D3 = D1;
-
-// sixteen neighbours of VEC
-__device__ __forceinline__ void row16(const float* p, float (&x)[16]) {
-#pragma unroll
-  for (int e = 0; e < 16; e += 4) *reinterpret_cast<float4*>(&x[e]) = *reinterpret_cast<const float4*>(p + e);
-}
 
 }  // namespace
 
@@ -94,10 +88,8 @@ __global__ void __launch_bounds__(NT, 1) delta_scan_t_kernel(const __grid_consta
         umma::tmem_st8(tq + AH + (k0 + e) / 2, a.hi, b.hi);
         umma::tmem_st8(tq + AL + (k0 + e) / 2, a.lo, b.lo);
         if constexpr (TRAIN) {
-          const uint32_t w[8] = {a.hi.x, a.hi.y, a.hi.z, a.hi.w, b.hi.x, b.hi.y, b.hi.z, b.hi.w};
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-            *reinterpret_cast<uint16_t*>(s.H[v >> 6] + umma::sw128(k0 + e + j, v & 63)) = static_cast<uint16_t>(j & 1 ? w[j / 2] >> 16 : w[j / 2]);
+          *reinterpret_cast<uint4*>(piece(s.H[g >> 1], v, 4 * (g & 1) + e / 8)) = a.hi;
+          *reinterpret_cast<uint4*>(piece(s.H[g >> 1], v, 4 * (g & 1) + e / 8 + 1)) = b.hi;
         }
       }
       umma::tmem_st_wait();
@@ -113,11 +105,15 @@ __global__ void __launch_bounds__(NT, 1) delta_scan_t_kernel(const __grid_consta
 #pragma unroll
       for (int e = 0; e < 32; ++e) S[e] *= last;
       // ---- r ----
-      if (!(ok = warp_wait(&s.fullB, i & 1))) break;
+      const uint32_t at_v = column_at(s.V[i & 1][v >> 6], t0, v & 63), at_o = column_at(s.KQ[i & 1][v >> 6] + 8192, t0, v & 63);
       float r[16], y[16], w[16];
       row16(vec + V_BETA + t0, w);
 #pragma unroll
-      for (int j = 0; j < 16; ++j) r[j] = __uint_as_float(static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(s.V[v >> 6] + umma::sw128(t0 + j, v & 63))) << 16) * w[j];
+      for (int j = 0; j < 16; ++j) r[j] = __uint_as_float(column_get(at_v, j) << 16) * w[j];
+      if (len < C) {      // what stands there belongs to the next sequence
+#pragma unroll
+        for (int j = 0; j < 16; ++j) r[j] = t0 + j < len ? r[j] : 0.f;
+      }
       row16(vec + V_KG + t0, w);
       if (!(ok = warp_wait(&s.m1, i & 1))) break;
       umma::fence_after_sync();
@@ -127,7 +123,7 @@ __global__ void __launch_bounds__(NT, 1) delta_scan_t_kernel(const __grid_consta
         umma::tmem_ld16(tq + D1 + 64 + t0, y);
         umma::tmem_ld_wait();
 #pragma unroll
-        for (int j = 0; j < 16; ++j) r[j] = t0 + j < len ? fmaf(-w[j], x[j], r[j]) : 0.f;
+        for (int j = 0; j < 16; ++j) r[j] = fmaf(-w[j], x[j], r[j]);      // (behind a sequence's end k's rows are zero)
         const Split a = split8(&r[0]), b = split8(&r[8]);
         umma::tmem_st8(tq + RH + t0 / 2, a.hi, b.hi);
         umma::tmem_st8(tq + RL + t0 / 2, a.lo, b.lo);
@@ -159,11 +155,11 @@ __global__ void __launch_bounds__(NT, 1) delta_scan_t_kernel(const __grid_consta
       warp_arrive(&s.uReady, lane);
       if constexpr (TRAIN) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) *reinterpret_cast<__nv_bfloat16*>(s.V[v >> 6] + umma::sw128(t0 + j, v & 63)) = __float2bfloat16_rn(r[j]);
+        for (int j = 0; j < 16; ++j) column_put(at_v, j, r[j]);
       }
       if (len == C) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) *reinterpret_cast<__nv_bfloat16*>(s.KQ[i & 1][v >> 6] + 8192 + umma::sw128(t0 + j, v & 63)) = __float2bfloat16_rn(y[j]);
+        for (int j = 0; j < 16; ++j) column_put(at_o, j, y[j]);
       } else if (v < p.vc) {
 #pragma unroll
         for (int j = 0; j < 16; ++j)
@@ -251,14 +247,14 @@ __global__ void __launch_bounds__(NT, 1) delta_scan_t_kernel(const __grid_consta
       auto tile_of = [&](int i) { return static_cast<size_t>(c0 + i) * p.H + h; };
       auto loadA = [&](int i) {
         const int b = i & 1, tok0 = first(i);
-        mbar_expect_tx(&s.fullA[b], 4 * 8192 + VEC_COPY);
+        mbar_expect_tx(&s.fullA[b], 6 * 8192 + VEC_COPY);
         for (int x = 0; x < 2; ++x) tma_load_rows(s.KQ[b][x], &p.tm_k, 64 * x, hq, tok0, &s.fullA[b]);
         for (int x = 0; x < 2; ++x) tma_load_rows(s.KQ[b][x] + 8192, &p.tm_q, 64 * x, hq, tok0, &s.fullA[b]);
+        for (int x = 0; x < 2; ++x) tma_load_rows(s.V[b][x], &p.tm_v, 64 * x, h, tok0, &s.fullA[b]);
         bulk_g2s(s.vec[b], p.VEC + tile_of(i) * T_VEC, VEC_COPY, &s.fullA[b]);
       };
       auto loadB = [&](int i) {
-        mbar_expect_tx(&s.fullB, 2 * 16384 + 2 * 8192);
-        for (int x = 0; x < 2; ++x) tma_load_rows(s.V[x], &p.tm_v, 64 * x, h, first(i), &s.fullB);
+        mbar_expect_tx(&s.fullB, 2 * 16384);
         bulk_g2s(s.TP[0], p.TP + tile_of(i) * T_TP, 32768, &s.fullB);
       };
       bool ok = true;
@@ -268,30 +264,23 @@ __global__ void __launch_bounds__(NT, 1) delta_scan_t_kernel(const __grid_consta
         if (nchunks > 1) loadA(1);
       }
       for (int i = 0; i < nchunks; ++i) {
-        if (i + 3 < nchunks) {                 // into L2, ahead of the loads: from DRAM a stage takes longer than a chunk
-          for (int x = 0; x < 2; ++x) {
-            if (64 * x < p.kc) tma_prefetch_rows(&p.tm_k, 64 * x, hq, first(i + 3));
-            if (64 * x < p.kc) tma_prefetch_rows(&p.tm_q, 64 * x, hq, first(i + 3));
-            if (64 * x < p.vc) tma_prefetch_rows(&p.tm_v, 64 * x, h, first(i + 3));
-          }
-          bulk_prefetch(p.TP + tile_of(i + 3) * T_TP, 32768);
+        if (i + 2 < nchunks) bulk_prefetch(p.TP + tile_of(i + 2) * T_TP, 32768);      // into L2
+        if (i + 1 < nchunks) {
+          if (s.dead || !mbar_wait(&s.freeB, i & 1)) { ok = false; break; }
+          loadB(i + 1);
         }
         if (s.dead || !mbar_wait(&s.oReady, i & 1)) { ok = false; break; }
         if constexpr (TRAIN) {                 // v_new stands in v's tile
 #pragma unroll
-          for (int x = 0; x < 2; ++x) bulk_s2g(p.VN + tile_of(i) * T_VN + x * 8192, s.V[x], 8192);
+          for (int x = 0; x < 2; ++x) bulk_s2g(p.VN + tile_of(i) * T_VN + x * 8192, s.V[i & 1][x], 8192);
         }
         if (tok_end - first(i) >= C) {         // o in q's rows
           for (int x = 0; x < 2 && 64 * x < p.vc; ++x) tma_store_rows(&p.tm_o, 64 * x, h, first(i), s.KQ[i & 1][x] + 8192);
         }
         bulk_commit();
-        if (i + 1 < nchunks) {
-          if (!mbar_wait(&s.freeB, i & 1)) { ok = false; break; }
-          bulk_wait_read<0>();
-          loadB(i + 1);
-        }
         if (i + 2 < nchunks) {
           if (!mbar_wait(&s.freeA[i & 1], (i >> 1) & 1)) { ok = false; break; }
+          bulk_wait_read<0>();
           loadA(i + 2);
         }
       }

@@ -18,7 +18,7 @@ namespace delta {
 
 namespace {
 
-constexpr int NT = 9 * 32;      // eight warps (TMEM lane quadrant = warp & 3, column half = warp >> 2) and one that issues products and loads
+constexpr int CW = 16, NT = (CW + 1) * 32;      // sixteen warps (TMEM lane quadrant = warp & 3, column group = warp >> 2) and one that issues products and loads
 
 struct MainSmem {
   unsigned char E[16384];              // [128][64]; as D5's A its second span is what follows, whose rows of the result nobody reads
@@ -28,8 +28,8 @@ struct MainSmem {
   unsigned char V[2][8192];
   unsigned char HS[2][16384], DH[2][16384];
   float vec[2][V_LAST + 4];
-  float red[2][3][C], redq[2][C];      // partial sums over the two column halves: k rows: k (row terms), k (column terms), dbeta; q rows: q dq
-  float redz[8], redh[8];
+  float red[4][3][C], redq[4][C];      // partial sums of the four column groups: k rows: k (row terms), k (column terms), dbeta; q rows: q dq
+  float redz[8], redh[CW];
   uint64_t fullA[2], fullB, ready, eReady, used, mS, mY, mD;
   uint32_t tmem_slot;
   volatile int dead;
@@ -48,15 +48,15 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_main_kernel(const __grid_cons
   chain_point();
   extern __shared__ unsigned char smem_raw[];
   MainSmem& s = *reinterpret_cast<MainSmem*>(smem_raw + pad_to_1024(smem_raw));
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, q4 = warp & 3, half = warp >> 2;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, q4 = warp & 3, g = warp >> 2;
   const long long total = static_cast<long long>(p.map.total()) * p.H;
   if (tid == 0) {
     mbar_init(&s.fullA[0], 1);
     mbar_init(&s.fullA[1], 1);
     mbar_init(&s.fullB, 1);
-    mbar_init(&s.ready, 8);
-    mbar_init(&s.eReady, 8);
-    mbar_init(&s.used, 8);
+    mbar_init(&s.ready, CW);
+    mbar_init(&s.eReady, CW);
+    mbar_init(&s.used, CW);
     mbar_init(&s.mS, 1);
     mbar_init(&s.mY, 1);
     mbar_init(&s.mD, 1);
@@ -69,9 +69,10 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_main_kernel(const __grid_cons
   umma::fence_after_sync();
   const uint32_t tb = s.tmem_slot, tq = tb + (static_cast<uint32_t>(32 * q4) << 16);
 
-  if (warp < 8) {
-    const int t = 32 * (q4 & 1) + lane;      // this thread's token, of k's rows or of q's; its columns 64 half ..
+  if (warp < CW) {
+    const int t = 32 * (q4 & 1) + lane;      // this thread's token, of k's rows or of q's
     const bool krow = q4 < 2;
+    auto meet = [] { asm volatile("bar.sync 1, %0;" ::"n"(CW * 32) : "memory"); };
     bool ok = true;
     int n = 0;
     for (long long tile = blockIdx.x; tile < total; tile += gridDim.x, ++n) {
@@ -80,22 +81,22 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_main_kernel(const __grid_cons
       if (__any_sync(0xffffffffu, s.dead != 0)) { ok = false; break; }
       if (!(ok = warp_wait(&s.fullA[n & 1], (n >> 1) & 1) && warp_wait(&s.fullB, n & 1))) break;
       if (ci.len < C) {
-        for (int b = 0; b < 4; ++b) clear_rows(s.KQ[n & 1][b >> 1] + (b & 1) * 8192, ci.len, tid, 256);
-        for (int b = 0; b < 2; ++b) clear_rows(s.FD[b] + 8192, ci.len, tid, 256);
+        for (int b = 0; b < 4; ++b) clear_rows(s.KQ[n & 1][b >> 1] + (b & 1) * 8192, ci.len, tid, CW * 32);
+        for (int b = 0; b < 2; ++b) clear_rows(s.FD[b] + 8192, ci.len, tid, CW * 32);
         fence_proxy_async();
       }
       warp_arrive(&s.ready, lane);
       const float* const vec = s.vec[n & 1];
-      const float vb = vec[V_BETA + t], vk = vec[V_KG + t], vw = vec[V_W + t], vq = vec[V_Q + t], rk = vec[V_RK + t], rq = vec[V_RQ + t];
+      const float vk = vec[V_KG + t], vw = vec[V_W + t], vq = vec[V_Q + t], rk = vec[V_RK + t], rq = vec[V_RQ + t];
       const float gh = vec[V_GHI + t], gl = vec[V_GLO + t];
-      // ---- what needs only the tiles: f v, <h, dh'> ----
+      // ---- what needs only the tiles: f v (32 of the columns), <h, dh'> ----
       float fv = 0.f;
-      if (krow && half < spans && t < ci.len) {
+      if (krow && (g >> 1) < spans && t < ci.len) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
+        for (int e = 0; e < 4; ++e) {
           float x[8], y[8];
-          unpack8(*reinterpret_cast<const uint4*>(piece(s.FD[half], t, e)), x);
-          unpack8(*reinterpret_cast<const uint4*>(piece(s.V[half], t, e)), y);
+          unpack8(*reinterpret_cast<const uint4*>(piece(s.FD[g >> 1], t, 4 * (g & 1) + e)), x);
+          unpack8(*reinterpret_cast<const uint4*>(piece(s.V[g >> 1], t, 4 * (g & 1) + e)), y);
 #pragma unroll
           for (int j = 0; j < 8; ++j) fv = fmaf(x[j], y[j], fv);
         }
@@ -103,10 +104,10 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_main_kernel(const __grid_cons
       float hd = 0.f;
 #pragma unroll
       for (int b = 0; b < 2; ++b)
-        for (int e = 0; e < 2 * spans; ++e) {      // (the same places of both tiles: their order does not matter)
+        for (int e = 0; e < spans; ++e) {      // (the same places of both tiles: their order does not matter)
           float x[8], y[8];
-          unpack8(*reinterpret_cast<const uint4*>(s.HS[b] + (tid + 256 * e) * 16), x);
-          unpack8(*reinterpret_cast<const uint4*>(s.DH[b] + (tid + 256 * e) * 16), y);
+          unpack8(*reinterpret_cast<const uint4*>(s.HS[b] + (tid + CW * 32 * e) * 16), x);
+          unpack8(*reinterpret_cast<const uint4*>(s.DH[b] + (tid + CW * 32 * e) * 16), y);
 #pragma unroll
           for (int j = 0; j < 8; ++j) hd = fmaf(x[j], y[j], hd);
         }
@@ -114,116 +115,142 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_main_kernel(const __grid_cons
       if (lane == 0) s.redh[warp] = hd;
       __syncwarp();
       if (lane == 0) mbar_arrive(&s.used);
-      // ---- E ----
+      // ---- E: 16 columns ----
       if (!(ok = warp_wait(&s.mS, n & 1))) break;
       umma::fence_after_sync();
-      float bsum = 0.f;
-      {
-        float g2[32];
-        umma::tmem_ld16(tq + T_G2 + 32 * half, *reinterpret_cast<float(*)[16]>(&g2[0]));
-        umma::tmem_ld16(tq + T_G2 + 32 * half + 16, *reinterpret_cast<float(*)[16]>(&g2[16]));
+      float bsum = 0.f, e16[16];
+      if (g >= 2 && (q4 & 1) == 0) {      // above the diagonal
+#pragma unroll
+        for (int e = 0; e < 16; ++e) e16[e] = 0.f;
+      } else {
+        umma::tmem_ld16(tq + T_G2 + 16 * g, e16);
         umma::tmem_ld_wait();
-        const int last = t < ci.len ? (krow ? t - 1 : t) : -1;
+        const int last = (t < ci.len ? (krow ? t - 1 : t) : -1) - 16 * g;
         const float f = krow ? -rk : p.scale * rq;
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const int j = 32 * half + e;
-          g2[e] = j <= last ? g2[e] * (f * vec[V_RK + j]) * ex2((gh - vec[V_GHI + j]) + (gl - vec[V_GLO + j])) : 0.f;
+        for (int e = 0; e < 16; e += 4) {
+          const int j = 16 * g + e;
+          const float4 h4 = *reinterpret_cast<const float4*>(vec + V_GHI + j), l4 = *reinterpret_cast<const float4*>(vec + V_GLO + j),
+                       r4 = *reinterpret_cast<const float4*>(vec + V_RK + j);
+          e16[e] = e <= last ? e16[e] * (f * r4.x) * ex2((gh - h4.x) + (gl - l4.x)) : 0.f;
+          e16[e + 1] = e + 1 <= last ? e16[e + 1] * (f * r4.y) * ex2((gh - h4.y) + (gl - l4.y)) : 0.f;
+          e16[e + 2] = e + 2 <= last ? e16[e + 2] * (f * r4.z) * ex2((gh - h4.z) + (gl - l4.z)) : 0.f;
+          e16[e + 3] = e + 3 <= last ? e16[e + 3] * (f * r4.w) * ex2((gh - h4.w) + (gl - l4.w)) : 0.f;
         }
         if (krow) {
-          float x[32];
-          umma::tmem_ld16(tq + T_S + 32 * half, *reinterpret_cast<float(*)[16]>(&x[0]));
-          umma::tmem_ld16(tq + T_S + 32 * half + 16, *reinterpret_cast<float(*)[16]>(&x[16]));
+          float x[16];
+          umma::tmem_ld16(tq + T_S + 16 * g, x);
           umma::tmem_ld_wait();
+          const float vb = vec[V_BETA + t];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            bsum = 32 * half + e <= last ? fmaf(g2[e], x[e], bsum) : bsum;
-            g2[e] *= vb;
+          for (int e = 0; e < 16; ++e) {
+            bsum = e <= last ? fmaf(e16[e], x[e], bsum) : bsum;
+            e16[e] *= vb;
           }
         }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) *reinterpret_cast<uint4*>(piece(s.E, 64 * (krow ? 0 : 1) + t, 4 * half + e)) = pack8(&g2[8 * e]);
       }
+      *reinterpret_cast<uint4*>(piece(s.E, 64 * (krow ? 0 : 1) + t, 2 * g)) = pack8(&e16[0]);
+      *reinterpret_cast<uint4*>(piece(s.E, 64 * (krow ? 0 : 1) + t, 2 * g + 1)) = pack8(&e16[8]);
       fence_proxy_async();
       warp_arrive(&s.eReady, lane);
-      // ---- the rows ----
-      if (!(ok = warp_wait(&s.mY, n & 1) && warp_wait(&s.mD, n & 1))) break;
+      // ---- the rows: 32 columns ----
+      unsigned char* const row = s.KQ[n & 1][g >> 1] + (krow ? 0 : 8192);
+      const int pc = 4 * (g & 1);
+      float x[32], da = 0.f, db = 0.f, dy = 0.f, dz = 0.f;
+      if (!(ok = warp_wait(&s.mY, n & 1))) break;
       umma::fence_after_sync();
-      const unsigned char* const row = s.KQ[n & 1][half] + (krow ? 0 : 8192);
-      float x[64], da = 0.f, db = 0.f, dy = 0.f, dz = 0.f;
 #pragma unroll
-      for (int e = 0; e < 64; e += 16) {
-        float a[16], b[16], in[16];
-        unpack8(*reinterpret_cast<const uint4*>(piece(row, t, e >> 3)), &in[0]);
-        unpack8(*reinterpret_cast<const uint4*>(piece(row, t, (e >> 3) + 1)), &in[8]);
-        umma::tmem_ld16(tq + T_Y + 64 * half + e, a);
-        umma::tmem_ld16(tq + T_D4 + 64 * half + e, b);
+      for (int e = 0; e < 32; e += 16) {      // what the first products give
+        float a[16], in[16];
+        unpack8(*reinterpret_cast<const uint4*>(piece(row, t, pc + (e >> 3))), &in[0]);
+        unpack8(*reinterpret_cast<const uint4*>(piece(row, t, pc + (e >> 3) + 1)), &in[8]);
+        umma::tmem_ld16(tq + T_Y + 32 * g + e, a);
         umma::tmem_ld_wait();
-        if (krow) {
+        const float f = krow ? -vk : vq;
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            dy = fmaf(in[j], a[j], dy);
-            x[e + j] = fmaf(-vk, a[j], b[j]);
-            da = fmaf(in[j], x[e + j], da);
-          }
-          umma::tmem_ld16(tq + T_Z + 64 * half + e, a);
-          umma::tmem_ld16(tq + T_D5 + 64 * half + e, b);
+        for (int j = 0; j < 16; ++j) {
+          dy = fmaf(in[j], a[j], dy);
+          x[e + j] = f * a[j];
+        }
+        if (krow) {
+          umma::tmem_ld16(tq + T_Z + 32 * g + e, a);
           umma::tmem_ld_wait();
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
             dz = fmaf(in[j], a[j], dz);
-            const float y = fmaf(vw, a[j], b[j]);
-            db = fmaf(in[j], y, db);
-            x[e + j] += y;
+            x[e + j] = fmaf(vw, a[j], x[e + j]);
           }
-        } else {
+        }
+      }
+      if (!(ok = warp_wait(&s.mD, n & 1))) break;
+      umma::fence_after_sync();
+#pragma unroll
+      for (int e = 0; e < 32; e += 16) {
+        float a[16], in[16];
+        unpack8(*reinterpret_cast<const uint4*>(piece(row, t, pc + (e >> 3))), &in[0]);
+        unpack8(*reinterpret_cast<const uint4*>(piece(row, t, pc + (e >> 3) + 1)), &in[8]);
+        umma::tmem_ld16(tq + T_D4 + 32 * g + e, a);
+        umma::tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          da = fmaf(in[j], a[j], da);
+          x[e + j] += a[j];
+        }
+        if (krow) {
+          umma::tmem_ld16(tq + T_D5 + 32 * g + e, a);
+          umma::tmem_ld_wait();
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
-            x[e + j] = fmaf(vq, a[j], b[j]);
-            da = fmaf(in[j], x[e + j], da);
+            db = fmaf(in[j], a[j], db);
+            x[e + j] += a[j];
           }
         }
       }
       if (krow) {
-        s.red[half][0][t] = da;
-        s.red[half][1][t] = db;
-        s.red[half][2][t] = fv + bsum - ex2(gh + gl) * rk * dy;
+        s.red[g][0][t] = fmaf(-vk, dy, da);
+        s.red[g][1][t] = fmaf(vw, dz, db);
+        s.red[g][2][t] = fv + bsum - ex2(gh + gl) * rk * dy;
         const float z = warp_sum(t < ci.len ? vw * dz : 0.f);
-        if (lane == 0) s.redz[2 * half + q4] = z;
+        if (lane == 0) s.redz[2 * g + q4] = z;
       } else {
-        s.redq[half][t] = da;
+        s.redq[g][t] = fmaf(vq, dy, da);
       }
-      asm volatile("bar.sync 1, 256;" ::: "memory");
+      meet();
       if (p.use_l2norm) {      // through the normalisation: what lies along the row itself falls out
-        const float d = krow ? (s.red[0][0][t] + s.red[1][0][t] + s.red[0][1][t] + s.red[1][1][t]) * rk * rk : (s.redq[0][t] + s.redq[1][t]) * rq * rq;
+        float d = 0.f;
 #pragma unroll
-        for (int e = 0; e < 64; e += 8) {
+        for (int e = 0; e < 4; ++e) d += krow ? s.red[e][0][t] + s.red[e][1][t] : s.redq[e][t];
+        d *= krow ? rk * rk : rq * rq;
+#pragma unroll
+        for (int e = 0; e < 32; e += 8) {
           float in[8];
-          unpack8(*reinterpret_cast<const uint4*>(piece(row, t, e >> 3)), in);
+          unpack8(*reinterpret_cast<const uint4*>(piece(row, t, pc + (e >> 3))), in);
 #pragma unroll
           for (int j = 0; j < 8; ++j) x[e + j] = fmaf(-d, in[j], x[e + j]);
         }
       }
       if (ci.len == C) {
 #pragma unroll
-        for (int e = 0; e < 64; e += 8) *reinterpret_cast<uint4*>(const_cast<unsigned char*>(piece(row, t, e >> 3))) = pack8(&x[e]);
+        for (int e = 0; e < 32; e += 8) *reinterpret_cast<uint4*>(piece(row, t, pc + (e >> 3))) = pack8(&x[e]);
         fence_proxy_async();
       } else if (t < ci.len) {
         __nv_bfloat16* const out = (krow ? p.dk : p.dq) + (static_cast<size_t>(ci.tok0 + t) * p.H + h) * p.kc;
 #pragma unroll
-        for (int e = 0; e < 64; e += 8)
-          if (64 * half + e < p.kc) *reinterpret_cast<uint4*>(out + 64 * half + e) = pack8(&x[e]);
+        for (int e = 0; e < 32; e += 8)
+          if (32 * g + e < p.kc) *reinterpret_cast<uint4*>(out + 32 * g + e) = pack8(&x[e]);
       }
       if (warp == 0) {      // dg: the sum of dG from a token to the chunk's end, two tokens a lane
-        float tail = 0.f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) tail += s.redh[j];
-        tail = tail * vec[V_LAST] + s.redz[0] + s.redz[1] + s.redz[2] + s.redz[3];
+        float tail = lane < CW ? s.redh[lane] * vec[V_LAST] : 0.f;
+        if (lane < 8) tail += s.redz[lane];
+        tail = warp_sum(tail);
         float d[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const int r = 2 * lane + j;
-          d[j] = r < ci.len ? s.redq[0][r] + s.redq[1][r] + s.red[0][0][r] + s.red[1][0][r] - s.red[0][1][r] - s.red[1][1][r] : 0.f;
+          d[j] = 0.f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) d[j] += s.redq[e][r] + s.red[e][0][r] - s.red[e][1][r];
+          if (r >= ci.len) d[j] = 0.f;
         }
         float sum = d[0] + d[1];
 #pragma unroll
@@ -238,12 +265,12 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_main_kernel(const __grid_cons
           if (r < ci.len) {
             const size_t at = static_cast<size_t>(ci.tok0 + r) * p.H + h;
             store_any(p.dg, at, p.g_dtype, (j ? sum - d[0] : sum) + tail);
-            store_any(p.dbeta, at, p.beta_dtype, s.red[0][2][r] + s.red[1][2][r]);
+            store_any(p.dbeta, at, p.beta_dtype, s.red[0][2][r] + s.red[1][2][r] + s.red[2][2][r] + s.red[3][2][r]);
           }
         }
       }
       umma::fence_before_sync();
-      asm volatile("bar.sync 1, 256;" ::: "memory");      // the sums are read before the next tile's are written
+      meet();      // the sums are read before the next tile's are written
     }
     if (ok) warp_arrive(&s.ready, lane);                  // the last tile's rows stand in shared memory
     if (!ok) {
@@ -300,13 +327,13 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_main_kernel(const __grid_cons
         if (s.dead || !mbar_wait(&s.fullA[n & 1], (n >> 1) & 1) || !mbar_wait(&s.fullB, n & 1) || !mbar_wait(&s.ready, n & 1)) { ok = false; break; }
         umma::fence_after_sync();
 #pragma unroll 1
+        for (int b = 0; b < spans; ++b)
+          umma::mma4<umma::KSTEP_KMAJOR, umma::KSTEP_KMAJOR>(tb + T_G2, umma::desc_kmajor(smem_u32(s.FD[b]), 0), umma::desc_kmajor(smem_u32(s.VN[b]), 0), idS, b);
+#pragma unroll 1
         for (int b = 0; b < 2; ++b) {
           const uint64_t d = umma::desc_kmajor(aK + 16384 * b, 0);
           umma::mma4<umma::KSTEP_KMAJOR, umma::KSTEP_KMAJOR>(tb + T_S, d, d, idS, b);
         }
-#pragma unroll 1
-        for (int b = 0; b < spans; ++b)
-          umma::mma4<umma::KSTEP_KMAJOR, umma::KSTEP_KMAJOR>(tb + T_G2, umma::desc_kmajor(smem_u32(s.FD[b]), 0), umma::desc_kmajor(smem_u32(s.VN[b]), 0), idS, b);
         umma::commit(&s.mS);
 #pragma unroll 1
         for (int b = 0; b < spans; ++b) {

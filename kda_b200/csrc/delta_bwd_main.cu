@@ -18,7 +18,9 @@ namespace delta {
 
 namespace {
 
-constexpr int CW = 16, NT = (CW + 1) * 32;      // sixteen warps (TMEM lane quadrant = warp & 3, column group = warp >> 2) and one that issues products and loads
+// sixteen warps (TMEM lane quadrant = warp & 3, column group = warp >> 2), one that issues the products, and one that has the loads, the stores and dg
+// (with loads and stores the issuing warp came late for the second products: 707 instead of 807 us without its stores)
+constexpr int CW = 16, NT = (CW + 2) * 32, W_ISSUE = CW;
 
 struct MainSmem {
   unsigned char E[16384];              // [128][64]; as D5's A its second span is what follows, whose rows of the result nobody reads
@@ -28,9 +30,11 @@ struct MainSmem {
   unsigned char V[2][8192];
   unsigned char HS[2][16384], DH[2][16384];
   float vec[2][V_LAST + 4];
-  float red[4][3][C], redq[4][C];      // partial sums of the four column groups: k rows: k (row terms), k (column terms), dbeta; q rows: q dq
-  float redz[8], redh[CW];
-  uint64_t fullA[2], fullB, ready, eReady, used, mS, mY, mD;
+  struct Sums {                        // of a tile, partial: of the four column groups
+    float k[4][3][C], q[4][C];         // k rows: k (row terms), k (column terms), dbeta; q rows: q dq
+    float z[8], h[CW];
+  } sums[2];
+  uint64_t fullA[2], fullB, ready, eReady, used, done, mS, mY, mD;
   uint32_t tmem_slot;
   volatile int dead;
 };
@@ -57,6 +61,7 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_main_kernel(const __grid_cons
     mbar_init(&s.ready, CW);
     mbar_init(&s.eReady, CW);
     mbar_init(&s.used, CW);
+    mbar_init(&s.done, CW);
     mbar_init(&s.mS, 1);
     mbar_init(&s.mY, 1);
     mbar_init(&s.mD, 1);
@@ -72,7 +77,6 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_main_kernel(const __grid_cons
   if (warp < CW) {
     const int t = 32 * (q4 & 1) + lane;      // this thread's token, of k's rows or of q's
     const bool krow = q4 < 2;
-    auto meet = [] { asm volatile("bar.sync 1, %0;" ::"n"(CW * 32) : "memory"); };
     bool ok = true;
     int n = 0;
     for (long long tile = blockIdx.x; tile < total; tile += gridDim.x, ++n) {
@@ -87,6 +91,7 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_main_kernel(const __grid_cons
       }
       warp_arrive(&s.ready, lane);
       const float* const vec = s.vec[n & 1];
+      MainSmem::Sums& sums = s.sums[n & 1];
       const float vk = vec[V_KG + t], vw = vec[V_W + t], vq = vec[V_Q + t], rk = vec[V_RK + t], rq = vec[V_RQ + t];
       const float gh = vec[V_GHI + t], gl = vec[V_GLO + t];
       // ---- what needs only the tiles: f v (32 of the columns), <h, dh'> ----
@@ -112,7 +117,7 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_main_kernel(const __grid_cons
           for (int j = 0; j < 8; ++j) hd = fmaf(x[j], y[j], hd);
         }
       hd = warp_sum(hd);
-      if (lane == 0) s.redh[warp] = hd;
+      if (lane == 0) sums.h[warp] = hd;
       __syncwarp();
       if (lane == 0) mbar_arrive(&s.used);
       // ---- E: 16 columns ----
@@ -207,19 +212,20 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_main_kernel(const __grid_cons
         }
       }
       if (krow) {
-        s.red[g][0][t] = fmaf(-vk, dy, da);
-        s.red[g][1][t] = fmaf(vw, dz, db);
-        s.red[g][2][t] = fv + bsum - ex2(gh + gl) * rk * dy;
+        sums.k[g][0][t] = fmaf(-vk, dy, da);
+        sums.k[g][1][t] = fmaf(vw, dz, db);
+        sums.k[g][2][t] = fv + bsum - ex2(gh + gl) * rk * dy;
         const float z = warp_sum(t < ci.len ? vw * dz : 0.f);
-        if (lane == 0) s.redz[2 * g + q4] = z;
+        if (lane == 0) sums.z[2 * g + q4] = z;
       } else {
-        s.redq[g][t] = fmaf(vq, dy, da);
+        sums.q[g][t] = fmaf(vq, dy, da);
       }
-      meet();
+      warp_arrive(&s.done, lane);
       if (p.use_l2norm) {      // through the normalisation: what lies along the row itself falls out
+        if (!(ok = warp_wait(&s.done, n & 1))) break;
         float d = 0.f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) d += krow ? s.red[e][0][t] + s.red[e][1][t] : s.redq[e][t];
+        for (int e = 0; e < 4; ++e) d += krow ? sums.k[e][0][t] + sums.k[e][1][t] : sums.q[e][t];
         d *= krow ? rk * rk : rq * rq;
 #pragma unroll
         for (int e = 0; e < 32; e += 8) {
@@ -239,91 +245,22 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_main_kernel(const __grid_cons
         for (int e = 0; e < 32; e += 8)
           if (32 * g + e < p.kc) *reinterpret_cast<uint4*>(out + 32 * g + e) = pack8(&x[e]);
       }
-      if (warp == 0) {      // dg: the sum of dG from a token to the chunk's end, two tokens a lane
-        float tail = lane < CW ? s.redh[lane] * vec[V_LAST] : 0.f;
-        if (lane < 8) tail += s.redz[lane];
-        tail = warp_sum(tail);
-        float d[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int r = 2 * lane + j;
-          d[j] = 0.f;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) d[j] += s.redq[e][r] + s.red[e][0][r] - s.red[e][1][r];
-          if (r >= ci.len) d[j] = 0.f;
-        }
-        float sum = d[0] + d[1];
-#pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-          const float y = __shfl_down_sync(0xffffffffu, sum, off);
-          if (lane + off < 32) sum += y;
-        }
-        // sum: over this lane's two tokens and all behind them
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int r = 2 * lane + j;
-          if (r < ci.len) {
-            const size_t at = static_cast<size_t>(ci.tok0 + r) * p.H + h;
-            store_any(p.dg, at, p.g_dtype, (j ? sum - d[0] : sum) + tail);
-            store_any(p.dbeta, at, p.beta_dtype, s.red[0][2][r] + s.red[1][2][r] + s.red[2][2][r] + s.red[3][2][r]);
-          }
-        }
-      }
       umma::fence_before_sync();
-      meet();      // the sums are read before the next tile's are written
     }
     if (ok) warp_arrive(&s.ready, lane);                  // the last tile's rows stand in shared memory
     if (!ok) {
       s.dead = 1;
       if (lane == 0) atomicOr(p.status, KDA_STATUS_BWD_MAIN_MMA_WAIT);
     }
-  } else {
+  } else if (warp == W_ISSUE) {
     if (lane == 0) {
-      auto loadA = [&](long long tile, int n) {
-        const ChunkInfo ci = p.map.info(static_cast<int>(tile / p.H));
-        const int h = static_cast<int>(tile % p.H), hq = h / p.grp, tok0 = static_cast<int>(ci.tok0), b = n & 1;
-        mbar_expect_tx(&s.fullA[b], 4 * 8192 + VEC_COPY);
-        for (int x = 0; x < 2; ++x) tma_load_rows(s.KQ[b][x], &p.tm_k, 64 * x, hq, tok0, &s.fullA[b]);
-        for (int x = 0; x < 2; ++x) tma_load_rows(s.KQ[b][x] + 8192, &p.tm_q, 64 * x, hq, tok0, &s.fullA[b]);
-        bulk_g2s(s.vec[b], p.VEC + static_cast<size_t>(tile) * T_VEC, VEC_COPY, &s.fullA[b]);
-      };
-      auto loadB = [&](long long tile) {
-        const ChunkInfo ci = p.map.info(static_cast<int>(tile / p.H));
-        const int h = static_cast<int>(tile % p.H), tok0 = static_cast<int>(ci.tok0);
-        const size_t at = static_cast<size_t>(tile);
-        mbar_expect_tx(&s.fullB, spans * (4 * 8192 + 2 * 16384));
-        for (int x = 0; x < spans; ++x) {
-          bulk_g2s(s.FD[x], p.DF + at * T_VN + x * 8192, 8192, &s.fullB);
-          bulk_g2s(s.VN[x], p.VN + at * T_VN + x * 8192, 8192, &s.fullB);
-          tma_load_rows(s.FD[x] + 8192, &p.tm_do, 64 * x, h, tok0, &s.fullB);
-          tma_load_rows(s.V[x], &p.tm_v, 64 * x, h, tok0, &s.fullB);
-        }
-        for (int x = 0; x < 2; ++x) {      // spans of 64 keys: the rows of the value columns that there are
-          bulk_g2s(s.HS[x], p.HS + at * T_STATE + x * 16384, spans * 8192, &s.fullB);
-          bulk_g2s(s.DH[x], p.DH + at * T_STATE + x * 16384, spans * 8192, &s.fullB);
-        }
-      };
       constexpr uint32_t idS = umma::instr_desc(128, 64, false, false),
                          id4 = umma::instr_desc(128, 128, false, true) /* Y and Z too: the states' rows are value columns */, id5 = umma::instr_desc(128, 128, true, true);
-      auto store = [&](long long tile, int n) {      // dk, dq of a full chunk
-        const ChunkInfo ci = p.map.info(static_cast<int>(tile / p.H));
-        if (ci.len < C) return;
-        const int h = static_cast<int>(tile % p.H), tok0 = static_cast<int>(ci.tok0);
-        for (int x = 0; x < 2 && 64 * x < p.kc; ++x) {
-          tma_store_rows(&p.tm_dk, 64 * x, h, tok0, s.KQ[n & 1][x]);
-          tma_store_rows(&p.tm_dq, 64 * x, h, tok0, s.KQ[n & 1][x] + 8192);
-        }
-        bulk_commit();
-      };
+      const uint32_t aE = smem_u32(s.E);
       bool ok = true;
       int n = 0;
-      if (blockIdx.x < total) {
-        loadA(blockIdx.x, 0);
-        loadB(blockIdx.x);
-      }
       for (long long tile = blockIdx.x; tile < total; tile += gridDim.x, ++n) {
-        const long long next = tile + gridDim.x;
-        const uint32_t aK = smem_u32(s.KQ[n & 1][0]), aE = smem_u32(s.E);
+        const uint32_t aK = smem_u32(s.KQ[n & 1][0]);
         if (s.dead || !mbar_wait(&s.fullA[n & 1], (n >> 1) & 1) || !mbar_wait(&s.fullB, n & 1) || !mbar_wait(&s.ready, n & 1)) { ok = false; break; }
         umma::fence_after_sync();
 #pragma unroll 1
@@ -341,11 +278,6 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_main_kernel(const __grid_cons
           umma::mma4<umma::KSTEP_KMAJOR, umma::KSTEP_MNMAJOR>(tb + T_Z, umma::desc_kmajor(smem_u32(s.VN[b]), 0), umma::desc_mnmajor(smem_u32(s.DH[0]), 4 * b, 16384), id4, b);
         }
         umma::commit(&s.mY);
-        if (n > 0) store(tile - gridDim.x, n - 1);      // everybody is past the tile before: `ready`
-        if (next < total) {
-          bulk_wait_read<0>();
-          loadA(next, n + 1);
-        }
         if (!mbar_wait(&s.eReady, n & 1)) { ok = false; break; }
         umma::fence_after_sync();
         umma::mma4<umma::KSTEP_KMAJOR, umma::KSTEP_MNMAJOR>(tb + T_D4, umma::desc_kmajor(aE, 0), umma::desc_mnmajor(aK, 0, 16384), id4, 0);
@@ -353,21 +285,115 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_main_kernel(const __grid_cons
         for (int b = 0; b < 2; ++b)      // E's rows 0..63 with K's, 64..127 with Q's: one run of 128 rows in both
           umma::mma4<umma::KSTEP_MNMAJOR, umma::KSTEP_MNMAJOR>(tb + T_D5, umma::desc_mnmajor(aE, 4 * b, 16384), umma::desc_mnmajor(aK, 4 * b, 16384), id5, b);
         umma::commit(&s.mD);
-        if (next < total) {
-          if (!mbar_wait(&s.mY, n & 1) || !mbar_wait(&s.used, n & 1)) { ok = false; break; }
-          loadB(next);
-        }
-      }
-      if (ok && n > 0) {
-        ok = mbar_wait(&s.ready, n & 1);
-        if (ok) store(blockIdx.x + static_cast<long long>(n - 1) * gridDim.x, n - 1);
       }
       if (!ok) {
         s.dead = 1;
-        atomicOr(p.status, KDA_STATUS_BWD_MAIN_LOAD_WAIT);
+        atomicOr(p.status, KDA_STATUS_BWD_MAIN_MMA_WAIT);
       }
-      bulk_wait_read<0>();      // the stores read shared memory that goes with the CTA
     }
+    __syncwarp();
+  } else {
+    // ================= loads, stores, dg and dbeta =================
+    auto loadA = [&](long long tile, int n) {
+      const ChunkInfo ci = p.map.info(static_cast<int>(tile / p.H));
+      const int h = static_cast<int>(tile % p.H), hq = h / p.grp, tok0 = static_cast<int>(ci.tok0), b = n & 1;
+      mbar_expect_tx(&s.fullA[b], 4 * 8192 + VEC_COPY);
+      for (int x = 0; x < 2; ++x) tma_load_rows(s.KQ[b][x], &p.tm_k, 64 * x, hq, tok0, &s.fullA[b]);
+      for (int x = 0; x < 2; ++x) tma_load_rows(s.KQ[b][x] + 8192, &p.tm_q, 64 * x, hq, tok0, &s.fullA[b]);
+      bulk_g2s(s.vec[b], p.VEC + static_cast<size_t>(tile) * T_VEC, VEC_COPY, &s.fullA[b]);
+    };
+    auto loadB = [&](long long tile) {
+      const ChunkInfo ci = p.map.info(static_cast<int>(tile / p.H));
+      const int h = static_cast<int>(tile % p.H), tok0 = static_cast<int>(ci.tok0);
+      const size_t at = static_cast<size_t>(tile);
+      mbar_expect_tx(&s.fullB, spans * (4 * 8192 + 2 * 16384));
+      for (int x = 0; x < spans; ++x) {
+        bulk_g2s(s.FD[x], p.DF + at * T_VN + x * 8192, 8192, &s.fullB);
+        bulk_g2s(s.VN[x], p.VN + at * T_VN + x * 8192, 8192, &s.fullB);
+        tma_load_rows(s.FD[x] + 8192, &p.tm_do, 64 * x, h, tok0, &s.fullB);
+        tma_load_rows(s.V[x], &p.tm_v, 64 * x, h, tok0, &s.fullB);
+      }
+      for (int x = 0; x < 2; ++x) {      // spans of 64 keys: the rows of the value columns that there are
+        bulk_g2s(s.HS[x], p.HS + at * T_STATE + x * 16384, spans * 8192, &s.fullB);
+        bulk_g2s(s.DH[x], p.DH + at * T_STATE + x * 16384, spans * 8192, &s.fullB);
+      }
+    };
+    auto store = [&](long long tile, int n) {      // dk, dq of a full chunk
+      const ChunkInfo ci = p.map.info(static_cast<int>(tile / p.H));
+      if (ci.len < C) return;
+      const int h = static_cast<int>(tile % p.H), tok0 = static_cast<int>(ci.tok0);
+      for (int x = 0; x < 2 && 64 * x < p.kc; ++x) {
+        tma_store_rows(&p.tm_dk, 64 * x, h, tok0, s.KQ[n & 1][x]);
+        tma_store_rows(&p.tm_dq, 64 * x, h, tok0, s.KQ[n & 1][x] + 8192);
+      }
+      bulk_commit();
+    };
+    bool ok = true;
+    int n = 0;
+    if (lane == 0 && blockIdx.x < total) {
+      loadA(blockIdx.x, 0);
+      loadB(blockIdx.x);
+    }
+    for (long long tile = blockIdx.x; tile < total; tile += gridDim.x, ++n) {
+      const long long next = tile + gridDim.x;
+      if (__any_sync(0xffffffffu, s.dead != 0)) { ok = false; break; }
+      if (!(ok = warp_wait(&s.ready, n & 1))) break;      // everybody is past the tile before
+      if (lane == 0) {
+        if (n > 0) store(tile - gridDim.x, n - 1);
+        if (next < total) {
+          bulk_wait_read<0>();
+          loadA(next, n + 1);
+        }
+      }
+      if (next < total) {
+        if (!(ok = warp_wait(&s.mY, n & 1) && warp_wait(&s.used, n & 1))) break;
+        if (lane == 0) loadB(next);
+      }
+      if (!(ok = warp_wait(&s.done, n & 1))) break;
+      {      // dg: the sum of dG from a token to the chunk's end, two tokens a lane (these sums are written again behind the load of the tile after the next)
+        const ChunkInfo ci = p.map.info(static_cast<int>(tile / p.H));
+        const int h = static_cast<int>(tile % p.H);
+        const float* const vec = s.vec[n & 1];
+        const MainSmem::Sums& sums = s.sums[n & 1];
+        float tail = lane < CW ? sums.h[lane] * vec[V_LAST] : 0.f;
+        if (lane < 8) tail += sums.z[lane];
+        tail = warp_sum(tail);
+        float d[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int r = 2 * lane + j;
+          d[j] = 0.f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) d[j] += sums.q[e][r] + sums.k[e][0][r] - sums.k[e][1][r];
+          if (r >= ci.len) d[j] = 0.f;
+        }
+        float sum = d[0] + d[1];
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+          const float y = __shfl_down_sync(0xffffffffu, sum, off);
+          if (lane + off < 32) sum += y;
+        }
+        // sum: over this lane's two tokens and all behind them
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int r = 2 * lane + j;
+          if (r < ci.len) {
+            const size_t at = static_cast<size_t>(ci.tok0 + r) * p.H + h;
+            store_any(p.dg, at, p.g_dtype, (j ? sum - d[0] : sum) + tail);
+            store_any(p.dbeta, at, p.beta_dtype, sums.k[0][2][r] + sums.k[1][2][r] + sums.k[2][2][r] + sums.k[3][2][r]);
+          }
+        }
+      }
+    }
+    if (ok && n > 0) {
+      ok = warp_wait(&s.ready, n & 1);
+      if (ok && lane == 0) store(blockIdx.x + static_cast<long long>(n - 1) * gridDim.x, n - 1);
+    }
+    if (!ok) {
+      s.dead = 1;
+      if (lane == 0) atomicOr(p.status, KDA_STATUS_BWD_MAIN_LOAD_WAIT);
+    }
+    if (lane == 0) bulk_wait_read<0>();      // the stores read shared memory that goes with the CTA
     __syncwarp();
   }
   __syncthreads();

@@ -449,6 +449,9 @@ int kda_gated_norm_fwd(const kda_norm_args* args, void* stream);
 int kda_gated_norm_bwd(const kda_norm_args* args, void* stream);
 int kda_residual_norm_fwd(const kda_norm_args* args, void* stream);
 int kda_residual_norm_bwd(const kda_norm_args* args, void* stream);
+/* Calls with many rows move them by bulk copies and wait for these a bounded number of polls.  Copies the status word of those kernels to *host_out and
+ * clears it (waits for the device: a diagnostic).  0: every wait completed; bit 0: one gave up, and the outputs of that call are incomplete. */
+int kda_norm_status(uint32_t* host_out);
 
 /* ------------------------------------------------------------------------------------------------
  * Strided host <-> device copy for the host-resident pipeline (no counterpart in the Python operator): `rows`

@@ -101,6 +101,7 @@ EXPORTS = (
     "kda_gate_bwd_workspace_bytes", "kda_gate_fwd", "kda_gate_bwd",
     "kda_delta_chunk_workspace_bytes", "kda_delta_chunk_bwd_workspace_bytes", "kda_delta_chunk_fwd", "kda_delta_chunk_bwd", "kda_delta_recurrent_fwd",
     "kda_norm_bwd_workspace_bytes", "kda_gated_norm_fwd", "kda_gated_norm_bwd", "kda_residual_norm_fwd", "kda_residual_norm_bwd",
+    "kda_norm_status",
     "kda_copy_rows_async", "kda_b200_profile_enable", "kda_b200_profile_read",
 )
 
@@ -168,6 +169,8 @@ def load() -> C.CDLL:
         fn = getattr(lib, name)
         fn.restype = C.c_int
         fn.argtypes = [C.POINTER(DeltaArgs), C.c_void_p]
+    lib.kda_norm_status.restype = C.c_int
+    lib.kda_norm_status.argtypes = [C.POINTER(C.c_uint32)]
     lib.kda_norm_bwd_workspace_bytes.restype = C.c_size_t
     lib.kda_norm_bwd_workspace_bytes.argtypes = [C.c_int64, C.c_int32, C.c_int32]
     for name in ("kda_gated_norm_fwd", "kda_gated_norm_bwd", "kda_residual_norm_fwd", "kda_residual_norm_bwd"):
@@ -207,6 +210,13 @@ def recurrent_status() -> int:
     """Status word of the bulk-copy decode kernel since the last call (0 = every bounded wait completed); synchronises."""
     v = C.c_uint32(0)
     check(load().kda_recurrent_status(C.byref(v)), "kda_recurrent_status")
+    return int(v.value)
+
+
+def norm_status() -> int:
+    """Status word of the norm kernels that move rows by bulk copies, since the last call (0 = every bounded wait completed); synchronises."""
+    v = C.c_uint32(0)
+    check(load().kda_norm_status(C.byref(v)), "kda_norm_status")
     return int(v.value)
 
 

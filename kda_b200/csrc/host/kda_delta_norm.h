@@ -136,6 +136,15 @@ void check_param(const Tensor& t, const char* name, int64_t cols) {
 }
 int code_or(const Tensor& t) { return t.defined() ? dtype_code(t) : KDA_FP32; }
 
+void check_norm_status(const char* what) {
+  uint32_t st = 0;
+  check_rc(kda_norm_status(&st), "kda_norm_status");
+  if (!st) return;
+  GilAcquire gil;
+  PyErr_SetString(g_kda_error ? g_kda_error : PyExc_RuntimeError, cat(what, ": device status ", st, " (a bounded wait gave up); the outputs are incomplete").c_str());
+  throw_current_python_error();
+}
+
 class GatedNormFunction : public torch::autograd::Function<GatedNormFunction> {
  public:
   static kda_norm_args args(const Tensor& x, const Tensor& gate, const Tensor& w, double eps, int act) {
@@ -151,6 +160,7 @@ class GatedNormFunction : public torch::autograd::Function<GatedNormFunction> {
     kda_norm_args a = args(x, gate, w, eps, act);
     a.y = ptr(y);
     check_rc(kda_gated_norm_fwd(&a, stream_of(x.device())), "kda_gated_norm_fwd");
+    if (checked_mode()) check_norm_status("kda_gated_norm_fwd");
     return y;
   }
   static Tensor forward(AutogradContext* ctx, const Tensor& x_, const Tensor& gate_, const std::optional<Tensor>& w_, double eps, int64_t act) {
@@ -177,6 +187,7 @@ class GatedNormFunction : public torch::autograd::Function<GatedNormFunction> {
       a.workspace = ptr(ws); a.workspace_bytes = static_cast<size_t>(ws.numel());
     }
     check_rc(kda_gated_norm_bwd(&a, stream_of(dev)), "kda_gated_norm_bwd");
+    if (checked_mode()) check_norm_status("kda_gated_norm_bwd");
     return {dx, dz, dw, Tensor(), Tensor()};
   }
 };
@@ -209,6 +220,7 @@ class ResidualNormFunction : public torch::autograd::Function<ResidualNormFuncti
     a.y = ptr(y);
     a.r = ptr(r);
     check_rc(kda_residual_norm_fwd(&a, stream_of(x.device())), "kda_residual_norm_fwd");
+    if (checked_mode()) check_norm_status("kda_residual_norm_fwd");
     return {y, r};
   }
   static variable_list forward(AutogradContext* ctx, const Tensor& x_, const Tensor& res_, const Tensor& w_, const std::optional<Tensor>& post_, const std::optional<Tensor>& scale_,
@@ -240,6 +252,7 @@ class ResidualNormFunction : public torch::autograd::Function<ResidualNormFuncti
       a.workspace = ptr(ws); a.workspace_bytes = static_cast<size_t>(ws.numel());
     }
     check_rc(kda_residual_norm_bwd(&a, stream_of(dev)), "kda_residual_norm_bwd");
+    if (checked_mode()) check_norm_status("kda_residual_norm_bwd");
     return {dx, dres, dw, dpost, dscale, Tensor(), Tensor()};
   }
 };

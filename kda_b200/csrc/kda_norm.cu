@@ -11,90 +11,18 @@
 // 2^n lanes of a warp (a warp has several rows in flight and no barrier), beyond that to a CTA.  The backward recomputes the norms from the inputs, which it
 // reads anyway, so the forward keeps nothing.  Sums over rows stay in registers while a CTA walks its rows; its partial sums are added in a second kernel in a
 // fixed order, so that gradients have the same bits on every run.  Columns that are no multiple of eight, or rows at odd addresses, are read one by one.
+// Calls with many rows take kda_norm_ring.cu's kernels, where rows travel through shared memory; these here serve the others (a decode step's 48 rows: no
+// ring to set up) and odd rows that are too wide for it.
 #include <algorithm>
 
-#include "kda_common.cuh"
-#include "kda_device.cuh"
+#include "kda_norm.cuh"
 
 namespace kda {
 
 namespace {
 
 constexpr int NORM_CTA = 256;           // threads of a CTA of the kernels for narrow rows
-constexpr int NORM_MOST = 8192;         // columns
 constexpr int NARROW = 256;             // columns up to which a row stays inside a warp
-
-struct Bits { uint4 a, b; };            // eight values as they stand in memory: fp32, or bf16 in a
-
-template <bool VEC>
-struct Cols {                           // which columns a thread has: vector i of a row whose threads are `lane` of `lanes`
-  int lane, lanes, cols;
-  __device__ __forceinline__ bool any(int i) const { return VEC ? (i * lanes + lane) * 8 < cols : i * 8 * lanes + lane < cols; }
-  __device__ __forceinline__ int at(int i, int j) const { return VEC ? (i * lanes + lane) * 8 + j : (i * 8 + j) * lanes + lane; }
-  __device__ __forceinline__ bool has(int i, int j) const { return VEC || at(i, j) < cols; }
-};
-
-template <bool VEC>
-__device__ __forceinline__ Bits fetch(const void* p, size_t row, int dtype, const Cols<VEC>& c, int i) {
-  Bits r{make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-  const size_t base = row * c.cols;
-  if constexpr (VEC) {
-    if (c.any(i)) {
-      if (dtype == KDA_BF16) r.a = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p) + base + c.at(i, 0));
-      else {
-        const uint4* q = reinterpret_cast<const uint4*>(static_cast<const float*>(p) + base + c.at(i, 0));
-        r.a = q[0];
-        r.b = q[1];
-      }
-    }
-  } else {
-    uint32_t w[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      w[j] = 0;
-      if (c.has(i, j)) w[j] = dtype == KDA_BF16 ? static_cast<const unsigned short*>(p)[base + c.at(i, j)] : static_cast<const uint32_t*>(p)[base + c.at(i, j)];
-    }
-    if (dtype == KDA_BF16) r.a = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
-    else {
-      r.a = make_uint4(w[0], w[1], w[2], w[3]);
-      r.b = make_uint4(w[4], w[5], w[6], w[7]);
-    }
-  }
-  return r;
-}
-__device__ __forceinline__ void values(const Bits& r, int dtype, float (&v)[8]) {
-  if (dtype == KDA_BF16) {
-    const float2 a = unpack_bf16(r.a.x), b = unpack_bf16(r.a.y), c = unpack_bf16(r.a.z), d = unpack_bf16(r.a.w);
-    v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y; v[4] = c.x; v[5] = c.y; v[6] = d.x; v[7] = d.y;
-  } else {
-    v[0] = __uint_as_float(r.a.x); v[1] = __uint_as_float(r.a.y); v[2] = __uint_as_float(r.a.z); v[3] = __uint_as_float(r.a.w);
-    v[4] = __uint_as_float(r.b.x); v[5] = __uint_as_float(r.b.y); v[6] = __uint_as_float(r.b.z); v[7] = __uint_as_float(r.b.w);
-  }
-}
-template <bool VEC>
-__device__ __forceinline__ void load8(const void* p, size_t row, int dtype, const Cols<VEC>& c, int i, float (&v)[8]) { values(fetch<VEC>(p, row, dtype, c, i), dtype, v); }
-template <bool VEC>
-__device__ __forceinline__ void store8(void* p, size_t row, int dtype, const Cols<VEC>& c, int i, const float (&v)[8]) {
-  if (!c.any(i)) return;
-  const size_t base = row * c.cols;
-  if constexpr (VEC) {
-    if (dtype == KDA_BF16) {
-      *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p) + base + c.at(i, 0)) =
-          make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
-    } else {
-      float4* q = reinterpret_cast<float4*>(static_cast<float*>(p) + base + c.at(i, 0));
-      q[0] = make_float4(v[0], v[1], v[2], v[3]);
-      q[1] = make_float4(v[4], v[5], v[6], v[7]);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (c.has(i, j)) {
-        if (dtype == KDA_BF16) static_cast<__nv_bfloat16*>(p)[base + c.at(i, j)] = __float2bfloat16_rn(v[j]);
-        else static_cast<float*>(p)[base + c.at(i, j)] = v[j];
-      }
-  }
-}
 
 // The sum over a row's threads of one value, in all of them.  Wide: through shared memory, in turns of two so that one barrier is enough.
 template <bool WIDE>
@@ -123,12 +51,6 @@ struct NormParams {
   float* partial;         // [CTAs][sums][cols]
   int lanes;              // threads of a row (narrow)
 };
-
-__device__ __forceinline__ void act_of(float z, int activation, float& act, float& slope) {
-  const float sg = sigmoid_fast(z);
-  act = activation == KDA_ACT_SILU ? z * sg : sg;
-  slope = activation == KDA_ACT_SILU ? sg * fmaf(z, 1.f - sg, 1.f) : sg * (1.f - sg);
-}
 
 // a CTA's sums over its rows -> partial[CTA][which][column]
 template <bool VEC, int NV, bool WIDE, int SUMS>
@@ -295,15 +217,6 @@ __global__ void __launch_bounds__(WIDE ? 512 : NORM_CTA) gated_bwd_kernel(const 
 }
 
 // ---- residual ----------------------------------------------------------------------------------------------------------------------------------
-// eight columns of a parameter (1 where there is none), of the scale (its one value where it is a number)
-template <bool VEC>
-__device__ __forceinline__ void param8(const void* p, int dtype, float other, const Cols<VEC>& c, int i, float (&v)[8]) {
-  if (p) load8<VEC>(p, 0, dtype, c, i, v);
-  else
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = other;
-}
-
 template <bool VEC, int NV, bool WIDE>
 __global__ void residual_fwd_kernel(const __grid_constant__ NormParams p) {
   __shared__ float part[2][32];
@@ -546,12 +459,6 @@ int check_norm(const kda_norm_args& a, bool gated, bool backward) {
   }
   return KDA_OK;
 }
-bool aligned16(std::initializer_list<const void*> ps) {
-  uintptr_t bits = 0;
-  for (const void* p : ps) bits |= reinterpret_cast<uintptr_t>(p);
-  return (bits & 15u) == 0;
-}
-
 int run_norm(const kda_norm_args& a, bool gated, bool backward, cudaStream_t st) {
   int rc = check_norm(a, gated, backward);
   if (rc != KDA_OK) return rc;
@@ -564,7 +471,10 @@ int run_norm(const kda_norm_args& a, bool gated, bool backward, cudaStream_t st)
   p.partial = sums ? static_cast<float*>(a.workspace) : nullptr;
   int ctas = 0;
   if (a.rows > 0) {
-    const bool vec = a.cols % 8 == 0 && aligned16({a.x, a.gate, a.residual, a.weight, a.post_weight, a.scale, a.y, a.r, a.dy, a.dr, a.dx, a.dgate, a.dresidual});
+    if (norm_ring_covers(a, gated, backward)) {
+      if ((rc = norm_ring(a, gated, backward, p.partial, &ctas, st)) != KDA_OK) return rc;
+    } else {
+    const bool vec = a.cols % 8 == 0 && norm_aligned(a);
     ctas = backward ? bwd_ctas(a.rows, s) : static_cast<int>(std::min<int64_t>((a.rows + s.per - 1) / s.per, static_cast<int64_t>(sm_count()) * 64));
     rc = with_shape(s, vec, [&](auto V, auto N, auto W) {
       if (gated) {
@@ -577,6 +487,7 @@ int run_norm(const kda_norm_args& a, bool gated, bool backward, cudaStream_t st)
       return static_cast<int>(cudaGetLastError());
     });
     if (rc != KDA_OK) return rc;
+    }
   }
   if (!sums) return KDA_OK;
   SumParams q{p.partial, {a.dweight, a.dpost_weight, a.dscale}, {a.weight_dtype, a.post_dtype, a.scale_dtype}, ctas, gated ? 1 : 3, a.cols};
@@ -589,8 +500,9 @@ int run_norm(const kda_norm_args& a, bool gated, bool backward, cudaStream_t st)
 
 extern "C" size_t kda_norm_bwd_workspace_bytes(int64_t rows, int32_t cols, int32_t sums) {
   if (rows < 0 || cols <= 0 || cols > kda::NORM_MOST || sums < 1 || sums > 3) return 0;
-  return static_cast<size_t>(std::max(1, kda::bwd_ctas(rows, kda::shape_of(cols)))) * sums * cols * sizeof(float);
+  return std::max<size_t>(std::max(1, kda::bwd_ctas(rows, kda::shape_of(cols))), kda::norm_ring_partials(cols)) * sums * cols * sizeof(float);
 }
+extern "C" int kda_norm_status(uint32_t* host_out) { return kda::norm_ring_status(host_out); }
 extern "C" int kda_gated_norm_fwd(const kda_norm_args* a, void* st) { return a ? kda::run_norm(*a, true, false, static_cast<cudaStream_t>(st)) : KDA_E_NULL; }
 extern "C" int kda_gated_norm_bwd(const kda_norm_args* a, void* st) { return a ? kda::run_norm(*a, true, true, static_cast<cudaStream_t>(st)) : KDA_E_NULL; }
 extern "C" int kda_residual_norm_fwd(const kda_norm_args* a, void* st) { return a ? kda::run_norm(*a, false, false, static_cast<cudaStream_t>(st)) : KDA_E_NULL; }

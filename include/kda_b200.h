@@ -434,7 +434,7 @@ typedef struct kda_norm_args {
   void* dweight;               /* out, backward: [cols] of the parameter's type, or NULL (as the next two) */
   void* dpost_weight;
   void* dscale;
-  void* workspace;             /* backward with a sum over rows: >= kda_norm_bwd_workspace_bytes(rows, cols, gated: 1, residual: 3) */
+  void* workspace;             /* backward with a sum over rows: >= kda_norm_bwd_workspace_bytes(rows, cols, gated: 1, residual: 2) */
   size_t workspace_bytes;
   int64_t rows;
   int32_t cols;

@@ -248,7 +248,7 @@ class ResidualNormFunction : public torch::autograd::Function<ResidualNormFuncti
     a.dy = ptr(dy); a.dr = ptr(dr); a.dx = ptr(dx); a.dresidual = ptr(dres); a.dweight = ptr(dw); a.dpost_weight = ptr(dpost); a.dscale = ptr(dscale);
     Tensor ws;
     if (dw.defined() || dpost.defined() || dscale.defined()) {
-      ws = bytes(kda_norm_bwd_workspace_bytes(a.rows, a.cols, 3), dev);
+      ws = bytes(kda_norm_bwd_workspace_bytes(a.rows, a.cols, 2), dev);
       a.workspace = ptr(ws); a.workspace_bytes = static_cast<size_t>(ws.numel());
     }
     check_rc(kda_residual_norm_bwd(&a, stream_of(dev)), "kda_residual_norm_bwd");

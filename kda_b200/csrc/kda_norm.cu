@@ -4,7 +4,7 @@
 //              dn = dy w act,  dx = (dn - n mean(dn n)) / rms(x),  dz = dy n w act'(z),  dw = sum over rows of dy n act
 //   residual   b = x, or n1 wp with n1 = x / rms(x);  r = residual + s b;  y = n w,  n = r / rms(r)        (between two blocks)
 //              t = dr + (dy w - n mean(dy w n)) / rms(r):  the gradient of the residual;  db = s t;  dx = db, or (db wp - n1 mean(db wp n1)) / rms(x)
-//              dw = sum of dy n,  dwp = sum of db n1,  ds = sum of t b
+//              dw = sum of dy n;  with A the sum of t n1 (n1 = x without a norm of its own):  dwp = s A,  ds = wp A
 //   rms(x) = sqrt(mean x^2 + eps).  All sums are fp32; every tensor may be bf16 or fp32 on its own.
 //
 // Bound by HBM: each tensor crosses it once.  A thread holds eight neighbouring columns (16 or 32 bytes) of a row; up to 256 columns a row belongs to
@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(WIDE ? 512 : NORM_CTA) residual_bwd_kernel(con
   const float inv = 1.f / a.cols;
   long long row, step, last;
   my_rows<WIDE>(p, row, step, last);
-  float acc[3][NV][8] = {};      // dw, dwp, ds
+  float acc[2][NV][8] = {};      // dw, A
   for (; row < last; row += step) {
     const bool there = row < a.rows;
     Bits bx[NV], br[NV], bdy[NV], bdr[NV];
@@ -356,8 +356,7 @@ __global__ void __launch_bounds__(WIDE ? 512 : NORM_CTA) residual_bwd_kernel(con
       for (int j = 0; j < 8; ++j) {
         t[i][j] = fmaf(rstd, fmaf(-dot, r[i][j], t[i][j]), dr[j]);
         const float n1 = x[j] * rstd1, db = s[j] * t[i][j];
-        acc[1][i][j] = there ? fmaf(db, n1, acc[1][i][j]) : acc[1][i][j];
-        acc[2][i][j] = there ? fmaf(t[i][j], n1 * wp[j], acc[2][i][j]) : acc[2][i][j];
+        acc[1][i][j] = there ? fmaf(t[i][j], n1, acc[1][i][j]) : acc[1][i][j];
         dn[i][j] = db * wp[j];
         dot1 = fmaf(dn[i][j], n1, dot1);
       }
@@ -377,30 +376,36 @@ __global__ void __launch_bounds__(WIDE ? 512 : NORM_CTA) residual_bwd_kernel(con
 #pragma unroll
     for (int i = 0; i < NV; ++i) store8<VEC>(a.dx, row, a.io_dtype, c, i, dn[i]);
   }
-  if (p.partial) leave_sums<VEC, NV, WIDE, 3>(p, c, acc);
+  if (p.partial) leave_sums<VEC, NV, WIDE, 2>(p, c, acc);
 }
 
 // ---- the CTAs' partial sums, in their order: 32 columns and 32 runs of CTAs per block --------------------------------------------------------------
 struct SumParams {
+  kda_norm_args a;
   const float* partial;
-  void* out[3];
-  int dtype[3];
-  int ctas, sums, cols;
+  int ctas, sums;
 };
-__global__ void __launch_bounds__(1024) norm_sums_kernel(const SumParams p) {
+__global__ void __launch_bounds__(1024) norm_sums_kernel(const __grid_constant__ SumParams p) {
   __shared__ float m[32][33];
+  const kda_norm_args& a = p.a;
   const int s = blockIdx.y, lane = threadIdx.x & 31, run = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
-  if (!p.out[s]) return;
   float x = 0.f;
-  if (col < p.cols)
-    for (int b = run; b < p.ctas; b += 32) x += p.partial[(static_cast<size_t>(b) * p.sums + s) * p.cols + col];
+  if (col < a.cols)
+    for (int b = run; b < p.ctas; b += 32) x += p.partial[(static_cast<size_t>(b) * p.sums + s) * a.cols + col];
   m[run][lane] = x;
   __syncthreads();
-  if (run == 0 && col < p.cols) {
-    x = 0.f;
-    for (int r = 0; r < 32; ++r) x += m[r][lane];
-    if (p.dtype[s] == KDA_BF16) static_cast<__nv_bfloat16*>(p.out[s])[col] = __float2bfloat16_rn(x);
-    else static_cast<float*>(p.out[s])[col] = x;
+  if (run != 0 || col >= a.cols) return;
+  x = 0.f;
+  for (int r = 0; r < 32; ++r) x += m[r][lane];
+  auto leave = [&](void* out, int dtype, float y) {
+    if (!out) return;
+    if (dtype == KDA_BF16) static_cast<__nv_bfloat16*>(out)[col] = __float2bfloat16_rn(y);
+    else static_cast<float*>(out)[col] = y;
+  };
+  if (s == 0) leave(a.dweight, a.weight_dtype, x);
+  else {
+    leave(a.dpost_weight, a.post_dtype, x * (a.scale ? load_raw(a.scale, col, a.scale_dtype) : a.scale_value));
+    leave(a.dscale, a.scale_dtype, x * (a.post_weight ? load_raw(a.post_weight, col, a.post_dtype) : 1.f));
   }
 }
 
@@ -455,7 +460,7 @@ int check_norm(const kda_norm_args& a, bool gated, bool backward) {
   if (backward && (a.dweight || a.dpost_weight || a.dscale)) {
     if (!a.workspace) return KDA_E_NULL;
     if (reinterpret_cast<uintptr_t>(a.workspace) & 15u) return KDA_E_ALIGN;
-    if (a.workspace_bytes < kda_norm_bwd_workspace_bytes(a.rows, a.cols, gated ? 1 : 3)) return KDA_E_WORKSPACE;
+    if (a.workspace_bytes < kda_norm_bwd_workspace_bytes(a.rows, a.cols, gated ? 1 : 2)) return KDA_E_WORKSPACE;
   }
   return KDA_OK;
 }
@@ -490,7 +495,7 @@ int run_norm(const kda_norm_args& a, bool gated, bool backward, cudaStream_t st)
     }
   }
   if (!sums) return KDA_OK;
-  SumParams q{p.partial, {a.dweight, a.dpost_weight, a.dscale}, {a.weight_dtype, a.post_dtype, a.scale_dtype}, ctas, gated ? 1 : 3, a.cols};
+  const SumParams q{a, p.partial, ctas, gated ? 1 : 2};
   norm_sums_kernel<<<dim3((a.cols + 31) / 32, q.sums), 1024, 0, st>>>(q);
   return static_cast<int>(cudaGetLastError());
 }
@@ -499,7 +504,7 @@ int run_norm(const kda_norm_args& a, bool gated, bool backward, cudaStream_t st)
 }  // namespace kda
 
 extern "C" size_t kda_norm_bwd_workspace_bytes(int64_t rows, int32_t cols, int32_t sums) {
-  if (rows < 0 || cols <= 0 || cols > kda::NORM_MOST || sums < 1 || sums > 3) return 0;
+  if (rows < 0 || cols <= 0 || cols > kda::NORM_MOST || sums < 1 || sums > 2) return 0;
   return std::max<size_t>(std::max(1, kda::bwd_ctas(rows, kda::shape_of(cols))), kda::norm_ring_partials(cols)) * sums * cols * sizeof(float);
 }
 extern "C" int kda_norm_status(uint32_t* host_out) { return kda::norm_ring_status(host_out); }

@@ -15,55 +15,65 @@ namespace {
 // Bit 0: a bounded wait on a stage gave up (the call's results are incomplete).
 __device__ unsigned g_norm_status = 0;
 
-constexpr int RING_MOST = 200 * 1024, STAGES_MOST = 4;
+constexpr int RING_MOST = 224 * 1024, RING_STAGE = 32 * 1024, STAGES_MOST = 4;
 
 // The sum over a row's threads, in all of them.  More than a warp: through shared memory, in turns of two so that one barrier is enough.
 struct GroupSum {
   float* part;      // [2][16] of this group
-  int lanes, bar, turn = 0;
+  int lanes, bar, warp, turn = 0;      // warp: of the row's
   __device__ __forceinline__ float operator()(float x) {
     if (lanes <= 32) {
-      for (int o = lanes >> 1; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1)
+        if (lanes > o) x += __shfl_xor_sync(0xffffffffu, x, o);
       return x;
     }
     x = warp_sum(x);
-    const int warps = lanes >> 5, warp = (threadIdx.x >> 5) % warps;
-    if ((threadIdx.x & 31) == 0) part[16 * turn + warp] = x;
+    float* const p = part + 16 * turn;      // (places of warps that there are not hold zeros)
+    if ((threadIdx.x & 31) == 0) p[warp] = x;
     asm volatile("bar.sync %0, %1;" ::"r"(bar), "r"(lanes) : "memory");
-    x = 0.f;
-    for (int w = 0; w < warps; ++w) x += part[16 * turn + w];
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    x = (a.x + a.y) + (a.z + a.w) + ((b.x + b.y) + (b.z + b.w));
+    if (lanes > 256) {
+      const float4 c = *reinterpret_cast<const float4*>(p + 8), d = *reinterpret_cast<const float4*>(p + 12);
+      x += (c.x + c.y) + (c.z + c.w) + ((d.x + d.y) + (d.z + d.w));
+    }
     turn ^= 1;
     return x;
   }
 };
 
-// vector i of a thread's columns in a row in shared memory
-template <bool VEC>
-__device__ __forceinline__ void get8(const unsigned char* row, int dtype, const Cols<VEC>& c, int i, float (&v)[8]) {
+constexpr int NV = 2;      // vectors of eight columns per thread: what a thread does once a row (sums, addresses) it does for sixteen columns
+
+// vector i of a thread's columns in a row in shared memory, of type T (KDA_BF16 or KDA_FP32)
+template <int T, bool VEC>
+__device__ __forceinline__ void get8(const unsigned char* row, const Cols<VEC>& c, int i, float (&v)[8]) {
   if constexpr (VEC) {
-    if (!c.any(i)) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = 0.f;
-      return;
+    Bits b{make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+    if (c.any(i)) {
+      if constexpr (T == KDA_BF16) b.a = *reinterpret_cast<const uint4*>(row + 2 * c.at(i, 0));
+      else {
+        b.a = *reinterpret_cast<const uint4*>(row + 4 * c.at(i, 0));
+        b.b = *reinterpret_cast<const uint4*>(row + 4 * c.at(i, 0) + 16);
+      }
     }
-    Bits b;
-    if (dtype == KDA_BF16) b.a = *reinterpret_cast<const uint4*>(row + 2 * c.at(i, 0));
-    else {
-      b.a = *reinterpret_cast<const uint4*>(row + 4 * c.at(i, 0));
-      b.b = *reinterpret_cast<const uint4*>(row + 4 * c.at(i, 0) + 16);
-    }
-    values(b, dtype, v);
+    values(b, T, v);
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      v[j] = !c.has(i, j) ? 0.f : dtype == KDA_BF16 ? __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(row + 2 * c.at(i, j))) : *reinterpret_cast<const float*>(row + 4 * c.at(i, j));
+    for (int j = 0; j < 8; ++j) {
+      v[j] = 0.f;
+      if (c.has(i, j)) {
+        if constexpr (T == KDA_BF16) v[j] = __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(row + 2 * c.at(i, j)));
+        else v[j] = *reinterpret_cast<const float*>(row + 4 * c.at(i, j));
+      }
+    }
   }
 }
-template <bool VEC>
-__device__ __forceinline__ void put8(unsigned char* row, int dtype, const Cols<VEC>& c, int i, const float (&v)[8]) {
+template <int T, bool VEC>
+__device__ __forceinline__ void put8(unsigned char* row, const Cols<VEC>& c, int i, const float (&v)[8]) {
   if constexpr (VEC) {
     if (!c.any(i)) return;
-    if (dtype == KDA_BF16) {
+    if constexpr (T == KDA_BF16) {
       *reinterpret_cast<uint4*>(row + 2 * c.at(i, 0)) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
     } else {
       *reinterpret_cast<float4*>(row + 4 * c.at(i, 0)) = make_float4(v[0], v[1], v[2], v[3]);
@@ -73,21 +83,35 @@ __device__ __forceinline__ void put8(unsigned char* row, int dtype, const Cols<V
 #pragma unroll
     for (int j = 0; j < 8; ++j)
       if (c.has(i, j)) {
-        if (dtype == KDA_BF16) *reinterpret_cast<__nv_bfloat16*>(row + 2 * c.at(i, j)) = __float2bfloat16_rn(v[j]);
+        if constexpr (T == KDA_BF16) *reinterpret_cast<__nv_bfloat16*>(row + 2 * c.at(i, j)) = __float2bfloat16_rn(v[j]);
         else *reinterpret_cast<float*>(row + 4 * c.at(i, j)) = v[j];
       }
   }
 }
+// A parameter in shared memory, as fp32.  VEC: the first four of every eight columns, then the others, so that neighbours read neighbouring 16 bytes.
+template <bool VEC>
+__device__ __forceinline__ int param_at(int col, int cols) { return VEC ? ((col & 4) ? cols / 2 : 0) + (col >> 3) * 4 + (col & 3) : col; }
+template <bool VEC>
+__device__ __forceinline__ void get_param(const float* p, const Cols<VEC>& c, int i, float (&v)[8]) {
+  if constexpr (VEC) {
+    const float* const q = p + (c.any(i) ? c.at(i, 0) / 2 : 0);
+    const float4 a = *reinterpret_cast<const float4*>(q), b = *reinterpret_cast<const float4*>(q + c.cols / 2);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = c.has(i, j) ? p[c.at(i, j)] : 0.f;
+  }
+}
 
 // A row of the gated norm.  x, z, d: the row of x, of the gate, of dy; results over x and z.
-template <bool VEC, int NV, bool BWD>
-__device__ __forceinline__ void gated_row(const kda_norm_args& a, const Cols<VEC>& c, GroupSum& sum, bool there, unsigned char* x_, unsigned char* z_, const unsigned char* d_,
-                                          float (&acc)[3][NV][8]) {
+template <int XT, int ZT, bool VEC, bool BWD>
+__device__ __forceinline__ void gated_row(const kda_norm_args& a, const float* w_, const Cols<VEC>& c, GroupSum& sum, bool there, unsigned char* x_, unsigned char* z_,
+                                          const unsigned char* d_, float (&acc)[2][NV][8]) {
   const float inv = 1.f / a.cols;
   float x[NV][8], ss = 0.f;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    get8<VEC>(x_, a.io_dtype, c, i, x[i]);
+    get8<XT, VEC>(x_, c, i, x[i]);
 #pragma unroll
     for (int j = 0; j < 8; ++j) ss = fmaf(x[i][j], x[i][j], ss);
   }
@@ -97,35 +121,36 @@ __device__ __forceinline__ void gated_row(const kda_norm_args& a, const Cols<VEC
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       float z[8], w[8];
-      get8<VEC>(z_, a.gate_dtype, c, i, z);
-      param8<VEC>(a.weight, a.weight_dtype, 1.f, c, i, w);
+      get8<ZT, VEC>(z_, c, i, z);
+      get_param<VEC>(w_, c, i, w);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         float act, slope;
         act_of(z[j], a.activation, act, slope);
         z[j] = x[i][j] * rstd * w[j] * act;
       }
-      put8<VEC>(x_, a.io_dtype, c, i, z);
+      put8<XT, VEC>(x_, c, i, z);
     }
   } else {
     float dn[NV][8], dot = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       float z[8], d[8], w[8];
-      get8<VEC>(z_, a.gate_dtype, c, i, z);
-      get8<VEC>(d_, a.io_dtype, c, i, d);
-      param8<VEC>(a.weight, a.weight_dtype, 1.f, c, i, w);
+      get8<ZT, VEC>(z_, c, i, z);
+      get8<XT, VEC>(d_, c, i, d);
+      get_param<VEC>(w_, c, i, w);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         float act, slope;
         act_of(z[j], a.activation, act, slope);
         x[i][j] *= rstd;
-        if (there) acc[0][i][j] = fmaf(d[j] * x[i][j], act, acc[0][i][j]);
-        dn[i][j] = d[j] * w[j] * act;
-        z[j] = d[j] * w[j] * x[i][j] * slope;
+        const float da = d[j] * act, dx = d[j] * x[i][j] * w[j];
+        if (there) acc[0][i][j] = fmaf(da, x[i][j], acc[0][i][j]);
+        dn[i][j] = da * w[j];
         dot = fmaf(dn[i][j], x[i][j], dot);
+        z[j] = dx * slope;
       }
-      if (there) put8<VEC>(z_, a.gate_dtype, c, i, z);
+      if (there) put8<ZT, VEC>(z_, c, i, z);
     }
     dot = sum(dot) * inv;
     if (!there) return;
@@ -133,19 +158,19 @@ __device__ __forceinline__ void gated_row(const kda_norm_args& a, const Cols<VEC
     for (int i = 0; i < NV; ++i) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) dn[i][j] = rstd * fmaf(-dot, x[i][j], dn[i][j]);
-      put8<VEC>(x_, a.io_dtype, c, i, dn[i]);
+      put8<XT, VEC>(x_, c, i, dn[i]);
     }
   }
 }
 
-// A row of the residual norm.  x, r, dy, dr: the row of x, of the residual, of their gradients (or NULL); results over x and r.
-template <bool VEC, int NV, bool BWD>
-__device__ __forceinline__ void residual_row(const kda_norm_args& a, const Cols<VEC>& c, GroupSum& sum, bool there, unsigned char* x_, unsigned char* r_, const unsigned char* dy_,
-                                             const unsigned char* dr_, float (&acc)[3][NV][8]) {
+// A row of the residual norm.  x, r, dy, dr: the row of x, of the residual, of their gradients (or NULL); results over x and r.  sw: scale times post_weight.
+template <int XT, int RT, bool VEC, bool BWD>
+__device__ __forceinline__ void residual_row(const kda_norm_args& a, const float* w_, const float* sw_, const Cols<VEC>& c, GroupSum& sum, bool there, unsigned char* x_,
+                                             unsigned char* r_, const unsigned char* dy_, const unsigned char* dr_, float (&acc)[2][NV][8]) {
   const float inv = 1.f / a.cols;
   float x[NV][8], rstd1 = 1.f, ss = 0.f;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) get8<VEC>(x_, a.io_dtype, c, i, x[i]);
+  for (int i = 0; i < NV; ++i) get8<XT, VEC>(x_, c, i, x[i]);
   if (a.post_weight) {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
@@ -157,14 +182,13 @@ __device__ __forceinline__ void residual_row(const kda_norm_args& a, const Cols<
   ss = 0.f;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    float wp[8], s[8];
-    get8<VEC>(r_, a.residual_dtype, c, i, r[i]);
-    param8<VEC>(a.post_weight, a.post_dtype, 1.f, c, i, wp);
-    param8<VEC>(a.scale, a.scale_dtype, a.scale_value, c, i, s);
+    float sw[8];
+    get8<RT, VEC>(r_, c, i, r[i]);
+    get_param<VEC>(sw_, c, i, sw);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       x[i][j] *= rstd1;
-      r[i][j] = fmaf(s[j], x[i][j] * wp[j], r[i][j]);      // (columns that are not there: x and the residual read as zero)
+      r[i][j] = fmaf(sw[j], x[i][j], r[i][j]);      // (columns that are not there: x and the residual read as zero)
       ss = fmaf(r[i][j], r[i][j], ss);
     }
   }
@@ -174,22 +198,22 @@ __device__ __forceinline__ void residual_row(const kda_norm_args& a, const Cols<
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       float w[8];
-      put8<VEC>(r_, a.residual_dtype, c, i, r[i]);
-      param8<VEC>(a.weight, a.weight_dtype, 1.f, c, i, w);
+      put8<RT, VEC>(r_, c, i, r[i]);
+      get_param<VEC>(w_, c, i, w);
 #pragma unroll
       for (int j = 0; j < 8; ++j) w[j] *= r[i][j] * rstd;
-      put8<VEC>(x_, a.io_dtype, c, i, w);
+      put8<XT, VEC>(x_, c, i, w);
     }
   } else {
     float t[NV][8], dot = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       float w[8];
-      if (dy_) get8<VEC>(dy_, a.io_dtype, c, i, t[i]);
+      if (dy_) get8<XT, VEC>(dy_, c, i, t[i]);
       else
 #pragma unroll
         for (int j = 0; j < 8; ++j) t[i][j] = 0.f;
-      param8<VEC>(a.weight, a.weight_dtype, 1.f, c, i, w);
+      get_param<VEC>(w_, c, i, w);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         r[i][j] *= rstd;
@@ -202,25 +226,20 @@ __device__ __forceinline__ void residual_row(const kda_norm_args& a, const Cols<
     float dot1 = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      float wp[8], s[8], dr[8];
-      if (dr_) get8<VEC>(dr_, a.residual_dtype, c, i, dr);
+      float sw[8], dr[8];
+      if (dr_) get8<RT, VEC>(dr_, c, i, dr);
       else
 #pragma unroll
         for (int j = 0; j < 8; ++j) dr[j] = 0.f;
-      param8<VEC>(a.post_weight, a.post_dtype, 1.f, c, i, wp);
-      param8<VEC>(a.scale, a.scale_dtype, a.scale_value, c, i, s);
+      get_param<VEC>(sw_, c, i, sw);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         t[i][j] = fmaf(rstd, fmaf(-dot, r[i][j], t[i][j]), dr[j]);
-        const float db = s[j] * t[i][j];
-        if (there) {
-          acc[1][i][j] = fmaf(db, x[i][j], acc[1][i][j]);
-          acc[2][i][j] = fmaf(t[i][j], x[i][j] * wp[j], acc[2][i][j]);
-        }
-        r[i][j] = db * wp[j];      // (now the gradient of n1)
+        if (there) acc[1][i][j] = fmaf(t[i][j], x[i][j], acc[1][i][j]);
+        r[i][j] = sw[j] * t[i][j];      // (now the gradient of n1)
         dot1 = fmaf(r[i][j], x[i][j], dot1);
       }
-      if (there) put8<VEC>(r_, a.residual_dtype, c, i, t[i]);
+      if (there) put8<RT, VEC>(r_, c, i, t[i]);
     }
     if (a.post_weight) {
       dot1 = sum(dot1) * inv;
@@ -231,7 +250,7 @@ __device__ __forceinline__ void residual_row(const kda_norm_args& a, const Cols<
     }
     if (!there) return;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) put8<VEC>(x_, a.io_dtype, c, i, r[i]);
+    for (int i = 0; i < NV; ++i) put8<XT, VEC>(x_, c, i, r[i]);
   }
 }
 
@@ -239,29 +258,38 @@ struct RingParams {
   kda_norm_args a;
   float* partial;                 // [CTAs * groups][sums][cols] or NULL
   int lanes, groups;              // threads of a row, rows at a time
+  int params;                     // bytes of the parameters in front of the stages
   int rows, stages, stage_bytes;  // rows of a stage
   long long chunks;
-  int n;                          // tensors that are read: x, gate or residual, dy, dr
-  const void* in[4];
+  const void* in[4];              // x; gate or residual; dy; dr (NULL: not read)
   void* out[2];                   // over the first and the second one
   int size[4], off[4];            // bytes of an element; where a stage has it
 };
 
 }  // namespace
 
-template <bool GATED, bool VEC, int NV, bool BWD>
+template <bool GATED, int XT, int ZT, bool VEC, bool BWD>
 __global__ void __launch_bounds__(544, 1) norm_ring_kernel(const __grid_constant__ RingParams p) {
-  extern __shared__ __align__(128) unsigned char smem[];
+  extern __shared__ __align__(128) unsigned char smem_raw[];
   __shared__ uint64_t full[STAGES_MOST], done[STAGES_MOST];
-  __shared__ float part[16][32];
+  __shared__ __align__(16) float part[16][32];
   const kda_norm_args& a = p.a;
   const int warps = (blockDim.x >> 5) - 1, warp = threadIdx.x >> 5;
+  float* const w_ = reinterpret_cast<float*>(smem_raw);
+  float* const sw_ = w_ + a.cols;
+  unsigned char* const smem = smem_raw + p.params;
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES_MOST; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&done[s], warps);
     }
     fence_mbar_init();
+  }
+  for (int e = threadIdx.x; e < 16 * 32; e += blockDim.x) part[e / 32][e % 32] = 0.f;
+  for (int e = threadIdx.x; e < a.cols; e += blockDim.x) {
+    w_[param_at<VEC>(e, a.cols)] = a.weight ? load_raw(a.weight, e, a.weight_dtype) : 1.f;
+    if constexpr (!GATED)
+      sw_[param_at<VEC>(e, a.cols)] = (a.scale ? load_raw(a.scale, e, a.scale_dtype) : a.scale_value) * (a.post_weight ? load_raw(a.post_weight, e, a.post_dtype) : 1.f);
   }
   __syncthreads();
   if (warp == warps) {
@@ -272,7 +300,8 @@ __global__ void __launch_bounds__(544, 1) norm_ring_kernel(const __grid_constant
         unsigned char* const st = smem + s * p.stage_bytes;
         const int rows = rows_of(c);
         unsigned tx = 0;
-        for (int i = 0; i < p.n; ++i) {
+        for (int i = 0; i < 4; ++i) {
+          if (!p.in[i]) continue;
           const int bytes = rows * a.cols * p.size[i];
           const unsigned char* const src = static_cast<const unsigned char*>(p.in[i]) + static_cast<size_t>(c) * p.rows * a.cols * p.size[i];
           for (int b = bytes & ~15; b < bytes; b += 2)      // the end of the last rows: what is no 16 bytes
@@ -280,9 +309,9 @@ __global__ void __launch_bounds__(544, 1) norm_ring_kernel(const __grid_constant
           tx += bytes & ~15;
         }
         mbar_expect_tx(&full[s], tx);
-        for (int i = 0; i < p.n; ++i) {
+        for (int i = 0; i < 4; ++i) {
           const int bytes = rows * a.cols * p.size[i] & ~15;
-          if (bytes) bulk_g2s(st + p.off[i], static_cast<const unsigned char*>(p.in[i]) + static_cast<size_t>(c) * p.rows * a.cols * p.size[i], bytes, &full[s]);
+          if (p.in[i] && bytes) bulk_g2s(st + p.off[i], static_cast<const unsigned char*>(p.in[i]) + static_cast<size_t>(c) * p.rows * a.cols * p.size[i], bytes, &full[s]);
         }
       };
       auto store = [&](long long c, int s) {
@@ -319,31 +348,37 @@ __global__ void __launch_bounds__(544, 1) norm_ring_kernel(const __grid_constant
   }
   const int group = threadIdx.x / p.lanes;
   const Cols<VEC> c{static_cast<int>(threadIdx.x) % p.lanes, p.lanes, a.cols};
-  GroupSum sum{part[group & 15], p.lanes, 1 + (group & 15)};
-  float acc[3][NV][8] = {};
-  int k = 0;
+  GroupSum sum{part[group & 15], p.lanes, 1 + (group & 15), c.lane >> 5};
+  float acc[2][NV][8] = {};
+  constexpr int XS = XT == KDA_BF16 ? 2 : 4, ZS = ZT == KDA_BF16 ? 2 : 4;
+  int k = 0, s = 0, next = group;      // next: this group's next row of the stage
   bool ok = true;
-  for (long long ch = blockIdx.x; ch < p.chunks; ch += gridDim.x, ++k) {
-    const int s = k % p.stages;
-    if (!(ok = __all_sync(0xffffffffu, mbar_wait(&full[s], (k / p.stages) & 1)))) break;
+  for (long long ch = blockIdx.x; ch < p.chunks; ch += gridDim.x) {
+    if (!(ok = __all_sync(0xffffffffu, mbar_wait(&full[s], k & 1)))) break;
     unsigned char* const st = smem + s * p.stage_bytes;
     const long long left = a.rows - ch * p.rows;
-    for (int r = group; r < p.rows; r += p.groups) {      // the same number of turns for all of a warp
+    int r = next;
+    for (; r < p.rows; r += p.groups) {      // (groups that share a warp take the same number of turns)
       const bool there = r < left;
       const int at = there ? r * a.cols : 0;
       if constexpr (GATED)
-        gated_row<VEC, NV, BWD>(a, c, sum, there, st + p.off[0] + at * p.size[0], st + p.off[1] + at * p.size[1], BWD ? st + p.off[2] + at * p.size[2] : nullptr, acc);
+        gated_row<XT, ZT, VEC, BWD>(a, w_, c, sum, there, st + p.off[0] + at * XS, st + p.off[1] + at * ZS, st + p.off[2] + at * XS, acc);
       else
-        residual_row<VEC, NV, BWD>(a, c, sum, there, st + p.off[0] + at * p.size[0], st + p.off[1] + at * p.size[1], BWD && a.dy ? st + p.off[2] + at * p.size[2] : nullptr,
-                                   BWD && a.dr ? st + p.off[a.dy ? 3 : 2] + at * p.size[a.dy ? 3 : 2] : nullptr, acc);
+        residual_row<XT, ZT, VEC, BWD>(a, w_, sw_, c, sum, there, st + p.off[0] + at * XS, st + p.off[1] + at * ZS, a.dy ? st + p.off[2] + at * XS : nullptr,
+                                       a.dr ? st + p.off[3] + at * ZS : nullptr, acc);
     }
+    next = r - p.rows;
     fence_proxy_async();
     __syncwarp();
     if ((threadIdx.x & 31) == 0) mbar_arrive(&done[s]);
+    if (++s == p.stages) {
+      s = 0;
+      ++k;
+    }
   }
   if (!ok && (threadIdx.x & 31) == 0) atomicOr(&g_norm_status, 1u);
   if (BWD && p.partial && ok) {
-    constexpr int SUMS = GATED ? 1 : 3;
+    constexpr int SUMS = GATED ? 1 : 2;
     float* const out = p.partial + static_cast<size_t>(blockIdx.x * p.groups + group) * SUMS * a.cols;
 #pragma unroll
     for (int i = 0; i < SUMS; ++i)
@@ -364,45 +399,45 @@ int norm_ring_status(uint32_t* host_out) {
   return static_cast<int>(e);
 }
 
+// threads of a row and rows at a time
+static void split(int cols, int& lanes, int& groups) {
+  const int need = (cols + 8 * NV - 1) / (8 * NV);
+  for (lanes = 1; lanes < need && lanes < 32; lanes *= 2) {}
+  if (need > 32) lanes = (need + 31) / 32 * 32;
+  groups = 512 / lanes;
+}
+
 // How a call goes through the ring: false where its rows are too wide for two stages.
 static bool plan(const kda_norm_args& a, bool gated, bool backward, RingParams& p) {
-  auto size = [](int dtype) { return dtype == KDA_BF16 ? 2 : 4; };
-  p.n = 0;
-  auto add = [&](const void* t, int dtype) {
-    p.in[p.n] = t;
-    p.size[p.n++] = size(dtype);
-  };
-  add(a.x, a.io_dtype);
-  add(gated ? a.gate : a.residual, gated ? a.gate_dtype : a.residual_dtype);
-  if (backward && a.dy) add(a.dy, a.io_dtype);
-  if (backward && !gated && a.dr) add(a.dr, a.residual_dtype);
+  const int other = gated ? a.gate_dtype : a.residual_dtype;
+  p.in[0] = a.x;
+  p.in[1] = gated ? a.gate : a.residual;
+  p.in[2] = backward ? a.dy : nullptr;
+  p.in[3] = backward && !gated ? a.dr : nullptr;
+  p.size[0] = p.size[2] = a.io_dtype == KDA_BF16 ? 2 : 4;
+  p.size[1] = p.size[3] = other == KDA_BF16 ? 2 : 4;
   p.out[0] = backward ? a.dx : a.y;
   p.out[1] = backward ? (gated ? a.dgate : a.dresidual) : (gated ? nullptr : a.r);
-  int per_row = 0, narrow = 4;
-  for (int i = 0; i < p.n; ++i) {
-    per_row += p.size[i] * a.cols;
-    narrow = std::min(narrow, p.size[i]);
-  }
-  const int nv = a.cols <= 4096 ? 1 : 2, need = (a.cols + 8 * nv - 1) / (8 * nv);
-  if (need <= 32) {
-    for (p.lanes = 1; p.lanes < need; p.lanes *= 2) {}
-    p.groups = 512 / p.lanes;
-  } else {
-    p.lanes = (need + 31) / 32 * 32;
-    p.groups = 512 / p.lanes;
-  }
+  split(a.cols, p.lanes, p.groups);
+  int per_row = 0;
+  for (int i = 0; i < 4; ++i)
+    if (p.in[i]) per_row += p.size[i] * a.cols;
   int even = 1;      // rows that make 16 bytes even
-  while (even * a.cols * narrow % 16) even *= 2;
-  const int step = std::max(even, p.groups);      // (both are powers of two, or groups is one of 1, 2, 3, 5 with even <= 8)
-  const int unit = step % even ? step * even : step;
+  while (even * a.cols * std::min(p.size[0], p.size[1]) % 16) even *= 2;
+  p.params = (a.cols * (gated ? 4 : 8) + 127) / 128 * 128;
+  const int room = RING_MOST - p.params;
+  // a row for every group in each stage; it has to be so where groups share a warp, elsewhere if all stages fit
+  int unit = even;
+  while (unit % p.groups) unit += even;
+  if (p.lanes > 32 && static_cast<long long>(STAGES_MOST) * unit * per_row > room) unit = even;
   p.rows = unit;
-  while (p.rows * per_row < 24 * 1024 && (p.rows + unit) * per_row <= RING_MOST / 4) p.rows += unit;
+  while (p.rows * per_row < RING_STAGE && (p.rows + unit) * per_row <= room / STAGES_MOST) p.rows += unit;
   p.stage_bytes = 0;
-  for (int i = 0; i < p.n; ++i) {
+  for (int i = 0; i < 4; ++i) {
     p.off[i] = p.stage_bytes;
-    p.stage_bytes += (p.rows * a.cols * p.size[i] + 127) / 128 * 128;
+    if (p.in[i]) p.stage_bytes += (p.rows * a.cols * p.size[i] + 127) / 128 * 128;
   }
-  p.stages = std::min(STAGES_MOST, RING_MOST / p.stage_bytes);
+  p.stages = std::min(STAGES_MOST, room / std::max(1, p.stage_bytes));
   p.chunks = (a.rows + p.rows - 1) / p.rows;
   return p.stages >= 2;
 }
@@ -410,26 +445,35 @@ static bool plan(const kda_norm_args& a, bool gated, bool backward, RingParams& 
 static unsigned ring_ctas(const RingParams& p) { return static_cast<unsigned>(std::min<long long>(p.chunks, sm_count())); }
 
 bool norm_ring_covers(const kda_norm_args& a, bool gated, bool backward) {
-  if (a.rows * a.cols < NORM_RING_MIN || !norm_aligned(a)) return false;
+  if (a.rows * a.cols < NORM_RING_MIN || !norm_aligned(a) || (a.io_dtype == KDA_FP32 && (gated ? a.gate_dtype : a.residual_dtype) == KDA_BF16)) return false;
   RingParams p{};
   return plan(a, gated, backward, p);
 }
-// the most partial sums of a call: groups never exceed 512, CTAs the SMs
+// the most partial sums of a call: their number depends on the columns alone
 size_t norm_ring_partials(int cols) {
-  kda_norm_args a{};
-  a.cols = cols;
-  RingParams p{};
-  plan(a, true, false, p);
-  return static_cast<size_t>(sm_count()) * p.groups;
+  int lanes, groups;
+  split(cols, lanes, groups);
+  return static_cast<size_t>(sm_count()) * groups;
 }
 
-template <bool GATED, bool VEC, int NV, bool BWD>
+template <bool GATED, int XT, int ZT, bool VEC, bool BWD>
 static int launch_ring(const RingParams& p, cudaStream_t st) {
   static DeviceOnce once;
-  const int rc = once.run([] { return cudaFuncSetAttribute(norm_ring_kernel<GATED, VEC, NV, BWD>, cudaFuncAttributeMaxDynamicSharedMemorySize, RING_MOST); });
+  const int rc = once.run([] { return cudaFuncSetAttribute(norm_ring_kernel<GATED, XT, ZT, VEC, BWD>, cudaFuncAttributeMaxDynamicSharedMemorySize, RING_MOST); });
   if (rc != KDA_OK) return rc;
-  norm_ring_kernel<GATED, VEC, NV, BWD><<<ring_ctas(p), p.lanes * p.groups + 32, p.stages * p.stage_bytes, st>>>(p);
+  norm_ring_kernel<GATED, XT, ZT, VEC, BWD><<<ring_ctas(p), p.lanes * p.groups + 32, p.params + p.stages * p.stage_bytes, st>>>(p);
   return static_cast<int>(cudaGetLastError());
+}
+template <bool GATED, int XT, int ZT>
+static int launch_types(const RingParams& p, bool backward, cudaStream_t st) {
+  if (p.a.cols % 8 == 0) return backward ? launch_ring<GATED, XT, ZT, true, true>(p, st) : launch_ring<GATED, XT, ZT, true, false>(p, st);
+  return backward ? launch_ring<GATED, XT, ZT, false, true>(p, st) : launch_ring<GATED, XT, ZT, false, false>(p, st);
+}
+template <bool GATED>
+static int launch_norm(const RingParams& p, bool backward, cudaStream_t st) {
+  if (p.a.io_dtype == KDA_FP32) return launch_types<GATED, KDA_FP32, KDA_FP32>(p, backward, st);
+  return (GATED ? p.a.gate_dtype : p.a.residual_dtype) == KDA_BF16 ? launch_types<GATED, KDA_BF16, KDA_BF16>(p, backward, st)
+                                                                     : launch_types<GATED, KDA_BF16, KDA_FP32>(p, backward, st);
 }
 
 int norm_ring(const kda_norm_args& a, bool gated, bool backward, float* partial, int* partials, cudaStream_t st) {
@@ -438,25 +482,7 @@ int norm_ring(const kda_norm_args& a, bool gated, bool backward, float* partial,
   p.a = a;
   p.partial = partial;
   *partials = static_cast<int>(ring_ctas(p)) * p.groups;
-  const int which = (gated ? 8 : 0) + (a.cols % 8 == 0 ? 4 : 0) + (a.cols > 4096 ? 2 : 0) + (backward ? 1 : 0);
-  switch (which) {
-    case 0: return launch_ring<false, false, 1, false>(p, st);
-    case 1: return launch_ring<false, false, 1, true>(p, st);
-    case 2: return launch_ring<false, false, 2, false>(p, st);
-    case 3: return launch_ring<false, false, 2, true>(p, st);
-    case 4: return launch_ring<false, true, 1, false>(p, st);
-    case 5: return launch_ring<false, true, 1, true>(p, st);
-    case 6: return launch_ring<false, true, 2, false>(p, st);
-    case 7: return launch_ring<false, true, 2, true>(p, st);
-    case 8: return launch_ring<true, false, 1, false>(p, st);
-    case 9: return launch_ring<true, false, 1, true>(p, st);
-    case 10: return launch_ring<true, false, 2, false>(p, st);
-    case 11: return launch_ring<true, false, 2, true>(p, st);
-    case 12: return launch_ring<true, true, 1, false>(p, st);
-    case 13: return launch_ring<true, true, 1, true>(p, st);
-    case 14: return launch_ring<true, true, 2, false>(p, st);
-    default: return launch_ring<true, true, 2, true>(p, st);
-  }
+  return gated ? launch_norm<true>(p, backward, st) : launch_norm<false>(p, backward, st);
 }
 
 }  // namespace kda

@@ -43,8 +43,6 @@ struct GroupSum {
   }
 };
 
-constexpr int NV = 2;      // vectors of eight columns per thread: what a thread does once a row (sums, addresses) it does for sixteen columns
-
 // vector i of a thread's columns in a row in shared memory, of type T (KDA_BF16 or KDA_FP32)
 template <int T, bool VEC>
 __device__ __forceinline__ void get8(const unsigned char* row, const Cols<VEC>& c, int i, float (&v)[8]) {
@@ -104,7 +102,7 @@ __device__ __forceinline__ void get_param(const float* p, const Cols<VEC>& c, in
 }
 
 // A row of the gated norm.  x, z, d: the row of x, of the gate, of dy; results over x and z.
-template <int XT, int ZT, bool VEC, bool BWD>
+template <int XT, int ZT, bool VEC, bool BWD, int NV>
 __device__ __forceinline__ void gated_row(const kda_norm_args& a, const float* w_, const Cols<VEC>& c, GroupSum& sum, bool there, unsigned char* x_, unsigned char* z_,
                                           const unsigned char* d_, float (&acc)[2][NV][8]) {
   const float inv = 1.f / a.cols;
@@ -164,31 +162,39 @@ __device__ __forceinline__ void gated_row(const kda_norm_args& a, const float* w
 }
 
 // A row of the residual norm.  x, r, dy, dr: the row of x, of the residual, of their gradients (or NULL); results over x and r.  sw: scale times post_weight.
-template <int XT, int RT, bool VEC, bool BWD>
+template <int XT, int RT, bool VEC, bool BWD, int NV>
 __device__ __forceinline__ void residual_row(const kda_norm_args& a, const float* w_, const float* sw_, const Cols<VEC>& c, GroupSum& sum, bool there, unsigned char* x_,
                                              unsigned char* r_, const unsigned char* dy_, const unsigned char* dr_, float (&acc)[2][NV][8]) {
   const float inv = 1.f / a.cols;
-  float x[NV][8], rstd1 = 1.f, ss = 0.f;
+  float rstd1 = 1.f, ss = 0.f;
+  // x is read from shared memory wherever it is needed: with it, r, t and the sums over rows in registers the backward spilled, into an L1 that the ring leaves
+  // little of (32,768 x 4096: 596 us)
+  auto n1 = [&](int i, float (&x)[8]) {
+    get8<XT, VEC>(x_, c, i, x);
 #pragma unroll
-  for (int i = 0; i < NV; ++i) get8<XT, VEC>(x_, c, i, x[i]);
+    for (int j = 0; j < 8; ++j) x[j] *= rstd1;
+  };
   if (a.post_weight) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < NV; ++i) {
+      float x[8];
+      get8<XT, VEC>(x_, c, i, x);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) ss = fmaf(x[i][j], x[i][j], ss);
+      for (int j = 0; j < 8; ++j) ss = fmaf(x[j], x[j], ss);
+    }
     rstd1 = rsqrtf(fmaf(sum(ss), inv, a.eps));
   }
   float r[NV][8];
   ss = 0.f;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    float sw[8];
+    float x[8], sw[8];
+    n1(i, x);
     get8<RT, VEC>(r_, c, i, r[i]);
     get_param<VEC>(sw_, c, i, sw);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      x[i][j] *= rstd1;
-      r[i][j] = fmaf(sw[j], x[i][j], r[i][j]);      // (columns that are not there: x and the residual read as zero)
+      r[i][j] = fmaf(sw[j], x[j], r[i][j]);      // (columns that are not there: x and the residual read as zero)
       ss = fmaf(r[i][j], r[i][j], ss);
     }
   }
@@ -226,7 +232,8 @@ __device__ __forceinline__ void residual_row(const kda_norm_args& a, const float
     float dot1 = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      float sw[8], dr[8];
+      float x[8], sw[8], dr[8];
+      n1(i, x);
       if (dr_) get8<RT, VEC>(dr_, c, i, dr);
       else
 #pragma unroll
@@ -235,18 +242,21 @@ __device__ __forceinline__ void residual_row(const kda_norm_args& a, const float
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         t[i][j] = fmaf(rstd, fmaf(-dot, r[i][j], t[i][j]), dr[j]);
-        if (there) acc[1][i][j] = fmaf(t[i][j], x[i][j], acc[1][i][j]);
+        if (there) acc[1][i][j] = fmaf(t[i][j], x[j], acc[1][i][j]);
         r[i][j] = sw[j] * t[i][j];      // (now the gradient of n1)
-        dot1 = fmaf(r[i][j], x[i][j], dot1);
+        dot1 = fmaf(r[i][j], x[j], dot1);
       }
       if (there) put8<RT, VEC>(r_, c, i, t[i]);
     }
     if (a.post_weight) {
       dot1 = sum(dot1) * inv;
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
+      for (int i = 0; i < NV; ++i) {
+        float x[8];
+        n1(i, x);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) r[i][j] = rstd1 * fmaf(-dot1, x[i][j], r[i][j]);
+        for (int j = 0; j < 8; ++j) r[i][j] = rstd1 * fmaf(-dot1, x[j], r[i][j]);
+      }
     }
     if (!there) return;
 #pragma unroll
@@ -268,7 +278,7 @@ struct RingParams {
 
 }  // namespace
 
-template <bool GATED, int XT, int ZT, bool VEC, bool BWD>
+template <bool GATED, int XT, int ZT, bool VEC, bool BWD, int NV>
 __global__ void __launch_bounds__(544, 1) norm_ring_kernel(const __grid_constant__ RingParams p) {
   extern __shared__ __align__(128) unsigned char smem_raw[];
   __shared__ uint64_t full[STAGES_MOST], done[STAGES_MOST];
@@ -362,9 +372,9 @@ __global__ void __launch_bounds__(544, 1) norm_ring_kernel(const __grid_constant
       const bool there = r < left;
       const int at = there ? r * a.cols : 0;
       if constexpr (GATED)
-        gated_row<XT, ZT, VEC, BWD>(a, w_, c, sum, there, st + p.off[0] + at * XS, st + p.off[1] + at * ZS, st + p.off[2] + at * XS, acc);
+        gated_row<XT, ZT, VEC, BWD, NV>(a, w_, c, sum, there, st + p.off[0] + at * XS, st + p.off[1] + at * ZS, st + p.off[2] + at * XS, acc);
       else
-        residual_row<XT, ZT, VEC, BWD>(a, w_, sw_, c, sum, there, st + p.off[0] + at * XS, st + p.off[1] + at * ZS, a.dy ? st + p.off[2] + at * XS : nullptr,
+        residual_row<XT, ZT, VEC, BWD, NV>(a, w_, sw_, c, sum, there, st + p.off[0] + at * XS, st + p.off[1] + at * ZS, a.dy ? st + p.off[2] + at * XS : nullptr,
                                        a.dr ? st + p.off[3] + at * ZS : nullptr, acc);
     }
     next = r - p.rows;
@@ -399,9 +409,13 @@ int norm_ring_status(uint32_t* host_out) {
   return static_cast<int>(e);
 }
 
+// Vectors of eight columns per thread.  Two: what a thread does once a row (sums over it, addresses) it does for sixteen columns.  The residual norm's backward
+// has sums over rows, r and t in registers and takes one where a row's threads allow it (32,768 x 4096: two 575 us, spilling into an L1 that the ring
+// leaves little of).
+static int vectors(int cols, bool gated, bool backward) { return backward && !gated && cols <= 4096 ? 1 : 2; }
 // threads of a row and rows at a time
-static void split(int cols, int& lanes, int& groups) {
-  const int need = (cols + 8 * NV - 1) / (8 * NV);
+static void split(int cols, int nv, int& lanes, int& groups) {
+  const int need = (cols + 8 * nv - 1) / (8 * nv);
   for (lanes = 1; lanes < need && lanes < 32; lanes *= 2) {}
   if (need > 32) lanes = (need + 31) / 32 * 32;
   groups = 512 / lanes;
@@ -418,7 +432,7 @@ static bool plan(const kda_norm_args& a, bool gated, bool backward, RingParams& 
   p.size[1] = p.size[3] = other == KDA_BF16 ? 2 : 4;
   p.out[0] = backward ? a.dx : a.y;
   p.out[1] = backward ? (gated ? a.dgate : a.dresidual) : (gated ? nullptr : a.r);
-  split(a.cols, p.lanes, p.groups);
+  split(a.cols, vectors(a.cols, gated, backward), p.lanes, p.groups);
   int per_row = 0;
   for (int i = 0; i < 4; ++i)
     if (p.in[i]) per_row += p.size[i] * a.cols;
@@ -452,17 +466,24 @@ bool norm_ring_covers(const kda_norm_args& a, bool gated, bool backward) {
 // the most partial sums of a call: their number depends on the columns alone
 size_t norm_ring_partials(int cols) {
   int lanes, groups;
-  split(cols, lanes, groups);
+  split(cols, 2, lanes, groups);
   return static_cast<size_t>(sm_count()) * groups;
 }
 
+template <bool GATED, int XT, int ZT, bool VEC, bool BWD, int NV>
+static int launch_ring_nv(const RingParams& p, cudaStream_t st) {
+  static DeviceOnce once;
+  const int rc = once.run([] { return cudaFuncSetAttribute(norm_ring_kernel<GATED, XT, ZT, VEC, BWD, NV>, cudaFuncAttributeMaxDynamicSharedMemorySize, RING_MOST); });
+  if (rc != KDA_OK) return rc;
+  norm_ring_kernel<GATED, XT, ZT, VEC, BWD, NV><<<ring_ctas(p), p.lanes * p.groups + 32, p.params + p.stages * p.stage_bytes, st>>>(p);
+  return static_cast<int>(cudaGetLastError());
+}
 template <bool GATED, int XT, int ZT, bool VEC, bool BWD>
 static int launch_ring(const RingParams& p, cudaStream_t st) {
-  static DeviceOnce once;
-  const int rc = once.run([] { return cudaFuncSetAttribute(norm_ring_kernel<GATED, XT, ZT, VEC, BWD>, cudaFuncAttributeMaxDynamicSharedMemorySize, RING_MOST); });
-  if (rc != KDA_OK) return rc;
-  norm_ring_kernel<GATED, XT, ZT, VEC, BWD><<<ring_ctas(p), p.lanes * p.groups + 32, p.params + p.stages * p.stage_bytes, st>>>(p);
-  return static_cast<int>(cudaGetLastError());
+  if constexpr (BWD && !GATED) {
+    if (vectors(p.a.cols, GATED, BWD) == 1) return launch_ring_nv<GATED, XT, ZT, VEC, BWD, 1>(p, st);
+  }
+  return launch_ring_nv<GATED, XT, ZT, VEC, BWD, 2>(p, st);
 }
 template <bool GATED, int XT, int ZT>
 static int launch_types(const RingParams& p, bool backward, cudaStream_t st) {

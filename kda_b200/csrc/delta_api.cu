@@ -12,7 +12,7 @@ static int validate(const kda_delta_args& a, bool backward) {
   if (a.io_dtype != KDA_BF16) return KDA_E_DTYPE;
   if ((a.g_dtype != KDA_BF16 && a.g_dtype != KDA_FP32) || (a.beta_dtype != KDA_BF16 && a.beta_dtype != KDA_FP32)) return KDA_E_DTYPE;
   if (a.tokens > 0x7fffffffLL - 64) return KDA_E_SHAPE;                                          // tile coordinates are 32 bits
-  if ((a.tokens / C + a.N) * a.H > 0x7fffffffLL || static_cast<int64_t>(a.N) * a.H * 4 > 0x7fffffffLL) return KDA_E_SHAPE;      // so are grids
+  if ((a.tokens / C + a.N) * a.H > 0x7fff0000LL || static_cast<int64_t>(a.N) * a.H * 4 > 0x7fffffffLL) return KDA_E_SHAPE;      // so are grids
   if (a.tokens == 0 || a.N == 0) return KDA_OK;
   if (!a.q || !a.k || !a.v || !a.g || !a.beta || !a.workspace || (!backward && !a.o)) return KDA_E_NULL;
   if (!a.cu_seqlens && a.tokens % a.N != 0) return KDA_E_SHAPE;

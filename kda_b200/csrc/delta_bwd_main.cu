@@ -53,7 +53,7 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_main_kernel(const __grid_cons
   extern __shared__ unsigned char smem_raw[];
   MainSmem& s = *reinterpret_cast<MainSmem*>(smem_raw + pad_to_1024(smem_raw));
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, q4 = warp & 3, g = warp >> 2;
-  const long long total = static_cast<long long>(p.map.total()) * p.H;
+  const int total = p.map.total() * p.H;      // (below 2^31: checked by the entry points)
   if (tid == 0) {
     mbar_init(&s.fullA[0], 1);
     mbar_init(&s.fullA[1], 1);
@@ -79,9 +79,9 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_main_kernel(const __grid_cons
     const bool krow = q4 < 2;
     bool ok = true;
     int n = 0;
-    for (long long tile = blockIdx.x; tile < total; tile += gridDim.x, ++n) {
-      const ChunkInfo ci = p.map.info(static_cast<int>(tile / p.H));
-      const int h = static_cast<int>(tile % p.H);
+    for (int tile = blockIdx.x; tile < total; tile += gridDim.x, ++n) {
+      const ChunkInfo ci = p.map.info(tile / p.H);
+      const int h = tile % p.H;
       if (__any_sync(0xffffffffu, s.dead != 0)) { ok = false; break; }
       if (!(ok = warp_wait(&s.fullA[n & 1], (n >> 1) & 1) && warp_wait(&s.fullB, n & 1))) break;
       if (ci.len < C) {
@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_main_kernel(const __grid_cons
       const uint32_t aE = smem_u32(s.E);
       bool ok = true;
       int n = 0;
-      for (long long tile = blockIdx.x; tile < total; tile += gridDim.x, ++n) {
+      for (int tile = blockIdx.x; tile < total; tile += gridDim.x, ++n) {
         const uint32_t aK = smem_u32(s.KQ[n & 1][0]);
         if (s.dead || !mbar_wait(&s.fullA[n & 1], (n >> 1) & 1) || !mbar_wait(&s.fullB, n & 1) || !mbar_wait(&s.ready, n & 1)) { ok = false; break; }
         umma::fence_after_sync();
@@ -294,17 +294,17 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_main_kernel(const __grid_cons
     __syncwarp();
   } else {
     // ================= loads, stores, dg and dbeta =================
-    auto loadA = [&](long long tile, int n) {
-      const ChunkInfo ci = p.map.info(static_cast<int>(tile / p.H));
-      const int h = static_cast<int>(tile % p.H), hq = h / p.grp, tok0 = static_cast<int>(ci.tok0), b = n & 1;
+    auto loadA = [&](int tile, int n) {
+      const ChunkInfo ci = p.map.info(tile / p.H);
+      const int h = tile % p.H, hq = h / p.grp, tok0 = static_cast<int>(ci.tok0), b = n & 1;
       mbar_expect_tx(&s.fullA[b], 4 * 8192 + VEC_COPY);
       for (int x = 0; x < 2; ++x) tma_load_rows(s.KQ[b][x], &p.tm_k, 64 * x, hq, tok0, &s.fullA[b]);
       for (int x = 0; x < 2; ++x) tma_load_rows(s.KQ[b][x] + 8192, &p.tm_q, 64 * x, hq, tok0, &s.fullA[b]);
       bulk_g2s(s.vec[b], p.VEC + static_cast<size_t>(tile) * T_VEC, VEC_COPY, &s.fullA[b]);
     };
-    auto loadB = [&](long long tile) {
-      const ChunkInfo ci = p.map.info(static_cast<int>(tile / p.H));
-      const int h = static_cast<int>(tile % p.H), tok0 = static_cast<int>(ci.tok0);
+    auto loadB = [&](int tile) {
+      const ChunkInfo ci = p.map.info(tile / p.H);
+      const int h = tile % p.H, tok0 = static_cast<int>(ci.tok0);
       const size_t at = static_cast<size_t>(tile);
       mbar_expect_tx(&s.fullB, spans * (4 * 8192 + 2 * 16384));
       for (int x = 0; x < spans; ++x) {
@@ -318,10 +318,10 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_main_kernel(const __grid_cons
         bulk_g2s(s.DH[x], p.DH + at * T_STATE + x * 16384, spans * 8192, &s.fullB);
       }
     };
-    auto store = [&](long long tile, int n) {      // dk, dq of a full chunk
-      const ChunkInfo ci = p.map.info(static_cast<int>(tile / p.H));
+    auto store = [&](int tile, int n) {      // dk, dq of a full chunk
+      const ChunkInfo ci = p.map.info(tile / p.H);
       if (ci.len < C) return;
-      const int h = static_cast<int>(tile % p.H), tok0 = static_cast<int>(ci.tok0);
+      const int h = tile % p.H, tok0 = static_cast<int>(ci.tok0);
       for (int x = 0; x < 2 && 64 * x < p.kc; ++x) {
         tma_store_rows(&p.tm_dk, 64 * x, h, tok0, s.KQ[n & 1][x]);
         tma_store_rows(&p.tm_dq, 64 * x, h, tok0, s.KQ[n & 1][x] + 8192);
@@ -330,12 +330,12 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_main_kernel(const __grid_cons
     };
     bool ok = true;
     int n = 0;
-    if (lane == 0 && blockIdx.x < total) {
+    if (lane == 0 && static_cast<int>(blockIdx.x) < total) {
       loadA(blockIdx.x, 0);
       loadB(blockIdx.x);
     }
-    for (long long tile = blockIdx.x; tile < total; tile += gridDim.x, ++n) {
-      const long long next = tile + gridDim.x;
+    for (int tile = blockIdx.x; tile < total; tile += gridDim.x, ++n) {
+      const int next = tile + gridDim.x;
       if (__any_sync(0xffffffffu, s.dead != 0)) { ok = false; break; }
       if (!(ok = warp_wait(&s.ready, n & 1))) break;      // everybody is past the tile before
       if (lane == 0) {
@@ -351,8 +351,8 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_main_kernel(const __grid_cons
       }
       if (!(ok = warp_wait(&s.done, n & 1))) break;
       {      // dg: the sum of dG from a token to the chunk's end, two tokens a lane (these sums are written again behind the load of the tile after the next)
-        const ChunkInfo ci = p.map.info(static_cast<int>(tile / p.H));
-        const int h = static_cast<int>(tile % p.H);
+        const ChunkInfo ci = p.map.info(tile / p.H);
+        const int h = tile % p.H;
         const float* const vec = s.vec[n & 1];
         const MainSmem::Sums& sums = s.sums[n & 1];
         float tail = lane < CW ? sums.h[lane] * vec[V_LAST] : 0.f;
@@ -387,7 +387,7 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_main_kernel(const __grid_cons
     }
     if (ok && n > 0) {
       ok = warp_wait(&s.ready, n & 1);
-      if (ok && lane == 0) store(blockIdx.x + static_cast<long long>(n - 1) * gridDim.x, n - 1);
+      if (ok && lane == 0) store(blockIdx.x + (n - 1) * gridDim.x, n - 1);
     }
     if (!ok) {
       s.dead = 1;

@@ -4,7 +4,7 @@
 // beta multiply its fp32 result.  Tm = (I + A)^-1: the four 16 x 16 diagonal blocks by substitution in fp32, then two merges
 // T21 = -(T2 A21) T1, at 16 and 32 rows, by mma.sync on bf16 pairs: T2 A21 leaves the first product in the layout that the second takes its A in.
 // Pt = P Tm is a product of the tensor core again, in pairs, whose A operand's upper half is Tm's own tile (the rows it adds are not read).
-// G is summed in double and kept as two floats: after a strong decay early in a chunk one float leaves 1e-5 in every later D_ij.
+// G is a sum of two floats each: after a strong decay early in a chunk one float leaves 1e-5 in every later D_ij.
 // A tile is a row of short phases, each of them latency (14 k cycles a tile, 2 k of them instructions): the next tile's k and q are fetched once this one's have
 // been read, its g and beta while this one is worked on (16,384 tiles: 310 us with a CTA per tile, whose loads, tensor memory and stores nobody hid;
 // 578 with Tm's merges as fp32 sums over shared memory).
@@ -23,7 +23,8 @@ struct PrepSmem {
   unsigned char KQ[2][16384];      // [128 rows: k, then q][64 columns] x 2
   unsigned char TPh[16384], TPl[16384];      // rows 0..63: A, which Tm replaces block by block; rows 64..127: P, then Pt
   float D[4][16][16];              // A's diagonal blocks in fp32, transposed
-  double gs[2];
+  float gs[2];
+  struct Tile { int tok0, len, h; } next[2];      // where a tile is, by the thread that fetches it
   float ghi[C], glo[C], beta[C], rk[C], rq[C], q2[3][C];      // q2: of q's row halves, of k's rows
   float to16[C], to32[C];          // decay from a token to the end of its 16 tokens, of its 32
   uint64_t full, done;
@@ -45,6 +46,13 @@ __device__ __forceinline__ void frag_a(uint32_t (&f)[4], const unsigned char* ti
 __device__ __forceinline__ void frag_b(uint32_t (&f)[4], const unsigned char* tile, int row, int col, int lane) {
   ldsm_x4_t(f, smem_u32(tile) + umma::sw128(row + (lane & 15), col + 8 * (lane >> 4)));
 }
+// the sum of two numbers as two floats each, to the last bit but a few of 48
+struct Two { float hi, lo; };
+__device__ __forceinline__ Two add(const Two& a, const Two& b) {
+  const float s = a.hi + b.hi, v = s - a.hi, e = (a.hi - (s - v)) + (b.hi - v) + (a.lo + b.lo), hi = s + e;
+  return {hi, e - (hi - s)};
+}
+constexpr float LOG2E_REST = 1.92596299e-8f;      // log2(e) - LOG2E
 // exp(G_i - G_j)
 __device__ __forceinline__ float decay_between(const PrepSmem& s, int i, int j) { return ex2((s.ghi[i] - s.ghi[j]) + (s.glo[i] - s.glo[j])); }
 struct FragPair { uint32_t h[4], l[4]; };
@@ -79,44 +87,48 @@ __global__ void __launch_bounds__(PT, 3) delta_prepare_kernel(const __grid_const
   const int total = p.map.total() * p.H;      // (below 2^31: checked by the entry points)
   if (static_cast<int>(blockIdx.x) >= total) return;
 
-  auto load = [&](int tile) {      // one thread: k's and q's rows
+  auto place = [&](int tile) {
     const ChunkInfo ci = p.map.info(tile / p.H);
-    const int h = tile % p.H / p.grp;
+    return PrepSmem::Tile{static_cast<int>(ci.tok0), ci.len, tile % p.H};
+  };
+  auto load = [&](const PrepSmem::Tile& x) {      // one thread: k's and q's rows
     mbar_expect_tx(&s.full, 4 * 8192);
     for (int b = 0; b < 2; ++b) {
-      tma_load_rows(s.KQ[b], &p.tm_k, 64 * b, h, static_cast<int>(ci.tok0), &s.full);
-      tma_load_rows(s.KQ[b] + 8192, &p.tm_q, 64 * b, h, static_cast<int>(ci.tok0), &s.full);
+      tma_load_rows(s.KQ[b], &p.tm_k, 64 * b, x.h / p.grp, x.tok0, &s.full);
+      tma_load_rows(s.KQ[b] + 8192, &p.tm_q, 64 * b, x.h / p.grp, x.tok0, &s.full);
     }
   };
   const bool gater = warp == 4 || warp == 5;      // a token of the tile per thread
+  const bool fetcher = tid == 192;                // (of a warp whose part of A or P is zero)
   float g_next = 0.f, b_next = 0.f;
-  auto load_gates = [&](int tile) {         // rows behind the sequence's end neither decay nor write
-    const ChunkInfo ci = p.map.info(tile / p.H);
+  auto load_gates = [&](const PrepSmem::Tile& x) {         // rows behind the sequence's end neither decay nor write
     g_next = b_next = 0.f;
-    if (tid - 128 < ci.len) {
-      const size_t row = static_cast<size_t>(ci.tok0 + tid - 128) * p.H + tile % p.H;
+    if (tid - 128 < x.len) {
+      const size_t row = static_cast<size_t>(x.tok0 + tid - 128) * p.H + x.h;
       g_next = load_raw(p.g, row, p.g_dtype);
       b_next = load_raw(p.beta, row, p.beta_dtype);
     }
   };
-  if (tid == 0) {
+  if (fetcher) {
     mbar_init(&s.full, 1);
     mbar_init(&s.done, 1);
     fence_mbar_init();
-    load(blockIdx.x);
+    s.next[0] = place(blockIdx.x);
+    load(s.next[0]);
   }
   if (warp == 1) umma::tmem_alloc(&s.tmem_slot, 128);
-  if (gater) load_gates(blockIdx.x);
   umma::fence_before_sync();
   __syncthreads();
   umma::fence_after_sync();
+  if (gater) load_gates(s.next[0]);
   const uint32_t tb = s.tmem_slot, tq = tb + (static_cast<uint32_t>(32 * q4) << 16);
 
   bool ok = true;
   unsigned phase = 0;
   for (int tile = blockIdx.x; tile < total; tile += gridDim.x, phase ^= 1u) {
     const int next = tile + gridDim.x;
-    const int len = p.map.info(tile / p.H).len;
+    const int len = s.next[phase].len;
+    if (fetcher && next < total) s.next[phase ^ 1] = place(next);
     ok = mbar_wait(&s.full, phase);
     if (tid == 0 && ok) {
       constexpr uint32_t id = umma::instr_desc(128, 64, false, false);
@@ -147,25 +159,29 @@ __global__ void __launch_bounds__(PT, 3) delta_prepare_kernel(const __grid_const
     } else {      // sums of g, in log2
       const int t = tid - 128;
       const float g = g_next < -1e5f ? -1e5f : g_next;      // -inf: the state is forgotten; differences of G stay numbers
-      double x = static_cast<double>(g) * 1.4426950408889634;
+      Two x{g * LOG2E, 0.f};
+      x.lo = fmaf(g, LOG2E, -x.hi) + g * LOG2E_REST;
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {
-        const double y = __shfl_up_sync(0xffffffffu, x, off);
-        if (lane >= off) x += y;
+        const Two y{__shfl_up_sync(0xffffffffu, x.hi, off), __shfl_up_sync(0xffffffffu, x.lo, off)};
+        if (lane >= off) x = add(x, y);
       }
-      if (warp == 4 && lane == 31) s.gs[0] = x;
+      if (warp == 4 && lane == 31) {
+        s.gs[0] = x.hi;
+        s.gs[1] = x.lo;
+      }
       asm volatile("bar.sync 1, 64;" ::: "memory");
-      if (warp == 5) x += s.gs[0];
-      s.ghi[t] = static_cast<float>(x);
-      s.glo[t] = static_cast<float>(x - static_cast<double>(static_cast<float>(x)));
+      if (warp == 5) x = add(x, Two{s.gs[0], s.gs[1]});
+      s.ghi[t] = x.hi;
+      s.glo[t] = x.lo;
       s.beta[t] = b_next;
       asm volatile("bar.sync 1, 64;" ::: "memory");
       s.to16[t] = decay_between(s, t | 15, t);
       s.to32[t] = decay_between(s, t | 31, t);
-      if (next < total) load_gates(next);
     }
     if (tid == 0) bulk_wait_read<0>();       // the tile before has left TP
     ok = __syncthreads_and(ok);
+    if (gater && next < total) load_gates(s.next[phase ^ 1]);
     ok = ok && mbar_wait(&s.done, 0);
     umma::fence_after_sync();
     const int i = 32 * (q4 & 1) + lane;      // this thread's row, of A (q4 < 2) or of P; its columns 32 half ..
@@ -175,7 +191,7 @@ __global__ void __launch_bounds__(PT, 3) delta_prepare_kernel(const __grid_const
       umma::tmem_ld16(tq + 32 * half + 16, *reinterpret_cast<float(*)[16]>(&S[16]));
       umma::tmem_ld_wait();
     }
-    if (tid == 0 && ok && next < total) load(next);
+    if (fetcher && ok && next < total) load(s.next[phase ^ 1]);
     // ---- A and P: rows times decays ------------------------------------------------------------------------------------------------------------------
     const float rq = p.use_l2norm ? rsqrtf(s.q2[0][i] + s.q2[1][i] + L2NORM_EPS) : 1.f;
     if (q4 == 2 + (i >> 5) && half == 0) s.rq[i] = rq;
@@ -247,12 +263,11 @@ __global__ void __launch_bounds__(PT, 3) delta_prepare_kernel(const __grid_const
           if (4 * r4 + 3 > j) x[4 * r4 + 3] = fmaf(-a.w, x[j], x[4 * r4 + 3]);
         }
       }
+      const uint32_t at = column_at(s.TPh, 16 * b, 16 * b + col);
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const __nv_bfloat16 hi = __float2bfloat16_rn(x[r]);
-        const uint32_t off = umma::sw128(16 * b + r, 16 * b + col);
-        *reinterpret_cast<__nv_bfloat16*>(s.TPh + off) = hi;
-        *reinterpret_cast<__nv_bfloat16*>(s.TPl + off) = __float2bfloat16_rn(x[r] - __bfloat162float(hi));
+        column_put(at, r, x[r]);
+        column_put(at + 16384, r, x[r] - __bfloat162float(__float2bfloat16_rn(x[r])));
       }
       __syncwarp();
       // ---- merge of 16: each of the two warps has written both diagonal blocks of its pair; T21 takes A21's place -----------------------------------------

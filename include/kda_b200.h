@@ -359,6 +359,9 @@ int kda_gate_bwd(const kda_gate_args* args, void* stream);
  *
  * kda_delta_recurrent_fwd: kda_recurrent_fwd with that g.  The fields of kda_recurrent_args keep their meaning but for these: `g` points to
  * [tokens, H] of g_raw_dtype and `beta` to [tokens, H] of beta_raw_dtype, whether A_log and beta_sigmoid are given or not; dt_bias is [H].
+ * slots, slot_columns: with state_indices, the states in the pool h0 and the columns of the table.  A sequence whose starting slot lies outside the pool (a
+ * padded entry of a batch), or whose accepted count names no column, has zeros for its rows of o and touches no state; the state behind a token whose slot
+ * lies outside is not kept.  Two sequences must not name the same slot.
  *
  * kda_delta_chunk_fwd / _bwd: whole sequences in chunks of 64 tokens on the tensor cores, bf16 q, k, v, o.  States, their gradients and every sum are
  * fp32, and operands that are not inputs are bf16 pairs in the two walks over a sequence: final states and dh0 carry about 1e-5 of their norm.  Rules as
@@ -403,7 +406,7 @@ size_t kda_delta_chunk_workspace_bytes(int64_t tokens, int32_t N, int32_t H, int
 size_t kda_delta_chunk_bwd_workspace_bytes(int64_t tokens, int32_t N, int32_t H, int32_t HQ, int32_t K, int32_t V);
 int kda_delta_chunk_fwd(const kda_delta_args* args, void* stream);
 int kda_delta_chunk_bwd(const kda_delta_args* args, void* stream);
-int kda_delta_recurrent_fwd(const kda_recurrent_args* args, void* stream);
+int kda_delta_recurrent_fwd(const kda_recurrent_args* args, int32_t slots, int32_t slot_columns, void* stream);
 
 /* ------------------------------------------------------------------------------------------------
  * The norms around a block, over the last dimension of [rows, cols] tensors (rms(x) = sqrt(mean x^2 + eps)):

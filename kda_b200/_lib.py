@@ -162,7 +162,7 @@ def load() -> C.CDLL:
         fn.restype = C.c_int
         fn.argtypes = [C.POINTER(GateArgs), C.c_void_p]
     lib.kda_delta_recurrent_fwd.restype = C.c_int
-    lib.kda_delta_recurrent_fwd.argtypes = [C.POINTER(RecurrentArgs), C.c_void_p]
+    lib.kda_delta_recurrent_fwd.argtypes = [C.POINTER(RecurrentArgs), C.c_int32, C.c_int32, C.c_void_p]
     lib.kda_delta_chunk_workspace_bytes.restype = lib.kda_delta_chunk_bwd_workspace_bytes.restype = C.c_size_t
     lib.kda_delta_chunk_workspace_bytes.argtypes = lib.kda_delta_chunk_bwd_workspace_bytes.argtypes = [C.c_int64] + [C.c_int32] * 5
     for name in ("kda_delta_chunk_fwd", "kda_delta_chunk_bwd"):

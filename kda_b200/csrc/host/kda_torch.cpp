@@ -256,7 +256,10 @@ std::pair<Tensor, Tensor> recurrent_fwd(RecurrentCall& c) {
     else check_rc(kda_recurrent_walk_fwd(&a, stream_of(dev)), "kda_recurrent_walk_fwd");
     return {o, ht};
   }
-  if (c.per_head) check_rc(kda_delta_recurrent_fwd(&a, stream_of(dev)), "kda_delta_recurrent_fwd");
+  if (c.per_head) {
+    const int32_t pool = idx.defined() ? static_cast<int32_t>(h0.size(0)) : 0, columns = !idx.defined() ? 0 : idx.dim() == 1 ? 1 : static_cast<int32_t>(idx.size(1));
+    check_rc(kda_delta_recurrent_fwd(&a, pool, columns, stream_of(dev)), "kda_delta_recurrent_fwd");
+  }
   else check_rc(kda_recurrent_fwd(&a, stream_of(dev)), "kda_recurrent_fwd");
   if (checked_mode()) {
     uint32_t st = 0;

@@ -1,5 +1,6 @@
 // Device-side helpers shared by the KDA kernels (sm_100a only).
 #pragma once
+#include <type_traits>
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -42,6 +43,21 @@ __device__ __forceinline__ float warp_sum(float x) {
   for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
   return x;
 }
+
+// The decode call with one decay per head: what it knows of the pool of states.  A slot outside it (a padded entry of a batch), or an accepted count that
+// names no column of the table, is never followed: nothing of such a sequence is read or written but its rows of o, which become zero.
+struct HeadArgs : kda_recurrent_args {
+  int32_t pool, columns;      // states in h0, columns of state_indices; both only with state_indices
+  __device__ __forceinline__ bool holds(long long slot) const { return slot >= 0 && slot < pool; }
+  __device__ __forceinline__ long long start_slot(long long n) const {
+    const int c = num_accepted_tokens ? num_accepted_tokens[n] - 1 : 0;
+    return c >= 0 && c < columns ? state_indices[static_cast<size_t>(n) * state_indices_stride + c] : -1;
+  }
+};
+template <bool HEAD>
+using RecArgs = std::conditional_t<HEAD, HeadArgs, kda_recurrent_args>;
+__device__ __forceinline__ bool token_slot_there(const HeadArgs& a, const int32_t* slots, long long t) { return t < a.columns && a.holds(slots[t]); }
+__device__ __forceinline__ bool token_slot_there(const kda_recurrent_args&, const int32_t*, long long) { return true; }
 
 // ---- the gate's activations (gate kernels, preparation, recurrent kernels: the same values from each) --------------
 __device__ __forceinline__ float sigmoid_fast(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }

@@ -35,12 +35,13 @@ struct DecSmem {
   float nrm[3][8];            // partial sums of squares: q (warps 0..3), k (warps 0..3)
   float beta[3];
   int dead;                   // a wait gave up
+  int pad[DEC_BUFS];          // HEAD: the buffer's unit is a padded entry
   uint64_t full[DEC_BUFS], ready[DEC_BUFS], gone[DEC_BUFS];      // loaded; written by the compute warps; read by the store
 };
 static_assert(2 * (sizeof(DecSmem<64>) + 128 + 1024) <= 227 * 1024 && sizeof(DecSmem<128>) + 128 <= 227 * 1024, "DecSmem too large");
 
 struct DecParams {
-  kda_recurrent_args a;
+  HeadArgs a;
   int total, step, dn, dh;    // units; grid; what a step of the grid adds to (sequence, head)
   alignas(64) CUtensorMap tm_in, tm_out;      // states as [rows][128] fp32 in boxes of 128 rows x HV columns
 };
@@ -104,7 +105,7 @@ __global__ void __launch_bounds__(HV * 2 + 32, 128 / HV) kda_decode_bulk_kernel(
   constexpr int NW = HV / 16, PARTS = DV / HV;
   constexpr unsigned DEC_TILE = DK * HV * 4;       // bytes of one unit's state
   DecSmem<HV>& s = *reinterpret_cast<DecSmem<HV>*>(smem_raw + ((128u - (smem_u32(smem_raw) & 127u)) & 127u));
-  const kda_recurrent_args& a = p.a;
+  const HeadArgs& a = p.a;
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   const int HQ = a.HQ > 0 ? a.HQ : a.H, grp = a.H / HQ;
@@ -138,10 +139,17 @@ __global__ void __launch_bounds__(HV * 2 + 32, 128 / HV) kda_decode_bulk_kernel(
     if (lane == 0) {
       auto start_slot = [&](const Pos& q) -> long long {
         if (!slotted) return q.n;
+        if constexpr (HEAD) return a.start_slot(q.n);
         const int32_t* row = a.state_indices + static_cast<size_t>(q.n) * a.state_indices_stride;
         return row[a.num_accepted_tokens ? a.num_accepted_tokens[q.n] - 1 : 0];
       };
+      bool pad[3] = {};      // HEAD: of this unit and the two behind it, does its state lie outside the pool
       auto load = [&](long long slot, int h, int b) {
+        if (HEAD && slotted) {      // a padded entry: some state keeps the buffers' turns
+          pad[2] = !a.holds(slot);
+          s.pad[b] = pad[2];
+          if (pad[2]) slot = 0;
+        }
         mbar_expect_tx(&s.full[b], DEC_TILE);
         const long long st = slot * a.H + h;
         if constexpr (TR || HV == DV) bulk_g2s(s.S[b], a.h0 + static_cast<size_t>(st) * (DK * DV) + half * (HV * DK), DEC_TILE, &s.full[b]);
@@ -150,8 +158,10 @@ __global__ void __launch_bounds__(HV * 2 + 32, 128 / HV) kda_decode_bulk_kernel(
       unsigned ready = 0;
       Pos cur = first, ahead = first;
       load(start_slot(ahead), ahead.h, 0);
+      pad[0] = pad[2];
       ahead.next_unit(p);
       if (ahead.u < p.total) load(start_slot(ahead), ahead.h, 1);
+      pad[1] = pad[2];
       ahead.next_unit(p);
       int x = 0, z = 1, y = 2, last = -1;      // this unit's buffer, the next unit's, the spare one; buffer of the last store
       for (; cur.u < p.total; cur.next_unit(p)) {
@@ -163,12 +173,15 @@ __global__ void __launch_bounds__(HV * 2 + 32, 128 / HV) kda_decode_bulk_kernel(
         long long recent[4] = {-1, -1, -1, -1};
         for (int c = 0; c < nst; ++c) {
           const int b = (c & 1) ? y : x;
-          const long long st = (slotted ? static_cast<long long>(a.state_indices[static_cast<size_t>(cur.n) * a.state_indices_stride + c]) : cur.n) * a.H + cur.h;
-          if (HV != DV && (st == recent[0] || st == recent[1] || st == recent[2] || st == recent[3])) bulk_wait<0>();
+          const long long sl = slotted ? static_cast<long long>(a.state_indices[static_cast<size_t>(cur.n) * a.state_indices_stride + c]) : cur.n;
+          const bool skip = HEAD && slotted && (pad[0] || !a.holds(sl));
+          const long long st = skip ? -1 : sl * a.H + cur.h;
+          if (HV != DV && !skip && (st == recent[0] || st == recent[1] || st == recent[2] || st == recent[3])) bulk_wait<0>();
           wait(s.ready, ready, b);
           ready ^= 1u << b;
           if (s.dead) break;
-          if constexpr (TR || HV == DV) bulk_s2g(a.ht + static_cast<size_t>(st) * (DK * DV) + half * (HV * DK), s.S[b], DEC_TILE);
+          if (skip) {}      // (an empty group)
+          else if constexpr (TR || HV == DV) bulk_s2g(a.ht + static_cast<size_t>(st) * (DK * DV) + half * (HV * DK), s.S[b], DEC_TILE);
           else tma_store_2d(&p.tm_out, HV * half, static_cast<int>(st * DK), s.S[b]);
           bulk_commit();
           bulk_wait_read<1>();
@@ -187,6 +200,8 @@ __global__ void __launch_bounds__(HV * 2 + 32, 128 / HV) kda_decode_bulk_kernel(
           if constexpr (HV == DV) bulk_wait_read<0>();
           load(lslot, ahead.h, other);
         }
+        pad[0] = pad[1];
+        pad[1] = pad[2];
         ahead.next_unit(p);
         x = z;
         z = other;
@@ -306,6 +321,7 @@ __global__ void __launch_bounds__(HV * 2 + 32, 128 / HV) kda_decode_bulk_kernel(
   meet();
   unsigned full = 0, sp = 0, any = 0;      // parities of the next load of each buffer; of its stores so far; has it been stored from
   int x = 0, z = 1, y = 2, buf = 0, c = 0;
+  bool pad = false;      // HEAD: a padded entry, whose rows of o are zero
   float4 Sr[16];
   for (int step = 0; cur.u < p.total; ++step) {
     const int par = step & 1;
@@ -316,6 +332,7 @@ __global__ void __launch_bounds__(HV * 2 + 32, 128 / HV) kda_decode_bulk_kernel(
       wait(s.full, full, x);
       full ^= 1u << x;
       c = 0;
+      if (HEAD && slotted) pad = s.pad[x];
     }
     const int dst = (c & 1) ? y : x;
     float rq = a.scale, rk = 1.f;
@@ -379,7 +396,8 @@ __global__ void __launch_bounds__(HV * 2 + 32, 128 / HV) kda_decode_bulk_kernel(
         part[i] = fmaf(q4.x, Sr[i].x, fmaf(q4.y, Sr[i].y, fmaf(q4.z, Sr[i].z, q4.w * Sr[i].w)));
         if (keep) *reinterpret_cast<float4*>(&s.S[dst][(16 * warp + i) * DK + 4 * lane]) = Sr[i];
       }
-      const float o = butterfly_sum16(part, lane);
+      float o = butterfly_sum16(part, lane);
+      if (HEAD && pad) o = 0.f;
       if (lane < 16) st1o(op + ((static_cast<size_t>(cur.n) * a.T + cur.t) * a.H + cur.h) * DV + half * HV + 16 * warp + lane, o);
     } else {
       hk = lds4f(&s.red[par][0][col]);
@@ -410,6 +428,7 @@ __global__ void __launch_bounds__(HV * 2 + 32, 128 / HV) kda_decode_bulk_kernel(
         oa.z += __shfl_xor_sync(0xffffffffu, oa.z, 16);
         oa.w += __shfl_xor_sync(0xffffffffu, oa.w, 16);
       }
+      if (HEAD && pad) oa = make_float4(0.f, 0.f, 0.f, 0.f);
       if (lead) *reinterpret_cast<float4*>(&s.red2[par][warp][col]) = oa;
     }
     if (keep) {
@@ -442,7 +461,7 @@ __global__ void __launch_bounds__(HV * 2 + 32, 128 / HV) kda_decode_bulk_kernel(
 namespace {
 
 template <typename IO, bool TR, bool GATE, int HV, bool HEAD>
-int launch_hv(const kda_recurrent_args& a, cudaStream_t st) {
+int launch_hv(const HeadArgs& a, cudaStream_t st) {
   const int smem = static_cast<int>(sizeof(DecSmem<HV>)) + 128;
   static DeviceOnce once;      // per template variant, per device
   const int rc = once.run([&] {
@@ -461,7 +480,7 @@ int launch_hv(const kda_recurrent_args& a, cudaStream_t st) {
 }
 
 template <typename IO, bool TR, bool GATE, bool HEAD = false>
-int launch(const kda_recurrent_args& a, cudaStream_t st) {
+int launch(const HeadArgs& a, cudaStream_t st) {
   if constexpr (TR || GATE) {
     if (a.T == 1) return launch_hv<IO, TR, GATE, 128, HEAD>(a, st);
   }
@@ -483,7 +502,7 @@ bool decode_bulk_covers(const kda_recurrent_args& a) {
   return states >= KDA_DECODE_BULK_MIN_UNITS_PER_SM * static_cast<long long>(sm_count()) && states <= 0x3fffffff;
 }
 
-int decode_bulk_launch(const kda_recurrent_args& a, bool per_head, cudaStream_t st) {
+int decode_bulk_launch(const HeadArgs& a, bool per_head, cudaStream_t st) {
   if (per_head) {
     if (a.io_dtype == KDA_BF16) return a.transpose_state ? launch<__nv_bfloat16, true, true, true>(a, st) : launch<__nv_bfloat16, false, true, true>(a, st);
     return a.transpose_state ? launch<float, true, true, true>(a, st) : launch<float, false, true, true>(a, st);

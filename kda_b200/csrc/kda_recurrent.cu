@@ -90,7 +90,7 @@ struct RowBits {
 // their latency (one sequence of four draft tokens: 14.2 us when each token fetched its own, 8.0 us so).
 // HEAD: one decay per token and head (kda_delta_recurrent_fwd).
 template <typename IO, int K, int VS, bool HEAD>
-__global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_kernel(const kda_recurrent_args a) {
+__global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_kernel(const RecArgs<HEAD> a) {
   chain_point();
   constexpr int CL = VS / 4;      // lanes across the V slice (4 columns each)
   constexpr int RG = 32 / CL;     // row groups
@@ -117,6 +117,10 @@ __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_kernel(const kda
   if (a.cu_seqlens) {
     bos = a.cu_seqlens[n];
     eos = a.cu_seqlens[n + 1];
+    if constexpr (HEAD) {      // (offsets outside the call's tokens are not followed either)
+      bos = bos < 0 ? 0 : bos;
+      eos = eos < a.tokens ? eos : a.tokens;
+    }
   } else {
     bos = static_cast<long long>(n) * a.T;
     eos = bos + a.T;
@@ -140,7 +144,16 @@ __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_kernel(const kda
   };
   // continuous batching: the sequence's row of slot numbers; it starts from the slot of the last accepted token
   const int32_t* slots = a.state_indices ? a.state_indices + static_cast<size_t>(n) * a.state_indices_stride : nullptr;
-  const long long slot = slots ? slots[a.num_accepted_tokens ? a.num_accepted_tokens[n] - 1 : 0] : n;
+  long long slot = n;
+  if constexpr (HEAD) {
+    if (slots && !a.holds(slot = a.start_slot(n))) {
+      if (rg == 0)
+        for (long long t = bos; t < eos; ++t) IoTraits<IO>::st4(static_cast<IO*>(a.o) + (static_cast<size_t>(t) * a.H + h) * a.V + col, make_float4(0.f, 0.f, 0.f, 0.f));
+      return;
+    }
+  } else if (slots) {
+    slot = slots[a.num_accepted_tokens ? a.num_accepted_tokens[n] - 1 : 0];
+  }
   Token cur, nxt;
   if (bos < eos) fetch(bos, cur);
   float bias[EG], al = 0.f, decay = 1.f;
@@ -233,7 +246,7 @@ __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_kernel(const kda
       oa.w += __shfl_xor_sync(0xffffffffu, oa.w, off);
     }
     if (rg == 0) IoTraits<IO>::st4(op + (static_cast<size_t>(t) * a.H + h) * a.V + col, oa);
-    if (slots && a.ht) {      // the state after every token goes to that token's slot
+    if (slots && a.ht && token_slot_there(a, slots, t - bos)) {      // the state after every token goes to that token's slot
       const size_t tb = (static_cast<size_t>(slots[t - bos]) * a.H + h) * K * a.V + col;
 #pragma unroll
       for (int i = 0; i < R; ++i) __stcs(reinterpret_cast<float4*>(a.ht + tb + static_cast<size_t>(rg + RG * i) * a.V), S[i]);
@@ -272,7 +285,7 @@ __device__ __forceinline__ void st_row(float* p, const float (&d)[E]) {
 // are per-lane partial dot products summed over the lanes 32 values at a time by a butterfly (lane L ends up with
 // the total of value row L); the delta-rule update needs every row's dv in every lane: one shuffle per row.
 template <typename IO, int K, bool HEAD>
-__global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_t_kernel(const kda_recurrent_args a) {
+__global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_t_kernel(const RecArgs<HEAD> a) {
   constexpr int E = K / 32;       // key columns per lane
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int nvs = a.V / 32;
@@ -287,12 +300,24 @@ __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_t_kernel(const k
   if (a.cu_seqlens) {
     bos = a.cu_seqlens[n];
     eos = a.cu_seqlens[n + 1];
+    if constexpr (HEAD) {      // (offsets outside the call's tokens are not followed either)
+      bos = bos < 0 ? 0 : bos;
+      eos = eos < a.tokens ? eos : a.tokens;
+    }
   } else {
     bos = static_cast<long long>(n) * a.T;
     eos = bos + a.T;
   }
   const int32_t* slots = a.state_indices ? a.state_indices + static_cast<size_t>(n) * a.state_indices_stride : nullptr;
-  const long long slot = slots ? slots[a.num_accepted_tokens ? a.num_accepted_tokens[n] - 1 : 0] : n;
+  long long slot = n;
+  if constexpr (HEAD) {
+    if (slots && !a.holds(slot = a.start_slot(n))) {
+      for (long long t = bos; t < eos; ++t) static_cast<IO*>(a.o)[(static_cast<size_t>(t) * a.H + h) * a.V + vs * 32 + lane] = IO(0.f);
+      return;
+    }
+  } else if (slots) {
+    slot = slots[a.num_accepted_tokens ? a.num_accepted_tokens[n] - 1 : 0];
+  }
   auto state_ptr = [&](const float* base, long long sl) {
     return base + ((static_cast<size_t>(sl) * a.H + h) * a.V + vs * 32) * K + lane * E;
   };
@@ -367,7 +392,7 @@ __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_t_kernel(const k
     const float o = butterfly_sum32(part, lane);
     if (sizeof(IO) == 2) reinterpret_cast<__nv_bfloat16*>(op)[(static_cast<size_t>(t) * a.H + h) * a.V + vs * 32 + lane] = __float2bfloat16_rn(o);
     else reinterpret_cast<float*>(op)[(static_cast<size_t>(t) * a.H + h) * a.V + vs * 32 + lane] = o;
-    if (slots && a.ht) {
+    if (slots && a.ht && token_slot_there(a, slots, t - bos)) {
       float* pt = const_cast<float*>(state_ptr(a.ht, slots[t - bos]));
 #pragma unroll
       for (int r = 0; r < 32; ++r) st_row<E>(pt + static_cast<size_t>(r) * K, S[r]);
@@ -381,7 +406,7 @@ __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_t_kernel(const k
 }
 
 template <typename IO, int K, bool HEAD>
-static int launch_rec_t(const kda_recurrent_args& a, cudaStream_t st) {
+static int launch_rec_t(const RecArgs<HEAD>& a, cudaStream_t st) {
   const long long total = static_cast<long long>(a.N) * a.H * (a.V / 32);
   const long long blocks = (total + REC_WARPS - 1) / REC_WARPS;
   if (blocks <= 0) return KDA_OK;
@@ -391,7 +416,7 @@ static int launch_rec_t(const kda_recurrent_args& a, cudaStream_t st) {
 }
 
 template <typename IO, int K, int VS, bool HEAD>
-static int launch_rec(const kda_recurrent_args& a, cudaStream_t st) {
+static int launch_rec(const RecArgs<HEAD>& a, cudaStream_t st) {
   const long long total = static_cast<long long>(a.N) * a.H * (a.V / VS);
   const long long blocks = (total + REC_WARPS - 1) / REC_WARPS;
   if (blocks <= 0) return KDA_OK;
@@ -400,7 +425,7 @@ static int launch_rec(const kda_recurrent_args& a, cudaStream_t st) {
 }
 
 template <typename IO, bool HEAD>
-static int dispatch_rec(const kda_recurrent_args& a, cudaStream_t st) {
+static int dispatch_rec(const RecArgs<HEAD>& a, cudaStream_t st) {
   if (a.transpose_state) {
     switch (a.K) {
       case 64: return launch_rec_t<IO, 64, HEAD>(a, st);
@@ -420,13 +445,13 @@ static int dispatch_rec(const kda_recurrent_args& a, cudaStream_t st) {
 }
 
 bool decode_bulk_covers(const kda_recurrent_args& a);                    // kda_decode_bulk.cu
-int decode_bulk_launch(const kda_recurrent_args& a, bool per_head, cudaStream_t st);
+int decode_bulk_launch(const HeadArgs& a, bool per_head, cudaStream_t st);
 
 }  // namespace kda
 
-static int recurrent_fwd(const kda_recurrent_args* args, bool per_head, void* stream) {
+static int recurrent_fwd(const kda_recurrent_args* args, bool per_head, int32_t pool, int32_t columns, void* stream) {
   if (!args) return KDA_E_NULL;
-  kda_recurrent_args a = *args;
+  kda::HeadArgs a{*args, pool, columns};
   if (a.state_indices) {
     if (a.state_indices_stride <= 0) a.state_indices_stride = 1;
     if (a.ht && a.ht != a.h0) return KDA_E_SHAPE;      // slot-addressed states are updated in place
@@ -459,10 +484,11 @@ static int recurrent_fwd(const kda_recurrent_args* args, bool per_head, void* st
   return KDA_E_DTYPE;
 }
 
-extern "C" int kda_recurrent_fwd(const kda_recurrent_args* args, void* stream) { return recurrent_fwd(args, false, stream); }
+extern "C" int kda_recurrent_fwd(const kda_recurrent_args* args, void* stream) { return recurrent_fwd(args, false, 0, 0, stream); }
 
-extern "C" int kda_delta_recurrent_fwd(const kda_recurrent_args* args, void* stream) {
+extern "C" int kda_delta_recurrent_fwd(const kda_recurrent_args* args, int32_t slots, int32_t slot_columns, void* stream) {
   if (args && ((args->g_raw_dtype != KDA_BF16 && args->g_raw_dtype != KDA_FP32) || (args->beta_raw_dtype != KDA_BF16 && args->beta_raw_dtype != KDA_FP32)))
     return KDA_E_DTYPE;
-  return recurrent_fwd(args, true, stream);
+  if (args && args->state_indices && (slots <= 0 || slot_columns <= 0)) return KDA_E_SHAPE;
+  return recurrent_fwd(args, true, slots, slot_columns, stream);
 }

@@ -5,6 +5,8 @@ Tolerances.  A rounding to bf16 is off by at most 2^-8 of the value.  o and dv r
 2^-8 + 2^-12.  Final states and dh0 are float32: per chunk five pair roundings (state, r, w v_new, Tm, and the products of two low parts, which are left out), at most
 5 * 2^-16 of the terms, which decay from chunk to chunk: 2^-13.  dq, dk, dg, dbeta: every term is a product with one bf16 operand that is not an input
 or, behind E, two, and E's own product has one; with the result's rounding four times 2^-8."""
+import gc
+
 import numpy as np
 import pytest
 import torch
@@ -14,6 +16,13 @@ from oracle.kda_oracle import recurrent_kda, recurrent_kda_grads, rel_l2_err
 pytestmark = pytest.mark.gpu
 ONCE, STATE, GRAD = 2.0 ** -8 + 2.0 ** -12, 2.0 ** -13, 4 * 2.0 ** -8
 TOL = dict(o=ONCE, ht=STATE, dq=GRAD, dk=GRAD, dv=ONCE, dg=GRAD, dbeta=GRAD, dh0=STATE)
+
+
+@pytest.fixture(scope="module", autouse=True)
+def leave_no_memory():
+    yield
+    gc.collect()
+    torch.cuda.empty_cache()
 
 
 def make(B, T, H, HV, K, V, seed, n_states=None, h0=True, normed=True, mild=None, dtype=torch.bfloat16):

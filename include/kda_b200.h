@@ -397,7 +397,7 @@ typedef struct kda_delta_args {
   int32_t g_dtype, beta_dtype; /* KDA_BF16 or KDA_FP32 */
   int32_t use_qk_l2norm;       /* rows of q and k count as x * rsqrt(sum x^2 + 1e-6) */
   int32_t save_for_backward;
-  int32_t scan_slices;         /* CTAs per (sequence, head) of the walks: 0 = by the number of units and SMs; 1 (backward: 2), 2, 4.  Results do not depend on it
+  int32_t scan_slices;         /* CTAs per (sequence, head) of the walks: 0 = by the number of units and SMs; 1, 2, 4.  Results do not depend on it
                                   beyond the order of a product's partial sums. */
   float scale;
 } kda_delta_args;

@@ -479,19 +479,19 @@ int run_norm(const kda_norm_args& a, bool gated, bool backward, cudaStream_t st)
     if (norm_ring_covers(a, gated, backward)) {
       if ((rc = norm_ring(a, gated, backward, p.partial, &ctas, st)) != KDA_OK) return rc;
     } else {
-    const bool vec = a.cols % 8 == 0 && norm_aligned(a);
-    ctas = backward ? bwd_ctas(a.rows, s) : static_cast<int>(std::min<int64_t>((a.rows + s.per - 1) / s.per, static_cast<int64_t>(sm_count()) * 64));
-    rc = with_shape(s, vec, [&](auto V, auto N, auto W) {
-      if (gated) {
-        if (backward) gated_bwd_kernel<V.value, N.value, W.value><<<ctas, s.threads, 0, st>>>(p);
-        else gated_fwd_kernel<V.value, N.value, W.value><<<ctas, s.threads, 0, st>>>(p);
-      } else {
-        if (backward) residual_bwd_kernel<V.value, N.value, W.value><<<ctas, s.threads, 0, st>>>(p);
-        else residual_fwd_kernel<V.value, N.value, W.value><<<ctas, s.threads, 0, st>>>(p);
-      }
-      return static_cast<int>(cudaGetLastError());
-    });
-    if (rc != KDA_OK) return rc;
+      const bool vec = a.cols % 8 == 0 && norm_aligned(a);
+      ctas = backward ? bwd_ctas(a.rows, s) : static_cast<int>(std::min<int64_t>((a.rows + s.per - 1) / s.per, static_cast<int64_t>(sm_count()) * 64));
+      rc = with_shape(s, vec, [&](auto V, auto N, auto W) {
+        if (gated) {
+          if (backward) gated_bwd_kernel<V.value, N.value, W.value><<<ctas, s.threads, 0, st>>>(p);
+          else gated_fwd_kernel<V.value, N.value, W.value><<<ctas, s.threads, 0, st>>>(p);
+        } else {
+          if (backward) residual_bwd_kernel<V.value, N.value, W.value><<<ctas, s.threads, 0, st>>>(p);
+          else residual_fwd_kernel<V.value, N.value, W.value><<<ctas, s.threads, 0, st>>>(p);
+        }
+        return static_cast<int>(cudaGetLastError());
+      });
+      if (rc != KDA_OK) return rc;
     }
   }
   if (!sums) return KDA_OK;
@@ -505,7 +505,7 @@ int run_norm(const kda_norm_args& a, bool gated, bool backward, cudaStream_t st)
 
 extern "C" size_t kda_norm_bwd_workspace_bytes(int64_t rows, int32_t cols, int32_t sums) {
   if (rows < 0 || cols <= 0 || cols > kda::NORM_MOST || sums < 1 || sums > 2) return 0;
-  return std::max<size_t>(std::max(1, kda::bwd_ctas(rows, kda::shape_of(cols))), kda::norm_ring_partials(cols)) * sums * cols * sizeof(float);
+  return std::max<size_t>(std::max(1, kda::bwd_ctas(rows, kda::shape_of(cols))), kda::norm_ring_partials()) * sums * cols * sizeof(float);
 }
 extern "C" int kda_norm_status(uint32_t* host_out) { return kda::norm_ring_status(host_out); }
 extern "C" int kda_gated_norm_fwd(const kda_norm_args* a, void* st) { return a ? kda::run_norm(*a, true, false, static_cast<cudaStream_t>(st)) : KDA_E_NULL; }

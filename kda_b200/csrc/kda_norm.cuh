@@ -7,11 +7,13 @@
 namespace kda {
 
 constexpr int NORM_MOST = 8192;         // columns
-// elements of a call from which rows travel through shared memory (kda_norm_ring.cu)
-constexpr int64_t NORM_RING_MIN = 1 << 21;
+// Elements of a call from which rows travel through shared memory (kda_norm_ring.cu).  us, ring | direct, gated in bf16, then with an fp32 residual:
+//   forward, 2^22 and 2^23 elements   128 columns 7.5 | 8.0, 11.0 | 14.2; 10.5 | 11.3, 18.4 | 22.4     4096: 9.3 | 8.0, 13.1 | 14.1; 12.1 | 13.9, 22.5 | 28.1
+//   backward, 2^19 and 2^20           128 columns 8.5 | 6.6, 8.9 | 9.6; 9.7 | 9.0, 12.1 | 13.6         4096: 10.8 | 8.6, 11.3 | 13.6; 17.7 | 14.7, 21.2 | 24.1
+constexpr int64_t ring_min(bool backward) { return backward ? 1 << 20 : 1 << 23; }
 
 bool norm_ring_covers(const kda_norm_args& a, bool gated, bool backward);
-size_t norm_ring_partials(int cols);
+size_t norm_ring_partials();
 // launches it; *partials: the number of partial sums over rows that it leaves, as [partials][sums][cols]
 int norm_ring(const kda_norm_args& a, bool gated, bool backward, float* partial, int* partials, cudaStream_t st);
 

@@ -15,7 +15,7 @@ namespace {
 // Bit 0: a bounded wait on a stage gave up (the call's results are incomplete).
 __device__ unsigned g_norm_status = 0;
 
-constexpr int RING_MOST = 224 * 1024, RING_STAGE = 32 * 1024, STAGES_MOST = 4;
+constexpr int RING_MOST = 224 * 1024, RING_STAGE = 32 * 1024, STAGES_LEAST = 4, STAGES_MOST = 6;
 
 // The sum over a row's threads, in all of them.  More than a warp: through shared memory, in turns of two so that one barrier is enough.
 struct GroupSum {
@@ -266,7 +266,7 @@ __device__ __forceinline__ void residual_row(const kda_norm_args& a, const float
 
 struct RingParams {
   kda_norm_args a;
-  float* partial;                 // [CTAs * groups][sums][cols] or NULL
+  float* partial;                 // [CTAs][sums][cols] or NULL
   int lanes, groups;              // threads of a row, rows at a time
   int params;                     // bytes of the parameters in front of the stages
   int rows, stages, stage_bytes;  // rows of a stage
@@ -305,55 +305,77 @@ __global__ void __launch_bounds__(544, 1) norm_ring_kernel(const __grid_constant
   if (warp == warps) {
     // ================= copies =================
     if ((threadIdx.x & 31) == 0) {
-      auto rows_of = [&](long long c) { return static_cast<int>(min(static_cast<long long>(p.rows), a.rows - c * p.rows)); };
+      // one chunk per stage and turn, some hundred cycles each: sizes of whole chunks are known ahead, and the last one takes its own way
+      unsigned whole[4], tx = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        whole[i] = p.in[i] ? static_cast<unsigned>(p.rows * a.cols * p.size[i]) : 0;
+        tx += whole[i];
+      }
+      const int last_rows = static_cast<int>(a.rows - (p.chunks - 1) * p.rows);
       auto load = [&](long long c, int s) {
         unsigned char* const st = smem + s * p.stage_bytes;
-        const int rows = rows_of(c);
-        unsigned tx = 0;
+        if (c + 1 < p.chunks) {
+          mbar_expect_tx(&full[s], tx);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (p.in[i]) bulk_g2s(st + p.off[i], static_cast<const unsigned char*>(p.in[i]) + static_cast<size_t>(c) * whole[i], whole[i], &full[s]);
+          return;
+        }
+        unsigned even = 0;
         for (int i = 0; i < 4; ++i) {
           if (!p.in[i]) continue;
-          const int bytes = rows * a.cols * p.size[i];
-          const unsigned char* const src = static_cast<const unsigned char*>(p.in[i]) + static_cast<size_t>(c) * p.rows * a.cols * p.size[i];
+          const int bytes = last_rows * a.cols * p.size[i];
+          const unsigned char* const src = static_cast<const unsigned char*>(p.in[i]) + static_cast<size_t>(c) * whole[i];
           for (int b = bytes & ~15; b < bytes; b += 2)      // the end of the last rows: what is no 16 bytes
             *reinterpret_cast<unsigned short*>(st + p.off[i] + b) = *reinterpret_cast<const unsigned short*>(src + b);
-          tx += bytes & ~15;
+          even += bytes & ~15;
         }
-        mbar_expect_tx(&full[s], tx);
+        mbar_expect_tx(&full[s], even);
         for (int i = 0; i < 4; ++i) {
-          const int bytes = rows * a.cols * p.size[i] & ~15;
-          if (p.in[i] && bytes) bulk_g2s(st + p.off[i], static_cast<const unsigned char*>(p.in[i]) + static_cast<size_t>(c) * p.rows * a.cols * p.size[i], bytes, &full[s]);
+          const int bytes = last_rows * a.cols * p.size[i] & ~15;
+          if (p.in[i] && bytes) bulk_g2s(st + p.off[i], static_cast<const unsigned char*>(p.in[i]) + static_cast<size_t>(c) * whole[i], bytes, &full[s]);
         }
       };
       auto store = [&](long long c, int s) {
         const unsigned char* const st = smem + s * p.stage_bytes;
-        const int rows = rows_of(c);
+#pragma unroll
         for (int i = 0; i < 2; ++i) {
           if (!p.out[i]) continue;
-          const int bytes = rows * a.cols * p.size[i];
-          unsigned char* const dst = static_cast<unsigned char*>(p.out[i]) + static_cast<size_t>(c) * p.rows * a.cols * p.size[i];
+          const int bytes = c + 1 < p.chunks ? static_cast<int>(whole[i]) : last_rows * a.cols * p.size[i];
+          unsigned char* const dst = static_cast<unsigned char*>(p.out[i]) + static_cast<size_t>(c) * whole[i];
           if (bytes & ~15) bulk_s2g(dst, st + p.off[i], bytes & ~15);
           for (int b = bytes & ~15; b < bytes; b += 2) *reinterpret_cast<unsigned short*>(dst + b) = *reinterpret_cast<const unsigned short*>(st + p.off[i] + b);
         }
         bulk_commit();
       };
-      // chunk k of this CTA is chunk blockIdx.x + k * gridDim.x, in stage k % stages
-      const long long mine = blockIdx.x < p.chunks ? (p.chunks - blockIdx.x + gridDim.x - 1) / gridDim.x : 0;
+      // the CTA's chunks are blockIdx.x, blockIdx.x + gridDim.x, ..; they take the stages in turn
       bool alive = true;
-      for (long long k = 0; k < mine + p.stages; ++k) {
-        const int s = static_cast<int>(k % p.stages);
-        if (k >= p.stages && k - p.stages < mine) {
-          if (!(alive = mbar_wait(&done[s], static_cast<unsigned>((k / p.stages - 1) & 1)))) break;
-          store(blockIdx.x + (k - p.stages) * gridDim.x, s);
-          if (k < mine) bulk_wait_read<0>();
+      long long ahead = blockIdx.x;
+      for (int s = 0; s < p.stages && ahead < p.chunks; ++s, ahead += gridDim.x) load(ahead, s);
+      int s = 0;
+      unsigned turn = 0;
+      for (long long c = blockIdx.x; c < p.chunks; c += gridDim.x) {
+        if (!(alive = mbar_wait(&done[s], turn))) break;
+        store(c, s);
+        if (c != blockIdx.x && ahead < p.chunks) {      // into the stage before, whose store has had a turn's time to read it
+          bulk_wait_read<1>();
+          load(ahead, s == 0 ? p.stages - 1 : s - 1);
+          ahead += gridDim.x;
         }
-        if (k < mine) load(blockIdx.x + k * gridDim.x, s);
+        if (++s == p.stages) {
+          s = 0;
+          turn ^= 1u;
+        }
       }
       if (!alive) {      // loads may still be under way into this CTA's memory
         atomicOr(&g_norm_status, 1u);
-        for (int s = 0; s < p.stages; ++s) mbar_drain(&full[s]);
+        for (int i = 0; i < p.stages; ++i) mbar_drain(&full[i]);
       }
       bulk_wait_read<0>();
     }
+    __syncwarp();
+    if (BWD && p.partial && p.groups > 1) asm volatile("bar.arrive 15, %0;" ::"r"(blockDim.x) : "memory");      // the stages are free
     return;
   }
   const int group = threadIdx.x / p.lanes;
@@ -387,16 +409,28 @@ __global__ void __launch_bounds__(544, 1) norm_ring_kernel(const __grid_constant
     }
   }
   if (!ok && (threadIdx.x & 31) == 0) atomicOr(&g_norm_status, 1u);
-  if (BWD && p.partial && ok) {
+  if (BWD && p.partial) {
     constexpr int SUMS = GATED ? 1 : 2;
-    float* const out = p.partial + static_cast<size_t>(blockIdx.x * p.groups + group) * SUMS * a.cols;
+    float* const out = p.partial + static_cast<size_t>(blockIdx.x) * SUMS * a.cols;
+    // the groups' sums meet in the stages' place (a partial sum per group: 1,048,576 x 128 has 4,736 of them, and joining those took 30 us)
+    float* const mine = p.groups > 1 ? reinterpret_cast<float*>(smem) + group * SUMS * a.cols : out;
+    if (p.groups > 1) asm volatile("bar.sync 15, %0;" ::"r"(blockDim.x) : "memory");
 #pragma unroll
     for (int i = 0; i < SUMS; ++i)
 #pragma unroll
       for (int v = 0; v < NV; ++v)
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          if (c.any(v) && c.has(v, j)) out[i * a.cols + c.at(v, j)] = acc[i][v][j];
+          if (c.any(v) && c.has(v, j)) mine[i * a.cols + c.at(v, j)] = acc[i][v][j];
+    if (p.groups > 1) {
+      const int threads = blockDim.x - 32;
+      asm volatile("bar.sync 14, %0;" ::"r"(threads) : "memory");
+      for (int e = threadIdx.x; e < SUMS * a.cols; e += threads) {
+        float x = 0.f;
+        for (int g = 0; g < p.groups; ++g) x += reinterpret_cast<const float*>(smem)[g * SUMS * a.cols + e];
+        out[e] = x;
+      }
+    }
   }
 }
 
@@ -439,36 +473,35 @@ static bool plan(const kda_norm_args& a, bool gated, bool backward, RingParams& 
   int even = 1;      // rows that make 16 bytes even
   while (even * a.cols * std::min(p.size[0], p.size[1]) % 16) even *= 2;
   p.params = (a.cols * (gated ? 4 : 8) + 127) / 128 * 128;
-  const int room = RING_MOST - p.params;
+  // Bytes under way.  The gated norm: all that fit (1,048,576 x 128 forward, stages of 32 KB: four 131.6 us, five 126.5, six 124.4).  The residual norm, whose
+  // forward writes as much as it reads: about 128 KB (32,768 x 4096 forward, fp32 residual: 120 KB 248 us, 144 276, 192 282; bf16 residual: 128 KB
+  // 170, 160 KB 197).
+  const int room = RING_MOST - p.params, most = gated ? room : std::min(room, 128 * 1024);
   // a row for every group in each stage; it has to be so where groups share a warp, elsewhere if all stages fit
   int unit = even;
   while (unit % p.groups) unit += even;
-  if (p.lanes > 32 && static_cast<long long>(STAGES_MOST) * unit * per_row > room) unit = even;
+  if (p.lanes > 32 && static_cast<long long>(STAGES_LEAST) * unit * per_row > most) unit = even;
   p.rows = unit;
-  while (p.rows * per_row < RING_STAGE && (p.rows + unit) * per_row <= room / STAGES_MOST) p.rows += unit;
+  while (p.rows * per_row < RING_STAGE && (p.rows + unit) * per_row <= most / STAGES_LEAST) p.rows += unit;
   p.stage_bytes = 0;
   for (int i = 0; i < 4; ++i) {
     p.off[i] = p.stage_bytes;
     if (p.in[i]) p.stage_bytes += (p.rows * a.cols * p.size[i] + 127) / 128 * 128;
   }
-  p.stages = std::min(STAGES_MOST, room / std::max(1, p.stage_bytes));
+  p.stages = std::min({STAGES_MOST, room / std::max(1, p.stage_bytes), std::max(STAGES_LEAST, most / std::max(1, p.stage_bytes))});
   p.chunks = (a.rows + p.rows - 1) / p.rows;
-  return p.stages >= 2;
+  return p.stages >= 2 && (!backward || p.groups == 1 || p.groups * (gated ? 1 : 2) * a.cols * 4 <= p.stages * p.stage_bytes);
 }
 
 static unsigned ring_ctas(const RingParams& p) { return static_cast<unsigned>(std::min<long long>(p.chunks, sm_count())); }
 
 bool norm_ring_covers(const kda_norm_args& a, bool gated, bool backward) {
-  if (a.rows * a.cols < NORM_RING_MIN || !norm_aligned(a) || (a.io_dtype == KDA_FP32 && (gated ? a.gate_dtype : a.residual_dtype) == KDA_BF16)) return false;
+  if (a.rows * a.cols < ring_min(backward) || !norm_aligned(a) || (a.io_dtype == KDA_FP32 && (gated ? a.gate_dtype : a.residual_dtype) == KDA_BF16)) return false;
   RingParams p{};
   return plan(a, gated, backward, p);
 }
-// the most partial sums of a call: their number depends on the columns alone
-size_t norm_ring_partials(int cols) {
-  int lanes, groups;
-  split(cols, 2, lanes, groups);
-  return static_cast<size_t>(sm_count()) * groups;
-}
+// the most partial sums of a call
+size_t norm_ring_partials() { return static_cast<size_t>(sm_count()); }
 
 template <bool GATED, int XT, int ZT, bool VEC, bool BWD, int NV>
 static int launch_ring_nv(const RingParams& p, cudaStream_t st) {
@@ -502,7 +535,7 @@ int norm_ring(const kda_norm_args& a, bool gated, bool backward, float* partial,
   if (!plan(a, gated, backward, p)) return KDA_E_SHAPE;
   p.a = a;
   p.partial = partial;
-  *partials = static_cast<int>(ring_ctas(p)) * p.groups;
+  *partials = static_cast<int>(ring_ctas(p));
   return gated ? launch_norm<true>(p, backward, st) : launch_norm<false>(p, backward, st);
 }
 

@@ -16,6 +16,7 @@ SHAPES = [(1, 1), (3, 7), (5, 8), (100, 77), (33, 96), (1000, 128), (17, 256), (
 RING = [(300000, 8), (300001, 7), (30001, 77), (25000, 96), (16385, 128), (16384, 128), (9001, 256), (8200, 257), (2101, 1000), (2100, 1001), (860, 2500), (520, 4096), (513, 4100),
         (261, 8191), (257, 8192)]
 
+RING_FORWARD = [(1200001, 7), (110000, 77), (65537, 128), (8400, 1000), (8387, 1001), (3361, 2500), (2101, 4096), (2049, 4100), (1027, 8191), (1026, 8192)]
 
 @pytest.fixture(scope="module", autouse=True)
 def leave_no_memory():
@@ -107,7 +108,7 @@ def check_residual(rows, cols, types, post, scale, seed, eps=1e-6):
     assert t.shape == r.shape
 
 
-@pytest.mark.parametrize("rows,cols", SHAPES + RING)
+@pytest.mark.parametrize("rows,cols", SHAPES + RING + RING_FORWARD)
 def test_gated(rows, cols):
     check_gated(rows, cols, (BF, BF, BF), "silu" if rows % 2 else "sigmoid", seed=rows + cols)
 
@@ -119,7 +120,7 @@ def test_gated_types(rows, cols, types):
     check_gated(rows, cols, types, "sigmoid", seed=4, weight=False, eps=1e-3)
 
 
-@pytest.mark.parametrize("rows,cols", SHAPES + RING)
+@pytest.mark.parametrize("rows,cols", SHAPES + RING + RING_FORWARD)
 def test_residual(rows, cols):
     check_residual(rows, cols, (BF, F if rows % 2 else BF, BF), post=cols % 2 == 0, scale=None if rows % 3 else 0.7, seed=rows + cols)
 

@@ -2,8 +2,6 @@
 One pass over each tensor, forward and backward, in hand-written sm_100a kernels (`csrc/kda_norm.cu`); bfloat16 and float32 tensors, no fallback."""
 from __future__ import annotations
 
-import torch
-
 from . import _lib
 
 _ACTIVATIONS = {"sigmoid": 0, "silu": 1, "swish": 1}
@@ -13,7 +11,6 @@ def _native():
     return _lib._native or _lib.native()
 
 
-@torch.compiler.disable
 def gated_rms_norm(x, gate, weight=None, eps=1e-6, activation="sigmoid"):
     """y = x / sqrt(mean(x^2) + eps) * weight * act(gate) over the last dimension (up to 8192 columns), act = "sigmoid", or "silu" ("swish"): z sigmoid(z).
 
@@ -24,7 +21,6 @@ def gated_rms_norm(x, gate, weight=None, eps=1e-6, activation="sigmoid"):
     return _native().gated_norm(x, gate, weight, eps, _ACTIVATIONS[activation])
 
 
-@torch.compiler.disable
 def residual_rms_norm(x, residual, weight, scale=None, post_weight=None, eps=1e-6):
     """What stands between two blocks: returns (y, r) with r = residual + scale * b and y = r / sqrt(mean(r^2) + eps) * weight, where b is the block's output x or,
     with `post_weight` [D], x / sqrt(mean(x^2) + eps) * post_weight.

@@ -24,6 +24,10 @@ static int validate(const kda_delta_args& a, bool backward) {
     if (addr(a.bwd_workspace) & 255u) return KDA_E_ALIGN;
   }
   if ((bits & 15u) || (addr(a.workspace) & 255u)) return KDA_E_ALIGN;
+  // the small tensors are read an element at a time
+  if (((addr(a.g) | (backward ? addr(a.dg) : 0)) & (a.g_dtype == KDA_BF16 ? 1u : 3u)) || ((addr(a.beta) | (backward ? addr(a.dbeta) : 0)) & (a.beta_dtype == KDA_BF16 ? 1u : 3u)) ||
+      (addr(a.cu_seqlens) & 3u))
+    return KDA_E_ALIGN;
   return KDA_OK;
 }
 

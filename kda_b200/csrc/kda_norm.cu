@@ -457,6 +457,13 @@ int check_norm(const kda_norm_args& a, bool gated, bool backward) {
   if (!a.x || (gated ? !a.gate : (!a.residual || !a.weight))) return KDA_E_NULL;
   if (!backward && (!a.y || (!gated && !a.r))) return KDA_E_NULL;
   if (backward && (!a.dx || (gated ? (!a.dy || !a.dgate) : (!a.dy && !a.dr)))) return KDA_E_NULL;
+  // elements at their natural boundary at least (16 bytes: the wide forms)
+  uintptr_t bf = 0, fp = 0;
+  for (const auto& [p, dtype] : {std::pair<const void*, int>{a.x, a.io_dtype}, {a.y, a.io_dtype}, {a.dy, a.io_dtype}, {a.dx, a.io_dtype}, {a.gate, a.gate_dtype}, {a.dgate, a.gate_dtype},
+                                 {a.residual, a.residual_dtype}, {a.r, a.residual_dtype}, {a.dr, a.residual_dtype}, {a.dresidual, a.residual_dtype}, {a.weight, a.weight_dtype},
+                                 {a.dweight, a.weight_dtype}, {a.post_weight, a.post_dtype}, {a.dpost_weight, a.post_dtype}, {a.scale, a.scale_dtype}, {a.dscale, a.scale_dtype}})
+    (dtype == KDA_BF16 ? bf : fp) |= reinterpret_cast<uintptr_t>(p);
+  if ((bf & 1u) || (fp & 3u)) return KDA_E_ALIGN;
   if (backward && (a.dweight || a.dpost_weight || a.dscale)) {
     if (!a.workspace) return KDA_E_NULL;
     if (reinterpret_cast<uintptr_t>(a.workspace) & 15u) return KDA_E_ALIGN;

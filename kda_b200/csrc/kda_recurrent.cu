@@ -490,5 +490,11 @@ extern "C" int kda_delta_recurrent_fwd(const kda_recurrent_args* args, int32_t s
   if (args && ((args->g_raw_dtype != KDA_BF16 && args->g_raw_dtype != KDA_FP32) || (args->beta_raw_dtype != KDA_BF16 && args->beta_raw_dtype != KDA_FP32)))
     return KDA_E_DTYPE;
   if (args && args->state_indices && (slots <= 0 || slot_columns <= 0)) return KDA_E_SHAPE;
+  if (args) {      // the small tensors are read an element at a time
+    auto addr = [](const void* p) { return reinterpret_cast<uintptr_t>(p); };
+    if ((addr(args->g) & (args->g_raw_dtype == KDA_BF16 ? 1u : 3u)) || (addr(args->beta) & (args->beta_raw_dtype == KDA_BF16 ? 1u : 3u)) ||
+        ((addr(args->cu_seqlens) | addr(args->state_indices) | addr(args->num_accepted_tokens) | addr(args->A_log) | addr(args->dt_bias)) & 3u))
+      return KDA_E_ALIGN;
+  }
   return recurrent_fwd(args, true, slots, slot_columns, stream);
 }

@@ -26,7 +26,7 @@ def fused_recurrent_gated_delta_fwd(q, k, v, g, beta, A_log=None, dt_bias=None, 
     g = -exp(A_log) softplus(g + dt_bias) with A_log, dt_bias [HV], or lower_bound sigmoid(exp(A_log) (g + dt_bias))).  K in {32, 64, 128, 256}, V a multiple of 32.
     With `inplace_final_state` states are written over `initial_state`, a float32 [slots, HV, K, V] pool where `ssm_state_indices` [N] or [N, T] names the slot of
     every token: a sequence starts from the slot of its first token (with `num_accepted_tokens` [N] of its last accepted one) and the state behind token t lands
-    in that token's slot.  No two sequences may name the same slot.  A sequence whose starting slot lies outside the pool (-1: a padded entry) or whose accepted count
+    in that token's slot.  Slots are read as 32-bit numbers; no two sequences may name the same one.  A sequence whose starting slot lies outside the pool (-1: a padded entry) or whose accepted count
     names no column gets zeros for its rows of o and touches no state; a later token's slot outside the pool is left out.  Returns (o, states)."""
     return _native().delta_recurrent_fwd(
         q, k, v, g, beta, A_log, dt_bias, initial_state, scale, output_final_state, inplace_final_state, cu_seqlens, ssm_state_indices, num_accepted_tokens,

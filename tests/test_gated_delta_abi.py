@@ -26,6 +26,7 @@ def delta_args(**kw):
 BAD_DELTA = [(dict(K=12), -2), (dict(K=0), -2), (dict(K=136), -2), (dict(V=256), -2), (dict(H=0), -2), (dict(HQ=3), -2), (dict(HQ=8), -2), (dict(N=-1), -2), (dict(tokens=-1), -2),
              (dict(N=3), -2), (dict(scan_slices=3), -2), (dict(tokens=1 << 31, N=1), -2), (dict(H=1 << 30, HQ=0), -2), (dict(io_dtype=0), -3), (dict(g_dtype=7), -3),
              (dict(beta_dtype=-1), -3), (dict(q=0), -1), (dict(beta=0), -1), (dict(workspace=0), -1), (dict(q=520), -4), (dict(h0=516), -4), (dict(workspace=640), -4),
+             (dict(g=514), -4), (dict(beta=513), -4), (dict(cu_seqlens=514), -4),
              (dict(workspace_bytes=64), -5)]
 
 
@@ -65,7 +66,7 @@ def test_recurrent_refusals(lib):      # noqa: F811
     assert call(slots=0, state_indices=512) == call(columns=0, state_indices=512) == call(slots=-1, state_indices=512) == -2      # nothing can be followed
     assert call(state_indices=512, ht=1024) == -2
     assert call(num_accepted_tokens=512) == call(v=0) == -1
-    assert call(q=520) == call(h0=516, ht=516) == -4
+    assert call(q=520) == call(h0=516, ht=516) == call(g=514) == call(beta=513) == call(state_indices=514) == call(A_log=513) == -4
     assert call(N=0, tokens=0) == 0
 
 
@@ -93,6 +94,7 @@ def test_norm_refusals_of_one_call(lib):      # noqa: F811
     assert gf(activation=2) == -2 and gf(gate_dtype=9) == -3 and rf(residual_dtype=9) == -3
     assert gf(gate=0) == gf(y=0) == gb(dgate=0) == gb(dy=0) == gb(workspace=0) == -1
     assert rf(weight=0) == rf(residual=0) == rf(r=0) == rb(dx=0) == rb(dy=0, dr=0) == rb(workspace=0) == -1
+    assert gf(x=513) == rf(residual=514) == gf(weight=513) == rb(dr=514) == gb(dgate=513) == -4
     assert gb(workspace_bytes=16) == rb(workspace_bytes=16) == -5 and gb(workspace=520) == -4
 
 

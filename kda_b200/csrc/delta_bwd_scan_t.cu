@@ -5,7 +5,7 @@
 //   2   x^T Tm + dO^T Pt            (128 v x 64 tokens, K = 64;  f)
 //   3   y^T K + (scale exp(G) dO)^T Q   (128 v x 128 keys, K = 64;  y = -beta exp(G) f), added to the gradient that the registers hold and decay
 // The terms with dO do not depend on the chain and run behind product 1.  x (then y) takes the columns that its own thread has just read product 1 from.
-// f leaves through dO's tile, dv through a tile of its own.
+// f leaves through dO's tile, dv through a tile of its own.  8 x 4,096 tokens x 32 heads 489 us (two rounds of units), 4.0 a chunk.
 #include "delta.cuh"
 
 namespace kda {

@@ -7,7 +7,8 @@
 //   3   (w v_new)^T K             (128 v x 128 keys, K = 64 tokens), added to the state that the registers hold and decay
 // A thread has one value column, 32 keys of its state and 16 tokens of a chunk.  v, o and v_new are turned on the way through shared memory, two bytes a
 // lane: o in q's rows once product 1 has read them, v_new (for a backward) in v's tile.  Tiles and full chunks of o leave by bulk copies.
-// Bound by the chain of a chunk: the products' 2.3 k cycles and three hand-overs each way.
+// Bound by the chain of a chunk, 3.6 us: the products' 2.3 k cycles and three hand-overs each way.  8 x 4,096 tokens x 32 heads with what a backward needs 504 us
+// (two rounds of units; the bytes alone 365).
 #include "delta.cuh"
 
 namespace kda {

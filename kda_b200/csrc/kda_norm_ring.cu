@@ -4,8 +4,8 @@
 // Bound by HBM.  A thread that loads its columns, waits for the row's sums and stores keeps too few bytes under way: 32,768 x 4096 backward 904 us, 1,048,576 x 128
 // backward 389, with half of HBM's rate.  Here one warp keeps 100 to 200 KB per SM coming and going whatever the others wait for.  Rows are copied as runs
 // of bytes, so columns need not be a multiple of anything: a stage holds as many rows as make 16 bytes even.
-//   us, forward + backward: gated 1,048,576 x 128 125 + 207 (6.4 TB/s); residual 32,768 x 4096 with an fp32 residual and post weight 248 + 531 (6.5, 4.5 TB/s: the
-//   backward's rows are read from shared memory four times over; its copies alone take 392)
+//   us, forward + backward: gated 1,048,576 x 128 125 + 207 (6.4 TB/s); residual 32,768 x 4096 with an fp32 residual and post weight 247 + 472 (6.5, 5.1 TB/s: the
+//   backward's copies alone take 392, and the four sums of a row one after the other are not quite hidden behind them)
 #include <algorithm>
 
 #include "kda_norm.cuh"
@@ -164,23 +164,41 @@ __device__ __forceinline__ void gated_row(const kda_norm_args& a, const float* w
 }
 
 // A row of the residual norm.  x, r, dy, dr: the row of x, of the residual, of their gradients (or NULL); results over x and r.  sw: scale times post_weight.
-template <int XT, int RT, bool VEC, bool BWD, int NV>
+template <int XT, int RT, bool VEC, bool BWD, int NV, bool ROOMY>
 __device__ __forceinline__ void residual_row(const kda_norm_args& a, const float* w_, const float* sw_, const Cols<VEC>& c, GroupSum& sum, bool there, unsigned char* x_,
-                                             unsigned char* r_, const unsigned char* dy_, const unsigned char* dr_, float (&acc)[2][NV][8]) {
+                                             unsigned char* r_, const unsigned char* dy_, const unsigned char* dr_, float (&acc)[2][NV][8], const float (&wr)[ROOMY ? NV : 1][8],
+                                             const float (&swr)[ROOMY ? NV : 1][8]) {
   const float inv = 1.f / a.cols;
   float rstd1 = 1.f, ss = 0.f;
-  // x is read from shared memory wherever it is needed: with it, r, t and the sums over rows in registers the backward spilled, into an L1 that the ring leaves
-  // little of (32,768 x 4096: 596 us)
+  // ROOMY: x and the parameters stay in registers.  Elsewhere x is read from shared memory wherever it is needed: with it, r, t and the sums over rows in
+  // registers the backward spilled, into an L1 that the ring leaves little of (32,768 x 4096: 596 us)
+  float xs[ROOMY ? NV : 1][8];
+  if constexpr (ROOMY) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) get8<XT, VEC>(x_, c, i, xs[i]);
+  }
+  auto raw = [&](int i, float (&x)[8]) {
+    if constexpr (ROOMY) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = xs[i][j];
+    } else get8<XT, VEC>(x_, c, i, x);
+  };
   auto n1 = [&](int i, float (&x)[8]) {
-    get8<XT, VEC>(x_, c, i, x);
+    raw(i, x);
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[j] *= rstd1;
+  };
+  auto param = [&](const float* p, const float (&kept)[ROOMY ? NV : 1][8], int i, float (&v)[8]) {
+    if constexpr (ROOMY) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = kept[i][j];
+    } else get_param<VEC>(p, c, i, v);
   };
   if (a.post_weight) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       float x[8];
-      get8<XT, VEC>(x_, c, i, x);
+      raw(i, x);
 #pragma unroll
       for (int j = 0; j < 8; ++j) ss = fmaf(x[j], x[j], ss);
     }
@@ -193,7 +211,7 @@ __device__ __forceinline__ void residual_row(const kda_norm_args& a, const float
     float x[8], sw[8];
     n1(i, x);
     get8<RT, VEC>(r_, c, i, r[i]);
-    get_param<VEC>(sw_, c, i, sw);
+    param(sw_, swr, i, sw);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       r[i][j] = fmaf(sw[j], x[j], r[i][j]);      // (columns that are not there: x and the residual read as zero)
@@ -207,7 +225,7 @@ __device__ __forceinline__ void residual_row(const kda_norm_args& a, const float
     for (int i = 0; i < NV; ++i) {
       float w[8];
       put8<RT, VEC>(r_, c, i, r[i]);
-      get_param<VEC>(w_, c, i, w);
+      param(w_, wr, i, w);
 #pragma unroll
       for (int j = 0; j < 8; ++j) w[j] *= r[i][j] * rstd;
       put8<XT, VEC>(x_, c, i, w);
@@ -221,7 +239,7 @@ __device__ __forceinline__ void residual_row(const kda_norm_args& a, const float
       else
 #pragma unroll
         for (int j = 0; j < 8; ++j) t[i][j] = 0.f;
-      get_param<VEC>(w_, c, i, w);
+      param(w_, wr, i, w);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         r[i][j] *= rstd;
@@ -240,7 +258,7 @@ __device__ __forceinline__ void residual_row(const kda_norm_args& a, const float
       else
 #pragma unroll
         for (int j = 0; j < 8; ++j) dr[j] = 0.f;
-      get_param<VEC>(sw_, c, i, sw);
+      param(sw_, swr, i, sw);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         t[i][j] = fmaf(rstd, fmaf(-dot, r[i][j], t[i][j]), dr[j]);
@@ -280,8 +298,9 @@ struct RingParams {
 
 }  // namespace
 
-template <bool GATED, int XT, int ZT, bool VEC, bool BWD, int NV>
-__global__ void __launch_bounds__(544, 1) norm_ring_kernel(const __grid_constant__ RingParams p) {
+// ROOMY (the residual norm's backward): half the threads, with registers for all of a row that they need more than once.
+template <bool GATED, int XT, int ZT, bool VEC, bool BWD, int NV, bool ROOMY>
+__global__ void __launch_bounds__(ROOMY ? 288 : 544, 1) norm_ring_kernel(const __grid_constant__ RingParams p) {
   extern __shared__ __align__(128) unsigned char smem_raw[];
   __shared__ uint64_t full[STAGES_MOST], done[STAGES_MOST];
   __shared__ __align__(16) float part[16][32];
@@ -383,7 +402,14 @@ __global__ void __launch_bounds__(544, 1) norm_ring_kernel(const __grid_constant
   const int group = threadIdx.x / p.lanes;
   const Cols<VEC> c{static_cast<int>(threadIdx.x) % p.lanes, p.lanes, a.cols};
   GroupSum sum{part[group & 15], p.lanes, 1 + (group & 15), c.lane >> 5};
-  float acc[2][NV][8] = {};
+  float acc[2][NV][8] = {}, wr[ROOMY ? NV : 1][8], swr[ROOMY ? NV : 1][8];
+  if constexpr (ROOMY) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      get_param<VEC>(w_, c, i, wr[i]);
+      get_param<VEC>(sw_, c, i, swr[i]);
+    }
+  }
   constexpr int XS = XT == KDA_BF16 ? 2 : 4, ZS = ZT == KDA_BF16 ? 2 : 4;
   int k = 0, s = 0, next = group;      // next: this group's next row of the stage
   bool ok = true;
@@ -398,8 +424,8 @@ __global__ void __launch_bounds__(544, 1) norm_ring_kernel(const __grid_constant
       if constexpr (GATED)
         gated_row<XT, ZT, VEC, BWD, NV>(a, w_, c, sum, there, st + p.off[0] + at * XS, st + p.off[1] + at * ZS, st + p.off[2] + at * XS, acc);
       else
-        residual_row<XT, ZT, VEC, BWD, NV>(a, w_, sw_, c, sum, there, st + p.off[0] + at * XS, st + p.off[1] + at * ZS, a.dy ? st + p.off[2] + at * XS : nullptr,
-                                       a.dr ? st + p.off[3] + at * ZS : nullptr, acc);
+        residual_row<XT, ZT, VEC, BWD, NV, ROOMY>(a, w_, sw_, c, sum, there, st + p.off[0] + at * XS, st + p.off[1] + at * ZS, a.dy ? st + p.off[2] + at * XS : nullptr,
+                                       a.dr ? st + p.off[3] + at * ZS : nullptr, acc, wr, swr);
     }
     next = r - p.rows;
     fence_proxy_async();
@@ -445,16 +471,24 @@ int norm_ring_status(uint32_t* host_out) {
   return static_cast<int>(e);
 }
 
-// Vectors of eight columns per thread.  Two: what a thread does once a row (sums over it, addresses) it does for sixteen columns.  The residual norm's backward
-// has sums over rows, r and t in registers and takes one where a row's threads allow it (32,768 x 4096: two 575 us, spilling into an L1 that the ring
-// leaves little of).
-static int vectors(int cols, bool gated, bool backward) { return backward && !gated && cols <= 4096 ? 1 : 2; }
 // threads of a row and rows at a time
-static void split(int cols, int nv, int& lanes, int& groups) {
+static void split(int cols, int nv, int threads, int& lanes, int& groups) {
   const int need = (cols + 8 * nv - 1) / (8 * nv);
   for (lanes = 1; lanes < need && lanes < 32; lanes *= 2) {}
   if (need > 32) lanes = (need + 31) / 32 * 32;
-  groups = 512 / lanes;
+  groups = threads / lanes;
+}
+// Vectors of eight columns per thread.  Two: what a thread does once a row (sums over it, addresses) it does for sixteen columns.  The residual norm's backward has
+// sums over rows, r and t in registers besides: one, where a row's threads allow it; or, with a norm of x to go back through and whole vectors, two with half the
+// threads (ROOMY), if these come to 200.  us, 2^26 elements with an fp32 residual, one | ROOMY: 128 columns 214 | 203, 512 261 | 221, 1,024 258 | 242, 4,096 279 | 253; with
+// two and 512 threads 4,096 took 300, spilling into an L1 that the ring leaves little of.  On the other side, without post_weight (bf16): 1,024 173 | 178; columns one by
+// one: 1,001 456 | 501; 160 threads: 2,500 474 | 610.
+struct Form { int nv; bool roomy; };
+static Form form(const kda_norm_args& a, bool gated, bool backward) {
+  if (gated || !backward || a.cols > 4096) return {2, false};
+  int lanes, groups;
+  split(a.cols, 2, 256, lanes, groups);
+  return a.post_weight && a.cols % 8 == 0 && lanes * groups >= 200 ? Form{2, true} : Form{1, false};
 }
 
 // How a call goes through the ring: false where its rows are too wide for two stages.
@@ -468,7 +502,8 @@ static bool plan(const kda_norm_args& a, bool gated, bool backward, RingParams& 
   p.size[1] = p.size[3] = other == KDA_BF16 ? 2 : 4;
   p.out[0] = backward ? a.dx : a.y;
   p.out[1] = backward ? (gated ? a.dgate : a.dresidual) : (gated ? nullptr : a.r);
-  split(a.cols, vectors(a.cols, gated, backward), p.lanes, p.groups);
+  const Form f = form(a, gated, backward);
+  split(a.cols, f.nv, f.roomy ? 256 : 512, p.lanes, p.groups);
   int per_row = 0;
   for (int i = 0; i < 4; ++i)
     if (p.in[i]) per_row += p.size[i] * a.cols;
@@ -505,20 +540,24 @@ bool norm_ring_covers(const kda_norm_args& a, bool gated, bool backward) {
 // the most partial sums of a call
 size_t norm_ring_partials() { return static_cast<size_t>(sm_count()); }
 
-template <bool GATED, int XT, int ZT, bool VEC, bool BWD, int NV>
+template <bool GATED, int XT, int ZT, bool VEC, bool BWD, int NV, bool ROOMY>
 static int launch_ring_nv(const RingParams& p, cudaStream_t st) {
   static DeviceOnce once;
-  const int rc = once.run([] { return cudaFuncSetAttribute(norm_ring_kernel<GATED, XT, ZT, VEC, BWD, NV>, cudaFuncAttributeMaxDynamicSharedMemorySize, RING_MOST); });
+  const int rc = once.run([] { return cudaFuncSetAttribute(norm_ring_kernel<GATED, XT, ZT, VEC, BWD, NV, ROOMY>, cudaFuncAttributeMaxDynamicSharedMemorySize, RING_MOST); });
   if (rc != KDA_OK) return rc;
-  norm_ring_kernel<GATED, XT, ZT, VEC, BWD, NV><<<ring_ctas(p), p.lanes * p.groups + 32, p.params + p.stages * p.stage_bytes, st>>>(p);
+  norm_ring_kernel<GATED, XT, ZT, VEC, BWD, NV, ROOMY><<<ring_ctas(p), p.lanes * p.groups + 32, p.params + p.stages * p.stage_bytes, st>>>(p);
   return static_cast<int>(cudaGetLastError());
 }
 template <bool GATED, int XT, int ZT, bool VEC, bool BWD>
 static int launch_ring(const RingParams& p, cudaStream_t st) {
   if constexpr (BWD && !GATED) {
-    if (vectors(p.a.cols, GATED, BWD) == 1) return launch_ring_nv<GATED, XT, ZT, VEC, BWD, 1>(p, st);
+    const Form f = form(p.a, GATED, BWD);
+    if constexpr (VEC) {
+      if (f.roomy) return launch_ring_nv<GATED, XT, ZT, VEC, BWD, 2, true>(p, st);
+    }
+    if (f.nv == 1) return launch_ring_nv<GATED, XT, ZT, VEC, BWD, 1, false>(p, st);
   }
-  return launch_ring_nv<GATED, XT, ZT, VEC, BWD, 2>(p, st);
+  return launch_ring_nv<GATED, XT, ZT, VEC, BWD, 2, false>(p, st);
 }
 template <bool GATED, int XT, int ZT>
 static int launch_types(const RingParams& p, bool backward, cudaStream_t st) {

@@ -79,6 +79,21 @@ inline Ws carve(unsigned char* base, unsigned char* bwd, int64_t tokens, int N, 
   return w;
 }
 
+// The walks of sixteen compute warps and a warpgroup of helpers (of which two warps work): 20 warps of 96 registers a thread at launch, 61,440 in all.  The helpers
+// give 32 of theirs up, and the compute warps have 104: 512 x 104 + 128 x 64 = 61,440.
+constexpr int CREW_THREADS = 640, CREW_REGS = 96;
+__device__ __forceinline__ void compute_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 104;"); }
+__device__ __forceinline__ void helper_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 64;"); }
+// the split draws on what the kernel was launched with: with fewer, the compute warps would wait forever
+template <class K>
+cudaError_t crew_ready(K kernel, int smem) {
+  cudaFuncAttributes f{};
+  const cudaError_t e = cudaFuncGetAttributes(&f, kernel);
+  if (e != cudaSuccess) return e;
+  if ((f.numRegs + 7) / 8 * 8 < CREW_REGS) return cudaErrorLaunchOutOfResources;
+  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+}
+
 struct PrepParams {
   ChunkMap map;
   const void *g, *beta;           // [tokens][H] of g_dtype, beta_dtype

@@ -347,7 +347,7 @@ static int launch_vc(const RScanParams& p, int units, cudaStream_t st) {
 }
 
 int launch_bwd_scan(const RScanParams& p, int units, int slices, cudaStream_t st) {
-  // (32 chunks each, us with 1 | 2 | 4 CTAs per unit: 37 units 127 | 113 | 86, 48 127 | 113 | 162, 74 127 | 115 | 166, 96 128 | 220 | 242)
+  // (32 chunks each, us with 1 | 2 | 4 CTAs per unit: 37 units 120 | 112 | 85, 48 120 | 112 | 161, 74 121 | 114 | 165, 96 122 | 219 | 241)
   if (slices == 0) slices = 4 * units <= sm_count() ? 4 : 2 * units <= sm_count() ? 2 : 1;
   return slices == 4 ? launch_vc<32>(p, units, st) : slices == 2 ? launch_vc<64>(p, units, st) : launch_bwd_scan_t(p, units, st);
 }

@@ -5,7 +5,7 @@
 //   2   x^T Tm + dO^T Pt            (128 v x 64 tokens, K = 64;  f)
 //   3   y^T K + (scale exp(G) dO)^T Q   (128 v x 128 keys, K = 64;  y = -beta exp(G) f), added to the gradient that the registers hold and decay
 // The terms with dO do not depend on the chain and run behind product 1.  x (then y) takes the columns that its own thread has just read product 1 from.
-// f leaves through dO's tile, dv through a tile of its own.  8 x 4,096 tokens x 32 heads 489 us (two rounds of units), 4.0 a chunk.
+// f leaves through dO's tile, dv through a tile of its own.  8 x 4,096 tokens x 32 heads 473 us (two rounds of units), 3.7 a chunk.
 #include "delta.cuh"
 
 namespace kda {
@@ -13,7 +13,7 @@ namespace delta {
 
 namespace {
 
-constexpr int CW = 16, NT = (CW + 2) * 32, W_ISSUE = CW;
+constexpr int CW = 16, NT = CREW_THREADS, W_ISSUE = CW;
 
 struct RTSmem {
   unsigned char KQ[2][2][16384];        // two stages, of dO and of what leaves as dv too
@@ -68,6 +68,7 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_scan_t_kernel(const __grid_co
   const uint32_t tb = s.tmem_slot, tq = tb + (static_cast<uint32_t>(32 * q4) << 16);
 
   if (warp < CW) {
+    compute_registers();
     // ================= the chain =================
     const int v = 32 * q4 + lane, g = warp >> 2, k0 = 32 * g, t0 = 16 * g;      // value column; first key and first token of this thread
     const size_t sb = (static_cast<size_t>(seq) * p.H + h) * p.kc * p.vc + v;
@@ -97,8 +98,6 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_scan_t_kernel(const __grid_co
       fence_proxy_async();
       warp_arrive(&s.hReady, lane);
       const float last = vec[V_LAST];
-#pragma unroll
-      for (int e = 0; e < 32; ++e) S[e] *= last;
       // ---- beside product 1: dO and scaled dO as operands ----
       const uint32_t at_o = column_at(s.dO[i & 1][v >> 6], t0, v & 63), at_v = column_at(s.dV[i & 1][v >> 6], t0, v & 63);
       {
@@ -170,7 +169,7 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_scan_t_kernel(const __grid_co
         umma::tmem_ld16(tq + D3 + k0 + e, f);
         umma::tmem_ld_wait();
 #pragma unroll
-        for (int j = 0; j < 16; ++j) S[e + j] += f[j];
+        for (int j = 0; j < 16; ++j) S[e + j] = fmaf(S[e + j], last, f[j]);
       }
       umma::fence_before_sync();
     }
@@ -182,117 +181,120 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_scan_t_kernel(const __grid_co
       for (int e = 0; e < 32; ++e)
         if (k0 + e < p.kc) p.dh0[sb + static_cast<size_t>(k0 + e) * p.vc] = S[e];
     }
-  } else if (warp == W_ISSUE) {
-    if (lane == 0) {
-      constexpr uint32_t id1 = umma::instr_desc(128, 64, false, false), id2 = umma::instr_desc(128, 64, false, true), id3 = umma::instr_desc(128, 128, false, true);
-      const uint32_t aT = smem_u32(s.TP[0]);
-      const uint64_t dT = umma::desc_mnmajor(aT, 0, 8192), dP = umma::desc_mnmajor(aT + 8192, 0, 8192);      // their low parts: 16 KiB behind
-      bool ok = true;
-      for (int i = 0; i < nchunks && ok; ++i) {
-        const uint32_t aK = smem_u32(s.KQ[i & 1][0]);
-        const uint64_t dK = umma::desc_kmajor(aK, 0), dKm = umma::desc_mnmajor(aK, 0, 16384), dQm = umma::desc_mnmajor(aK + 8192, 0, 16384);
-        if (s.dead || !mbar_wait(&s.fullA[i & 1], (i >> 1) & 1) || !mbar_wait(&s.hReady, i & 1)) { ok = false; break; }
-        umma::fence_after_sync();
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const uint64_t b = dK + (k >> 2) * 1024u + (k & 3) * umma::KSTEP_KMAJOR;
-          umma::mma_ts(tb + D1, tb + AH + 8 * k, b, id1, k > 0);
-          umma::mma_ts(tb + D1, tb + AL + 8 * k, b, id1, 1);
-        }
-        umma::commit(&s.m1);
-        bulk_s2g(p.DH + (static_cast<size_t>(c0 + nchunks - 1 - i) * p.H + h) * T_STATE, s.H[0], 16384);
-        bulk_s2g(p.DH + (static_cast<size_t>(c0 + nchunks - 1 - i) * p.H + h) * T_STATE + 16384, s.H[1], 16384);
-        bulk_commit();
-        if (!mbar_wait(&s.fullB, i & 1) || !mbar_wait(&s.dReady, i & 1)) { ok = false; break; }
-        umma::fence_after_sync();
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          umma::mma_ts(tb + D2, tb + DO + 8 * k, dP + k * umma::KSTEP_MNMAJOR, id2, k > 0);
-          umma::mma_ts(tb + D2, tb + DO + 8 * k, dP + 1024u + k * umma::KSTEP_MNMAJOR, id2, 1);
-        }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          umma::mma_ts(tb + D3, tb + OH + 8 * k, dQm + k * umma::KSTEP_MNMAJOR, id3, k > 0);
-          umma::mma_ts(tb + D3, tb + OL + 8 * k, dQm + k * umma::KSTEP_MNMAJOR, id3, 1);
-        }
-        if (!mbar_wait(&s.xReady, i & 1)) { ok = false; break; }
-        umma::fence_after_sync();
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint64_t b = dT + k * umma::KSTEP_MNMAJOR;
-          umma::mma_ts(tb + D2, tb + D1 + 16 * k, b, id2, 1);
-          umma::mma_ts(tb + D2, tb + D1 + 16 * k + 8, b, id2, 1);
-          umma::mma_ts(tb + D2, tb + D1 + 16 * k, b + 1024u, id2, 1);
-        }
-        umma::commit(&s.m2);
-        umma::commit(&s.freeB);
-        if (!mbar_wait(&s.yReady, i & 1)) { ok = false; break; }
-        umma::fence_after_sync();
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          umma::mma_ts(tb + D3, tb + D1 + 16 * k, dKm + k * umma::KSTEP_MNMAJOR, id3, 1);
-          umma::mma_ts(tb + D3, tb + D1 + 16 * k + 8, dKm + k * umma::KSTEP_MNMAJOR, id3, 1);
-        }
-        bulk_wait_read<0>();      // m3 also says that dh's tile may be overwritten
-        umma::commit(&s.m3);
-        umma::commit(&s.freeA[i & 1]);
-      }
-      if (!ok) {
-        s.dead = 1;
-        atomicOr(p.status, KDA_STATUS_BWD_SCAN_MMA_WAIT);
-      }
-      bulk_wait_read<0>();
-    }
-    __syncwarp();
   } else {
-    if (lane == 0) {
-      const int hq = h / p.grp;
-      auto first = [&](int i) { return static_cast<int>(tok_begin + static_cast<long long>(nchunks - 1 - i) * C); };
-      auto tile_of = [&](int i) { return static_cast<size_t>(c0 + nchunks - 1 - i) * p.H + h; };
-      auto loadA = [&](int i) {
-        const int b = i & 1, tok0 = first(i);
-        mbar_expect_tx(&s.fullA[b], 6 * 8192 + VEC_COPY);
-        for (int x = 0; x < 2; ++x) tma_load_rows(s.KQ[b][x], &p.tm_k, 64 * x, hq, tok0, &s.fullA[b]);
-        for (int x = 0; x < 2; ++x) tma_load_rows(s.KQ[b][x] + 8192, &p.tm_q, 64 * x, hq, tok0, &s.fullA[b]);
-        for (int x = 0; x < 2; ++x) tma_load_rows(s.dO[b][x], &p.tm_do, 64 * x, h, tok0, &s.fullA[b]);
-        bulk_g2s(s.vec[b], p.VEC + tile_of(i) * T_VEC, VEC_COPY, &s.fullA[b]);
-      };
-      auto loadB = [&](int i) {
-        mbar_expect_tx(&s.fullB, 2 * 16384);
-        bulk_g2s(s.TP[0], p.TP + tile_of(i) * T_TP, 32768, &s.fullB);
-      };
-      bool ok = true;
-      if (nchunks > 0) {
-        loadA(0);
-        loadB(0);
-        if (nchunks > 1) loadA(1);
-      }
-      for (int i = 0; i < nchunks; ++i) {
-        if (i + 2 < nchunks) bulk_prefetch(p.TP + tile_of(i + 2) * T_TP, 32768);      // into L2
-        if (i + 1 < nchunks) {
-          if (s.dead || !mbar_wait(&s.freeB, i & 1)) { ok = false; break; }
-          loadB(i + 1);
-        }
-        if (s.dead || !mbar_wait(&s.oReady, i & 1)) { ok = false; break; }
+    helper_registers();
+    if (warp == W_ISSUE) {
+      if (lane == 0) {
+        constexpr uint32_t id1 = umma::instr_desc(128, 64, false, false), id2 = umma::instr_desc(128, 64, false, true), id3 = umma::instr_desc(128, 128, false, true);
+        const uint32_t aT = smem_u32(s.TP[0]);
+        const uint64_t dT = umma::desc_mnmajor(aT, 0, 8192), dP = umma::desc_mnmajor(aT + 8192, 0, 8192);      // their low parts: 16 KiB behind
+        bool ok = true;
+        for (int i = 0; i < nchunks && ok; ++i) {
+          const uint32_t aK = smem_u32(s.KQ[i & 1][0]);
+          const uint64_t dK = umma::desc_kmajor(aK, 0), dKm = umma::desc_mnmajor(aK, 0, 16384), dQm = umma::desc_mnmajor(aK + 8192, 0, 16384);
+          if (s.dead || !mbar_wait(&s.fullA[i & 1], (i >> 1) & 1) || !mbar_wait(&s.hReady, i & 1)) { ok = false; break; }
+          umma::fence_after_sync();
 #pragma unroll
-        for (int x = 0; x < 2; ++x) bulk_s2g(p.DF + tile_of(i) * T_VN + x * 8192, s.dO[i & 1][x], 8192);
-        if (tok_end - first(i) >= C) {
-          for (int x = 0; x < 2 && 64 * x < p.vc; ++x) tma_store_rows(&p.tm_dv, 64 * x, h, first(i), s.dV[i & 1][x]);
+          for (int k = 0; k < 8; ++k) {
+            const uint64_t b = dK + (k >> 2) * 1024u + (k & 3) * umma::KSTEP_KMAJOR;
+            umma::mma_ts(tb + D1, tb + AH + 8 * k, b, id1, k > 0);
+            umma::mma_ts(tb + D1, tb + AL + 8 * k, b, id1, 1);
+          }
+          umma::commit(&s.m1);
+          bulk_s2g(p.DH + (static_cast<size_t>(c0 + nchunks - 1 - i) * p.H + h) * T_STATE, s.H[0], 16384);
+          bulk_s2g(p.DH + (static_cast<size_t>(c0 + nchunks - 1 - i) * p.H + h) * T_STATE + 16384, s.H[1], 16384);
+          bulk_commit();
+          if (!mbar_wait(&s.fullB, i & 1) || !mbar_wait(&s.dReady, i & 1)) { ok = false; break; }
+          umma::fence_after_sync();
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            umma::mma_ts(tb + D2, tb + DO + 8 * k, dP + k * umma::KSTEP_MNMAJOR, id2, k > 0);
+            umma::mma_ts(tb + D2, tb + DO + 8 * k, dP + 1024u + k * umma::KSTEP_MNMAJOR, id2, 1);
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            umma::mma_ts(tb + D3, tb + OH + 8 * k, dQm + k * umma::KSTEP_MNMAJOR, id3, k > 0);
+            umma::mma_ts(tb + D3, tb + OL + 8 * k, dQm + k * umma::KSTEP_MNMAJOR, id3, 1);
+          }
+          if (!mbar_wait(&s.xReady, i & 1)) { ok = false; break; }
+          umma::fence_after_sync();
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint64_t b = dT + k * umma::KSTEP_MNMAJOR;
+            umma::mma_ts(tb + D2, tb + D1 + 16 * k, b, id2, 1);
+            umma::mma_ts(tb + D2, tb + D1 + 16 * k + 8, b, id2, 1);
+            umma::mma_ts(tb + D2, tb + D1 + 16 * k, b + 1024u, id2, 1);
+          }
+          umma::commit(&s.m2);
+          umma::commit(&s.freeB);
+          if (!mbar_wait(&s.yReady, i & 1)) { ok = false; break; }
+          umma::fence_after_sync();
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            umma::mma_ts(tb + D3, tb + D1 + 16 * k, dKm + k * umma::KSTEP_MNMAJOR, id3, 1);
+            umma::mma_ts(tb + D3, tb + D1 + 16 * k + 8, dKm + k * umma::KSTEP_MNMAJOR, id3, 1);
+          }
+          bulk_wait_read<0>();      // m3 also says that dh's tile may be overwritten
+          umma::commit(&s.m3);
+          umma::commit(&s.freeA[i & 1]);
         }
-        bulk_commit();
-        if (i + 2 < nchunks) {
-          if (!mbar_wait(&s.freeA[i & 1], (i >> 1) & 1)) { ok = false; break; }
-          bulk_wait_read<0>();
-          loadA(i + 2);
+        if (!ok) {
+          s.dead = 1;
+          atomicOr(p.status, KDA_STATUS_BWD_SCAN_MMA_WAIT);
         }
+        bulk_wait_read<0>();
       }
-      if (!ok) {
-        s.dead = 1;
-        atomicOr(p.status, KDA_STATUS_BWD_SCAN_LOAD_WAIT);
+      __syncwarp();
+    } else if (warp == W_ISSUE + 1) {
+      if (lane == 0) {
+        const int hq = h / p.grp;
+        auto first = [&](int i) { return static_cast<int>(tok_begin + static_cast<long long>(nchunks - 1 - i) * C); };
+        auto tile_of = [&](int i) { return static_cast<size_t>(c0 + nchunks - 1 - i) * p.H + h; };
+        auto loadA = [&](int i) {
+          const int b = i & 1, tok0 = first(i);
+          mbar_expect_tx(&s.fullA[b], 6 * 8192 + VEC_COPY);
+          for (int x = 0; x < 2; ++x) tma_load_rows(s.KQ[b][x], &p.tm_k, 64 * x, hq, tok0, &s.fullA[b]);
+          for (int x = 0; x < 2; ++x) tma_load_rows(s.KQ[b][x] + 8192, &p.tm_q, 64 * x, hq, tok0, &s.fullA[b]);
+          for (int x = 0; x < 2; ++x) tma_load_rows(s.dO[b][x], &p.tm_do, 64 * x, h, tok0, &s.fullA[b]);
+          bulk_g2s(s.vec[b], p.VEC + tile_of(i) * T_VEC, VEC_COPY, &s.fullA[b]);
+        };
+        auto loadB = [&](int i) {
+          mbar_expect_tx(&s.fullB, 2 * 16384);
+          bulk_g2s(s.TP[0], p.TP + tile_of(i) * T_TP, 32768, &s.fullB);
+        };
+        bool ok = true;
+        if (nchunks > 0) {
+          loadA(0);
+          loadB(0);
+          if (nchunks > 1) loadA(1);
+        }
+        for (int i = 0; i < nchunks; ++i) {
+          if (i + 2 < nchunks) bulk_prefetch(p.TP + tile_of(i + 2) * T_TP, 32768);      // into L2
+          if (i + 1 < nchunks) {
+            if (s.dead || !mbar_wait(&s.freeB, i & 1)) { ok = false; break; }
+            loadB(i + 1);
+          }
+          if (s.dead || !mbar_wait(&s.oReady, i & 1)) { ok = false; break; }
+#pragma unroll
+          for (int x = 0; x < 2; ++x) bulk_s2g(p.DF + tile_of(i) * T_VN + x * 8192, s.dO[i & 1][x], 8192);
+          if (tok_end - first(i) >= C) {
+            for (int x = 0; x < 2 && 64 * x < p.vc; ++x) tma_store_rows(&p.tm_dv, 64 * x, h, first(i), s.dV[i & 1][x]);
+          }
+          bulk_commit();
+          if (i + 2 < nchunks) {
+            if (!mbar_wait(&s.freeA[i & 1], (i >> 1) & 1)) { ok = false; break; }
+            bulk_wait_read<0>();
+            loadA(i + 2);
+          }
+        }
+        if (!ok) {
+          s.dead = 1;
+          atomicOr(p.status, KDA_STATUS_BWD_SCAN_LOAD_WAIT);
+        }
+        bulk_wait_read<0>();      // the stores read shared memory that goes with the CTA
       }
-      bulk_wait_read<0>();      // the stores read shared memory that goes with the CTA
+      __syncwarp();
     }
-    __syncwarp();
   }
   __syncthreads();
   if (tid == 0 && s.dead) {      // somebody gave up: loads and products may still be under way
@@ -307,7 +309,7 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_scan_t_kernel(const __grid_co
 int launch_bwd_scan_t(const RScanParams& p, int units, cudaStream_t st) {
   static DeviceOnce once;
   const int smem = static_cast<int>(sizeof(RTSmem)) + 1024;
-  const int rc = once.run([&] { return cudaFuncSetAttribute(delta_bwd_scan_t_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
+  const int rc = once.run([&] { return crew_ready(delta_bwd_scan_t_kernel, smem); });
   if (rc != KDA_OK) return rc;
   return static_cast<int>(launch_chained(delta_bwd_scan_t_kernel, static_cast<unsigned>(units), NT, smem, st, p));
 }

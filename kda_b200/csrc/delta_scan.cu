@@ -349,7 +349,7 @@ static int launch_vc(const ScanParams& p, int units, cudaStream_t st) {
 
 // Few (sequence, head) units leave SMs idle: their value columns are spread over two or four CTAs, which shortens a chunk's products.
 int launch_scan(const ScanParams& p, int units, int slices, cudaStream_t st) {
-  // (32 chunks each, us with 1 | 2 | 4 CTAs per unit: 37 units 116 | 97 | 74, 48 117 | 98 | 139, 74 117 | 99 | 141, 96 119 | 183 | 206)
+  // (32 chunks each, us with 1 | 2 | 4 CTAs per unit: 37 units 112 | 96 | 73, 48 113 | 97 | 137, 74 113 | 98 | 140, 96 114 | 181 | 205)
   if (slices == 0) slices = 4 * units <= sm_count() ? 4 : 2 * units <= sm_count() ? 2 : 1;
   const bool train = p.HS != nullptr;
   if (slices == 4) return train ? launch_vc<32, true>(p, units, st) : launch_vc<32, false>(p, units, st);

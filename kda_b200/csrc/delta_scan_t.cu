@@ -7,8 +7,8 @@
 //   3   (w v_new)^T K             (128 v x 128 keys, K = 64 tokens), added to the state that the registers hold and decay
 // A thread has one value column, 32 keys of its state and 16 tokens of a chunk.  v, o and v_new are turned on the way through shared memory, two bytes a
 // lane: o in q's rows once product 1 has read them, v_new (for a backward) in v's tile.  Tiles and full chunks of o leave by bulk copies.
-// Bound by the chain of a chunk, 3.6 us: the products' 2.3 k cycles and three hand-overs each way.  8 x 4,096 tokens x 32 heads with what a backward needs 504 us
-// (two rounds of units; the bytes alone 365).
+// Bound by the chain of a chunk, 3.5 us: the products' 2.3 k cycles and three hand-overs each way.  8 x 4,096 tokens x 32 heads with what a backward needs 465 us
+// (two rounds of units; the bytes alone 365), with 96 registers for every thread 504.
 #include "delta.cuh"
 
 namespace kda {
@@ -16,7 +16,7 @@ namespace delta {
 
 namespace {
 
-constexpr int CW = 16, NT = (CW + 2) * 32, W_ISSUE = CW;
+constexpr int CW = 16, NT = CREW_THREADS, W_ISSUE = CW;
 
 template <bool TRAIN>
 struct TSmem {
@@ -71,6 +71,7 @@ __global__ void __launch_bounds__(NT, 1) delta_scan_t_kernel(const __grid_consta
   const uint32_t tb = s.tmem_slot, tq = tb + (static_cast<uint32_t>(32 * q4) << 16);
 
   if (warp < CW) {
+    compute_registers();
     // ================= the chain =================
     const int v = 32 * q4 + lane, g = warp >> 2, k0 = 32 * g, t0 = 16 * g;      // value column; first key and first token of this thread
     const size_t sb = (static_cast<size_t>(seq) * p.H + h) * p.kc * p.vc + v;
@@ -103,8 +104,6 @@ __global__ void __launch_bounds__(NT, 1) delta_scan_t_kernel(const __grid_consta
       if (TRAIN || len < C) fence_proxy_async();
       warp_arrive(&s.hReady, lane);
       const float last = vec[V_LAST];
-#pragma unroll
-      for (int e = 0; e < 32; ++e) S[e] *= last;
       // ---- r ----
       const uint32_t at_v = column_at(s.V[i & 1][v >> 6], t0, v & 63), at_o = column_at(s.KQ[i & 1][v >> 6] + 8192, t0, v & 63);
       float r[16], y[16], w[16];
@@ -176,8 +175,8 @@ __global__ void __launch_bounds__(NT, 1) delta_scan_t_kernel(const __grid_consta
       umma::tmem_ld_wait();
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
-        S[j] += r[j];
-        S[16 + j] += y[j];
+        S[j] = fmaf(S[j], last, r[j]);
+        S[16 + j] = fmaf(S[16 + j], last, y[j]);
       }
       umma::fence_before_sync();
     }
@@ -189,109 +188,112 @@ __global__ void __launch_bounds__(NT, 1) delta_scan_t_kernel(const __grid_consta
       for (int e = 0; e < 32; ++e)
         if (k0 + e < p.kc) p.ht[sb + static_cast<size_t>(k0 + e) * p.vc] = S[e];
     }
-  } else if (warp == W_ISSUE) {
-    if (lane == 0) {
-      constexpr uint32_t idK = umma::instr_desc(128, 128, false, false), idM = umma::instr_desc(128, 128, false, true);
-      const uint64_t dT = umma::desc_kmajor(smem_u32(s.TP[0]), 0);
-      bool ok = true;
-      for (int i = 0; i < nchunks && ok; ++i) {
-        const uint32_t aK = smem_u32(s.KQ[i & 1][0]);
-        const uint64_t dK = umma::desc_kmajor(aK, 0), dKm = umma::desc_mnmajor(aK, 0, 16384);
-        if (s.dead || !mbar_wait(&s.fullA[i & 1], (i >> 1) & 1) || !mbar_wait(&s.hReady, i & 1)) { ok = false; break; }
-        umma::fence_after_sync();
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {      // hi and lo with the same rows of B
-          const uint64_t b = dK + (k >> 2) * 1024u + (k & 3) * umma::KSTEP_KMAJOR;
-          umma::mma_ts(tb + D1, tb + AH + 8 * k, b, idK, k > 0);
-          umma::mma_ts(tb + D1, tb + AL + 8 * k, b, idK, 1);
-        }
-        umma::commit(&s.m1);
-        if constexpr (TRAIN) {
-#pragma unroll
-          for (int x = 0; x < 2; ++x) bulk_s2g(p.HS + (static_cast<size_t>(c0 + i) * p.H + h) * T_STATE + x * 16384, s.H[x], 16384);
-          bulk_commit();
-        }
-        if (!mbar_wait(&s.fullB, i & 1) || !mbar_wait(&s.rReady, i & 1)) { ok = false; break; }
-        umma::fence_after_sync();
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint64_t b = dT + k * umma::KSTEP_KMAJOR;
-          umma::mma_ts(tb + D2, tb + RH + 8 * k, b, idK, k > 0);
-          umma::mma_ts(tb + D2, tb + RL + 8 * k, b, idK, 1);
-          umma::mma_ts(tb + D2, tb + RH + 8 * k, b + 1024u, idK, 1);
-        }
-        umma::commit(&s.m2);
-        umma::commit(&s.freeB);
-        if (!mbar_wait(&s.uReady, i & 1)) { ok = false; break; }
-        umma::fence_after_sync();
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint64_t b = dKm + k * umma::KSTEP_MNMAJOR;
-          umma::mma_ts(tb + D3, tb + RH + 8 * k, b, idM, k > 0);
-          umma::mma_ts(tb + D3, tb + RL + 8 * k, b, idM, 1);
-        }
-        if constexpr (TRAIN) bulk_wait_read<0>();      // m3 also says that h's tile may be overwritten
-        umma::commit(&s.m3);
-        umma::commit(&s.freeA[i & 1]);
-      }
-      if (!ok) {
-        s.dead = 1;
-        atomicOr(p.status, KDA_STATUS_SCAN_MMA_WAIT);
-      }
-      if constexpr (TRAIN) bulk_wait_read<0>();
-    }
-    __syncwarp();
   } else {
-    if (lane == 0) {
-      const int hq = h / p.grp;
-      auto first = [&](int i) { return static_cast<int>(tok_begin + static_cast<long long>(i) * C); };
-      auto tile_of = [&](int i) { return static_cast<size_t>(c0 + i) * p.H + h; };
-      auto loadA = [&](int i) {
-        const int b = i & 1, tok0 = first(i);
-        mbar_expect_tx(&s.fullA[b], 6 * 8192 + VEC_COPY);
-        for (int x = 0; x < 2; ++x) tma_load_rows(s.KQ[b][x], &p.tm_k, 64 * x, hq, tok0, &s.fullA[b]);
-        for (int x = 0; x < 2; ++x) tma_load_rows(s.KQ[b][x] + 8192, &p.tm_q, 64 * x, hq, tok0, &s.fullA[b]);
-        for (int x = 0; x < 2; ++x) tma_load_rows(s.V[b][x], &p.tm_v, 64 * x, h, tok0, &s.fullA[b]);
-        bulk_g2s(s.vec[b], p.VEC + tile_of(i) * T_VEC, VEC_COPY, &s.fullA[b]);
-      };
-      auto loadB = [&](int i) {
-        mbar_expect_tx(&s.fullB, 2 * 16384);
-        bulk_g2s(s.TP[0], p.TP + tile_of(i) * T_TP, 32768, &s.fullB);
-      };
-      bool ok = true;
-      if (nchunks > 0) {
-        loadA(0);
-        loadB(0);
-        if (nchunks > 1) loadA(1);
-      }
-      for (int i = 0; i < nchunks; ++i) {
-        if (i + 2 < nchunks) bulk_prefetch(p.TP + tile_of(i + 2) * T_TP, 32768);      // into L2
-        if (i + 1 < nchunks) {
-          if (s.dead || !mbar_wait(&s.freeB, i & 1)) { ok = false; break; }
-          loadB(i + 1);
-        }
-        if (s.dead || !mbar_wait(&s.oReady, i & 1)) { ok = false; break; }
-        if constexpr (TRAIN) {                 // v_new stands in v's tile
+    helper_registers();
+    if (warp == W_ISSUE) {
+      if (lane == 0) {
+        constexpr uint32_t idK = umma::instr_desc(128, 128, false, false), idM = umma::instr_desc(128, 128, false, true);
+        const uint64_t dT = umma::desc_kmajor(smem_u32(s.TP[0]), 0);
+        bool ok = true;
+        for (int i = 0; i < nchunks && ok; ++i) {
+          const uint32_t aK = smem_u32(s.KQ[i & 1][0]);
+          const uint64_t dK = umma::desc_kmajor(aK, 0), dKm = umma::desc_mnmajor(aK, 0, 16384);
+          if (s.dead || !mbar_wait(&s.fullA[i & 1], (i >> 1) & 1) || !mbar_wait(&s.hReady, i & 1)) { ok = false; break; }
+          umma::fence_after_sync();
 #pragma unroll
-          for (int x = 0; x < 2; ++x) bulk_s2g(p.VN + tile_of(i) * T_VN + x * 8192, s.V[i & 1][x], 8192);
+          for (int k = 0; k < 8; ++k) {      // hi and lo with the same rows of B
+            const uint64_t b = dK + (k >> 2) * 1024u + (k & 3) * umma::KSTEP_KMAJOR;
+            umma::mma_ts(tb + D1, tb + AH + 8 * k, b, idK, k > 0);
+            umma::mma_ts(tb + D1, tb + AL + 8 * k, b, idK, 1);
+          }
+          umma::commit(&s.m1);
+          if constexpr (TRAIN) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x) bulk_s2g(p.HS + (static_cast<size_t>(c0 + i) * p.H + h) * T_STATE + x * 16384, s.H[x], 16384);
+            bulk_commit();
+          }
+          if (!mbar_wait(&s.fullB, i & 1) || !mbar_wait(&s.rReady, i & 1)) { ok = false; break; }
+          umma::fence_after_sync();
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint64_t b = dT + k * umma::KSTEP_KMAJOR;
+            umma::mma_ts(tb + D2, tb + RH + 8 * k, b, idK, k > 0);
+            umma::mma_ts(tb + D2, tb + RL + 8 * k, b, idK, 1);
+            umma::mma_ts(tb + D2, tb + RH + 8 * k, b + 1024u, idK, 1);
+          }
+          umma::commit(&s.m2);
+          umma::commit(&s.freeB);
+          if (!mbar_wait(&s.uReady, i & 1)) { ok = false; break; }
+          umma::fence_after_sync();
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint64_t b = dKm + k * umma::KSTEP_MNMAJOR;
+            umma::mma_ts(tb + D3, tb + RH + 8 * k, b, idM, k > 0);
+            umma::mma_ts(tb + D3, tb + RL + 8 * k, b, idM, 1);
+          }
+          if constexpr (TRAIN) bulk_wait_read<0>();      // m3 also says that h's tile may be overwritten
+          umma::commit(&s.m3);
+          umma::commit(&s.freeA[i & 1]);
         }
-        if (tok_end - first(i) >= C) {         // o in q's rows
-          for (int x = 0; x < 2 && 64 * x < p.vc; ++x) tma_store_rows(&p.tm_o, 64 * x, h, first(i), s.KQ[i & 1][x] + 8192);
+        if (!ok) {
+          s.dead = 1;
+          atomicOr(p.status, KDA_STATUS_SCAN_MMA_WAIT);
         }
-        bulk_commit();
-        if (i + 2 < nchunks) {
-          if (!mbar_wait(&s.freeA[i & 1], (i >> 1) & 1)) { ok = false; break; }
-          bulk_wait_read<0>();
-          loadA(i + 2);
-        }
+        if constexpr (TRAIN) bulk_wait_read<0>();
       }
-      if (!ok) {
-        s.dead = 1;
-        atomicOr(p.status, KDA_STATUS_SCAN_LOAD_WAIT);
+      __syncwarp();
+    } else if (warp == W_ISSUE + 1) {
+      if (lane == 0) {
+        const int hq = h / p.grp;
+        auto first = [&](int i) { return static_cast<int>(tok_begin + static_cast<long long>(i) * C); };
+        auto tile_of = [&](int i) { return static_cast<size_t>(c0 + i) * p.H + h; };
+        auto loadA = [&](int i) {
+          const int b = i & 1, tok0 = first(i);
+          mbar_expect_tx(&s.fullA[b], 6 * 8192 + VEC_COPY);
+          for (int x = 0; x < 2; ++x) tma_load_rows(s.KQ[b][x], &p.tm_k, 64 * x, hq, tok0, &s.fullA[b]);
+          for (int x = 0; x < 2; ++x) tma_load_rows(s.KQ[b][x] + 8192, &p.tm_q, 64 * x, hq, tok0, &s.fullA[b]);
+          for (int x = 0; x < 2; ++x) tma_load_rows(s.V[b][x], &p.tm_v, 64 * x, h, tok0, &s.fullA[b]);
+          bulk_g2s(s.vec[b], p.VEC + tile_of(i) * T_VEC, VEC_COPY, &s.fullA[b]);
+        };
+        auto loadB = [&](int i) {
+          mbar_expect_tx(&s.fullB, 2 * 16384);
+          bulk_g2s(s.TP[0], p.TP + tile_of(i) * T_TP, 32768, &s.fullB);
+        };
+        bool ok = true;
+        if (nchunks > 0) {
+          loadA(0);
+          loadB(0);
+          if (nchunks > 1) loadA(1);
+        }
+        for (int i = 0; i < nchunks; ++i) {
+          if (i + 2 < nchunks) bulk_prefetch(p.TP + tile_of(i + 2) * T_TP, 32768);      // into L2
+          if (i + 1 < nchunks) {
+            if (s.dead || !mbar_wait(&s.freeB, i & 1)) { ok = false; break; }
+            loadB(i + 1);
+          }
+          if (s.dead || !mbar_wait(&s.oReady, i & 1)) { ok = false; break; }
+          if constexpr (TRAIN) {                 // v_new stands in v's tile
+#pragma unroll
+            for (int x = 0; x < 2; ++x) bulk_s2g(p.VN + tile_of(i) * T_VN + x * 8192, s.V[i & 1][x], 8192);
+          }
+          if (tok_end - first(i) >= C) {         // o in q's rows
+            for (int x = 0; x < 2 && 64 * x < p.vc; ++x) tma_store_rows(&p.tm_o, 64 * x, h, first(i), s.KQ[i & 1][x] + 8192);
+          }
+          bulk_commit();
+          if (i + 2 < nchunks) {
+            if (!mbar_wait(&s.freeA[i & 1], (i >> 1) & 1)) { ok = false; break; }
+            bulk_wait_read<0>();
+            loadA(i + 2);
+          }
+        }
+        if (!ok) {
+          s.dead = 1;
+          atomicOr(p.status, KDA_STATUS_SCAN_LOAD_WAIT);
+        }
+        bulk_wait_read<0>();      // the stores read shared memory that goes with the CTA
       }
-      bulk_wait_read<0>();      // the stores read shared memory that goes with the CTA
+      __syncwarp();
     }
-    __syncwarp();
   }
   __syncthreads();
   if (tid == 0 && s.dead) {      // somebody gave up: loads and products may still be under way
@@ -307,7 +309,7 @@ template <bool TRAIN>
 static int launch(const ScanParams& p, int units, cudaStream_t st) {
   static DeviceOnce once;
   const int smem = static_cast<int>(sizeof(TSmem<TRAIN>)) + 1024;
-  const int rc = once.run([&] { return cudaFuncSetAttribute(delta_scan_t_kernel<TRAIN>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
+  const int rc = once.run([&] { return crew_ready(delta_scan_t_kernel<TRAIN>, smem); });
   if (rc != KDA_OK) return rc;
   return static_cast<int>(launch_chained(delta_scan_t_kernel<TRAIN>, static_cast<unsigned>(units), NT, smem, st, p));
 }

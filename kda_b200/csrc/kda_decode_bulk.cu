@@ -173,7 +173,8 @@ __global__ void __launch_bounds__(HV * 2 + 32, 128 / HV) kda_decode_bulk_kernel(
         long long recent[4] = {-1, -1, -1, -1};
         for (int c = 0; c < nst; ++c) {
           const int b = (c & 1) ? y : x;
-          const long long sl = slotted ? static_cast<long long>(a.state_indices[static_cast<size_t>(cur.n) * a.state_indices_stride + c]) : cur.n;
+          const bool named = !HEAD || !slotted || c < a.columns;
+          const long long sl = !slotted ? cur.n : named ? static_cast<long long>(a.state_indices[static_cast<size_t>(cur.n) * a.state_indices_stride + c]) : -1;
           const bool skip = HEAD && slotted && (pad[0] || !a.holds(sl));
           const long long st = skip ? -1 : sl * a.H + cur.h;
           if (HV != DV && !skip && (st == recent[0] || st == recent[1] || st == recent[2] || st == recent[3])) bulk_wait<0>();

@@ -205,6 +205,27 @@ def test_accepted_counts_outside_the_table(N, HV):
     assert rel_l2_err(o[2:], ref) <= tol(BF) and rel_l2_err(pool[slots[2:].long().flatten()].view(S.shape), S) <= STATE
 
 
+@pytest.mark.parametrize("N,HV", [(2, 3), (40, 8)])
+def test_fewer_columns_than_tokens(N, HV):
+    """Through the C entry: a table of one column for two tokens keeps the first token's state only."""
+    import ctypes as C
+    from kda_b200 import _lib
+    lib = _lib.load()
+    x = make(N, 2, HV, HV, 128, 128, 21)
+    wide, slim = states(2 * N, HV, 128, 128), states(2 * N, HV, 128, 128)
+    before = wide.clone()
+    table = torch.arange(2 * N, dtype=torch.int32).view(N, 2).cuda()
+    ref = run_pool(x, wide, table, scale=0.1)
+    first, o = table[:, 0].contiguous(), torch.empty_like(ref)
+    a = _lib.RecurrentArgs(q=x["q"].data_ptr(), k=x["k"].data_ptr(), v=x["v"].data_ptr(), g=x["g"].data_ptr(), beta=x["beta"].data_ptr(), h0=slim.data_ptr(), ht=slim.data_ptr(),
+                           o=o.data_ptr(), state_indices=first.data_ptr(), state_indices_stride=1, tokens=2 * N, N=N, T=2, H=HV, K=128, V=128, HQ=HV, io_dtype=_lib.KDA_BF16,
+                           g_raw_dtype=_lib.KDA_FP32, beta_raw_dtype=_lib.KDA_FP32, scale=0.1)
+    assert lib.kda_delta_recurrent_fwd(C.byref(a), 2 * N, 1, C.c_void_p(torch.cuda.current_stream().cuda_stream)) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(o, ref) and torch.equal(slim[first.long()], wide[first.long()])
+    assert torch.equal(slim[table[:, 1].long()], before[table[:, 1].long()])
+
+
 @pytest.mark.parametrize("which", few_and_many())
 def test_the_same_bits_alone_and_in_a_batch(which):
     """A sequence's result does not depend on its neighbours, NaN among them."""

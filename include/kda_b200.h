@@ -366,7 +366,7 @@ int kda_gate_bwd(const kda_gate_args* args, void* stream);
  * kda_delta_chunk_fwd / _bwd: whole sequences in chunks of 64 tokens on the tensor cores, bf16 q, k, v, o.  States, their gradients and every sum are
  * fp32, and operands that are not inputs are bf16 pairs in the two walks over a sequence: final states and dh0 carry about 1e-5 of their norm.  Rules as
  * for kda_chunk_fwd / _bwd: the workspace of a forward with save_for_backward goes to the backward untouched; kda_chunk_status reads its status word.
- * Rows in front of the first sequence of cu_seqlens and behind the last one are zero in o and in the gradients.
+ * Rows in front of the first sequence of cu_seqlens and behind the last one are zero in o and in the gradients; with N = 0 all rows are.
  * ------------------------------------------------------------------------------------------------ */
 typedef struct kda_delta_args {
   const void* q;               /* [tokens, HQ, K] bf16 */

@@ -13,7 +13,8 @@ static int validate(const kda_delta_args& a, bool backward) {
   if ((a.g_dtype != KDA_BF16 && a.g_dtype != KDA_FP32) || (a.beta_dtype != KDA_BF16 && a.beta_dtype != KDA_FP32)) return KDA_E_DTYPE;
   if (a.tokens > 0x7fffffffLL - 64) return KDA_E_SHAPE;                                          // tile coordinates are 32 bits
   if ((a.tokens / C + a.N) * a.H > 0x7fff0000LL || static_cast<int64_t>(a.N) * a.H * 4 > 0x7fffffffLL) return KDA_E_SHAPE;      // so are grids
-  if (a.tokens == 0 || a.N == 0) return KDA_OK;
+  if (a.tokens == 0) return KDA_OK;
+  if (a.N == 0) return backward ? (!a.dq || !a.dk || !a.dv || !a.dg || !a.dbeta ? KDA_E_NULL : KDA_OK) : (!a.o ? KDA_E_NULL : KDA_OK);      // only written: zeros
   if (!a.q || !a.k || !a.v || !a.g || !a.beta || !a.workspace || (!backward && !a.o)) return KDA_E_NULL;
   if (!a.cu_seqlens && a.tokens % a.N != 0) return KDA_E_SHAPE;
   auto addr = [](const void* p) { return reinterpret_cast<uintptr_t>(p); };
@@ -49,6 +50,14 @@ __global__ void __launch_bounds__(256) delta_tail_kernel(const TailParams p) {
     for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<long long>(gridDim.x) * 256)
       static_cast<unsigned short*>(p.out[o])[i < front ? i : b * per + (i - front)] = 0;
   }
+}
+// the same where there is no sequence at all: every row
+static int clear_rows_of(const TailParams& p, cudaStream_t st) {
+  for (int o = 0; o < p.outs; ++o) {
+    const cudaError_t e = cudaMemsetAsync(p.out[o], 0, static_cast<size_t>(p.bytes[o]) * static_cast<size_t>(p.tokens), st);
+    if (e != cudaSuccess) return static_cast<int>(e);
+  }
+  return KDA_OK;
 }
 static int launch_tail(const TailParams& p, cudaStream_t st) { return static_cast<int>(launch_chained(delta_tail_kernel, static_cast<unsigned>(sm_count()), 256, 0, st, p)); }
 
@@ -95,7 +104,8 @@ extern "C" int kda_delta_chunk_fwd(const kda_delta_args* args, void* stream) {
   int rc = validate(a, false);
   if (rc != KDA_OK) return rc;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (a.N == 0) return KDA_OK;
+  const TailParams tail{a.cu_seqlens, a.N, 1, a.tokens, {a.o}, {2LL * a.H * a.V}};
+  if (a.N == 0) return a.tokens > 0 ? clear_rows_of(tail, st) : KDA_OK;
   if (a.tokens == 0) {
     if (!a.ht || a.ht == a.h0) return KDA_OK;
     const size_t n = static_cast<size_t>(a.N) * a.H * a.K * a.V * sizeof(float);
@@ -129,10 +139,7 @@ extern "C" int kda_delta_chunk_fwd(const kda_delta_args* args, void* stream) {
   sp.map = map; sp.TP = w.TP; sp.VEC = w.VEC; sp.HS = a.save_for_backward ? w.HS : nullptr; sp.VN = a.save_for_backward ? w.VN : nullptr;
   sp.h0 = a.h0; sp.ht = a.ht; sp.o = static_cast<__nv_bfloat16*>(a.o); sp.status = w.status; sp.H = a.H; sp.grp = pp.grp; sp.kc = a.K; sp.vc = a.V;
   if ((rc = delta::launch_scan(sp, a.N * a.H, a.scan_slices, st)) != KDA_OK) return rc;
-  if (a.cu_seqlens) {
-    const TailParams tp{a.cu_seqlens, a.N, 1, a.tokens, {a.o}, {2LL * a.H * a.V}};
-    if ((rc = launch_tail(tp, st)) != KDA_OK) return rc;
-  }
+  if (a.cu_seqlens && (rc = launch_tail(tail, st)) != KDA_OK) return rc;
   prof_mark(prof, KDA_STAGE_SCAN, st);
   return KDA_OK;
 }
@@ -145,13 +152,15 @@ extern "C" int kda_delta_chunk_bwd(const kda_delta_args* args, void* stream) {
   int rc = validate(a, true);
   if (rc != KDA_OK) return rc;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (a.N == 0) return KDA_OK;
+  const int HQ = a.HQ > 0 ? a.HQ : a.H, grp = a.H / HQ, most = static_cast<int>(a.tokens / C + a.N);
+  const long long gb = a.g_dtype == KDA_BF16 ? 2 : 4, bb = a.beta_dtype == KDA_BF16 ? 2 : 4;
+  const TailParams tail{a.cu_seqlens, a.N, 5, a.tokens, {a.dq, a.dk, a.dv, a.dg, a.dbeta}, {2LL * HQ * a.K, 2LL * HQ * a.K, 2LL * a.H * a.V, gb * a.H, bb * a.H}};
+  if (a.N == 0) return a.tokens > 0 ? clear_rows_of(tail, st) : KDA_OK;
   if (a.tokens == 0) {
     if (!a.dh0 || a.dh0 == a.d_ht) return KDA_OK;
     const size_t n = static_cast<size_t>(a.N) * a.H * a.K * a.V * sizeof(float);
     return static_cast<int>(a.d_ht ? cudaMemcpyAsync(a.dh0, a.d_ht, n, cudaMemcpyDeviceToDevice, st) : cudaMemsetAsync(a.dh0, 0, n, st));
   }
-  const int HQ = a.HQ > 0 ? a.HQ : a.H, grp = a.H / HQ, most = static_cast<int>(a.tokens / C + a.N);
   const Ws w = carve(static_cast<unsigned char*>(a.workspace), static_cast<unsigned char*>(a.bwd_workspace), a.tokens, a.N, a.H, a.K, true, grp > 1);
   if (a.workspace_bytes < w.fwd_bytes || a.bwd_workspace_bytes < w.bwd_bytes) return KDA_E_WORKSPACE;
   ChunkWs cw{};
@@ -185,11 +194,7 @@ extern "C" int kda_delta_chunk_bwd(const kda_delta_args* args, void* stream) {
                                          static_cast<__nv_bfloat16*>(a.dk), pieces, per_row, grp));
     if (rc != KDA_OK) return rc;
   }
-  if (a.cu_seqlens) {
-    const long long gb = a.g_dtype == KDA_BF16 ? 2 : 4, bb = a.beta_dtype == KDA_BF16 ? 2 : 4;
-    const TailParams tp{a.cu_seqlens, a.N, 5, a.tokens, {a.dq, a.dk, a.dv, a.dg, a.dbeta}, {2LL * HQ * a.K, 2LL * HQ * a.K, 2LL * a.H * a.V, gb * a.H, bb * a.H}};
-    if ((rc = launch_tail(tp, st)) != KDA_OK) return rc;
-  }
+  if (a.cu_seqlens && (rc = launch_tail(tail, st)) != KDA_OK) return rc;
   prof_mark(prof, KDA_STAGE_BWD_MAIN, st);
   return KDA_OK;
 }

@@ -361,7 +361,8 @@ int kda_gate_bwd(const kda_gate_args* args, void* stream);
  * [tokens, H] of g_raw_dtype and `beta` to [tokens, H] of beta_raw_dtype, whether A_log and beta_sigmoid are given or not; dt_bias is [H].
  * slots, slot_columns: with state_indices, the states in the pool h0 and the columns of the table.  A sequence whose starting slot lies outside the pool (a
  * padded entry of a batch), or whose accepted count names no column, has zeros for its rows of o and touches no state; the state behind a token whose slot
- * lies outside is not kept.  Two sequences must not name the same slot.
+ * lies outside is not kept.  Two sequences must not name the same slot.  Rows of o in front of the first sequence of cu_seqlens and behind the last one become
+ * zeros; with N = 0 all rows do.
  *
  * kda_delta_chunk_fwd / _bwd: whole sequences in chunks of 64 tokens on the tensor cores, bf16 q, k, v, o.  States, their gradients and every sum are
  * fp32, and operands that are not inputs are bf16 pairs in the two walks over a sequence: final states and dh0 carry about 1e-5 of their norm.  Rules as

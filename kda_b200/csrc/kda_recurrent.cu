@@ -86,6 +86,15 @@ struct RowBits {
   }
 };
 
+// One decay per head, packed: rows of o in front of the first sequence and behind the last one become zeros, by the warps of these sequences.
+// (bos, eos: of sequence n, inside the call's tokens if cu_seqlens is in order; otherwise the rows are cut to them.)
+template <class Z>
+__device__ __forceinline__ void rows_of_none(const HeadArgs& a, int n, long long bos, long long eos, Z&& zeros) {
+  if (!a.cu_seqlens) return;
+  if (n == 0) zeros(0, bos < a.tokens ? bos : a.tokens);
+  if (n == a.N - 1) zeros(eos > 0 ? eos : 0, a.tokens);
+}
+
 // A token's vectors are fetched while the token before is worked on: with one warp per slice there is nobody else to hide
 // their latency (one sequence of four draft tokens: 14.2 us when each token fetched its own, 8.0 us so).
 // HEAD: one decay per token and head (kda_delta_recurrent_fwd).
@@ -146,9 +155,13 @@ __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_kernel(const Rec
   const int32_t* slots = a.state_indices ? a.state_indices + static_cast<size_t>(n) * a.state_indices_stride : nullptr;
   long long slot = n;
   if constexpr (HEAD) {
-    if (slots && !a.holds(slot = a.start_slot(n))) {
+    auto zeros = [&](long long from, long long to) {
       if (rg == 0)
-        for (long long t = bos; t < eos; ++t) IoTraits<IO>::st4(static_cast<IO*>(a.o) + (static_cast<size_t>(t) * a.H + h) * a.V + col, make_float4(0.f, 0.f, 0.f, 0.f));
+        for (long long t = from; t < to; ++t) IoTraits<IO>::st4(static_cast<IO*>(a.o) + (static_cast<size_t>(t) * a.H + h) * a.V + col, make_float4(0.f, 0.f, 0.f, 0.f));
+    };
+    rows_of_none(a, n, bos, eos, zeros);
+    if (slots && !a.holds(slot = a.start_slot(n))) {
+      zeros(bos, eos);
       return;
     }
   } else if (slots) {
@@ -311,8 +324,12 @@ __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_t_kernel(const R
   const int32_t* slots = a.state_indices ? a.state_indices + static_cast<size_t>(n) * a.state_indices_stride : nullptr;
   long long slot = n;
   if constexpr (HEAD) {
+    auto zeros = [&](long long from, long long to) {
+      for (long long t = from; t < to; ++t) static_cast<IO*>(a.o)[(static_cast<size_t>(t) * a.H + h) * a.V + vs * 32 + lane] = IO(0.f);
+    };
+    rows_of_none(a, n, bos, eos, zeros);
     if (slots && !a.holds(slot = a.start_slot(n))) {
-      for (long long t = bos; t < eos; ++t) static_cast<IO*>(a.o)[(static_cast<size_t>(t) * a.H + h) * a.V + vs * 32 + lane] = IO(0.f);
+      zeros(bos, eos);
       return;
     }
   } else if (slots) {
@@ -467,6 +484,10 @@ static int recurrent_fwd(const kda_recurrent_args* args, bool per_head, int32_t 
       cudaError_t e = a.h0 ? cudaMemcpyAsync(a.ht, a.h0, bytes, cudaMemcpyDeviceToDevice, static_cast<cudaStream_t>(stream))
                            : cudaMemsetAsync(a.ht, 0, bytes, static_cast<cudaStream_t>(stream));
       return static_cast<int>(e);
+    }
+    if (per_head && a.N == 0 && a.tokens > 0) {      // rows of no sequence
+      if (!a.o) return KDA_E_NULL;
+      return static_cast<int>(cudaMemsetAsync(a.o, 0, static_cast<size_t>(a.tokens) * a.H * a.V * (a.io_dtype == KDA_BF16 ? 2 : 4), static_cast<cudaStream_t>(stream)));
     }
     return KDA_OK;
   }

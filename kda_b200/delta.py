@@ -27,7 +27,8 @@ def fused_recurrent_gated_delta_fwd(q, k, v, g, beta, A_log=None, dt_bias=None, 
     With `inplace_final_state` states are written over `initial_state`, a float32 [slots, HV, K, V] pool where `ssm_state_indices` [N] or [N, T] names the slot of
     every token: a sequence starts from the slot of its first token (with `num_accepted_tokens` [N] of its last accepted one) and the state behind token t lands
     in that token's slot.  Slots are read as 32-bit numbers; no two sequences may name the same one.  A sequence whose starting slot lies outside the pool (-1: a padded entry) or whose accepted count
-    names no column gets zeros for its rows of o and touches no state; a later token's slot outside the pool is left out.  Returns (o, states)."""
+    names no column gets zeros for its rows of o and touches no state; a later token's slot outside the pool is left out.  With cu_seqlens, rows of o (of `out` too) in
+    front of the first sequence and behind the last one become zeros.  Returns (o, states)."""
     return _native().delta_recurrent_fwd(
         q, k, v, g, beta, A_log, dt_bias, initial_state, scale, output_final_state, inplace_final_state, cu_seqlens, ssm_state_indices, num_accepted_tokens,
         use_qk_l2norm_in_kernel, use_gate_in_kernel, use_beta_sigmoid_in_kernel, lower_bound, out, transpose_state_layout)
@@ -46,6 +47,17 @@ def fused_recurrent_gated_delta(q, k, v, g, beta, A_log=None, dt_bias=None, scal
         use_beta_sigmoid_in_kernel=use_beta_sigmoid_in_kernel, lower_bound=lower_bound, transpose_state_layout=transpose_state_layout)
 
 
+def _float32_packed(q, k, v, g, beta, cu_seqlens, call):
+    """A packed float32 call with gradients.  The kernels behind chunk_kda leave rows of no sequence unwritten; here these rows are cut off on the way in and on the
+    way out, so that they are zero in o and in the gradients."""
+    cu = cu_seqlens.to(q.device)
+    row = torch.arange(q.shape[1], device=q.device)
+    inside = (row >= cu[0]) & (row < cu[-1])
+    cut = lambda t: torch.where(inside.view(1, -1, *[1] * (t.dim() - 2)), t, 0)      # noqa: E731
+    o, ht = call(*(cut(t) for t in (q, k, v, g, beta)), cu)
+    return cut(o), ht
+
+
 @torch.compiler.disable
 def chunk_gated_delta(q, k, v, g, beta, scale=None, initial_state=None, output_final_state=False, use_qk_l2norm_in_kernel=False, cu_seqlens=None,
                       transpose_state_layout=False):
@@ -53,7 +65,8 @@ def chunk_gated_delta(q, k, v, g, beta, scale=None, initial_state=None, output_f
 
     q, k [B,T,H,K]; v [B,T,HV,V]; g [B,T,HV] log-space decay (<= 0; -inf forgets the state) and beta [B,T,HV], in bfloat16 or float32; initial_state [N,HV,K,V]
     float32; cu_seqlens [N+1] with B == 1.  HV is a multiple of H (value head h reads q/k head h // (HV // H)).  Returns (o, final_state or None), differentiable
-    with respect to q, k, v, g, beta and initial_state; gradients come in the types of their tensors.  `transpose_state_layout`: states are [.., V, K].
+    with respect to q, k, v, g, beta and initial_state; gradients come in the types of their tensors.  Rows in front of the first sequence of cu_seqlens and behind
+    the last one are zero, in o and in the gradients.  `transpose_state_layout`: states are [.., V, K].
 
     bfloat16 with K, V up to 128 takes the chunked tensor-core kernels (columns in multiples of 8 as they are, others zero-padded); final states and dh0 carry about
     1e-5 of their norm, which single bfloat16 operands would not give.  bfloat16 with K = 256 runs forward only, token by token.  float32 runs token by
@@ -66,8 +79,10 @@ def chunk_gated_delta(q, k, v, g, beta, scale=None, initial_state=None, output_f
         scale = K ** -0.5
     grads = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, g, beta, initial_state))
     if q.dtype == torch.float32 and grads:
-        return ops.chunk_kda(q, k, v, g.unsqueeze(-1).expand(*g.shape, K), beta, scale=scale, initial_state=initial_state, output_final_state=output_final_state,
-                             use_qk_l2norm_in_kernel=use_qk_l2norm_in_kernel, cu_seqlens=cu_seqlens, transpose_state_layout=transpose_state_layout)
+        def per_channel(q, k, v, g, beta, cu):
+            return ops.chunk_kda(q, k, v, g.unsqueeze(-1).expand(*g.shape, K), beta, scale=scale, initial_state=initial_state, output_final_state=output_final_state,
+                                 use_qk_l2norm_in_kernel=use_qk_l2norm_in_kernel, cu_seqlens=cu, transpose_state_layout=transpose_state_layout)
+        return per_channel(q, k, v, g, beta, None) if cu_seqlens is None else _float32_packed(q, k, v, g, beta, cu_seqlens, per_channel)
     if q.dtype == torch.float32 or K > 128 or V > 128:
         if grads or (q.dtype != torch.float32 and K != 256):
             raise NotImplementedError(f"kda_b200: the bf16 chunked kernels are built for head sizes up to 128, got K={K}, V={V} (K = 256 runs forward-only)")

@@ -17,3 +17,9 @@ def test_forward_without_sequences(lib, missing):      # noqa: F811
 def test_backward_without_sequences(lib, missing):      # noqa: F811
     assert lib.kda_delta_chunk_bwd(C.byref(delta_args(N=0, **{missing: 0})), None) == -1
     assert lib.kda_delta_chunk_bwd(C.byref(delta_args(N=0, tokens=0, **{missing: 0})), None) == 0
+
+
+def test_decode_without_sequences(lib):      # noqa: F811
+    from kda_b200 import _lib
+    call = lambda **kw: lib.kda_delta_recurrent_fwd(C.byref(_lib.RecurrentArgs(**{**dict(N=0, T=4, tokens=4, H=2, K=64, V=64, io_dtype=_lib.KDA_BF16, cu_seqlens=512), **kw})), 0, 0, None)      # noqa: E731
+    assert call(o=0) == -1 and call(tokens=0) == 0

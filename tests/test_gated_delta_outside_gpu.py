@@ -6,8 +6,8 @@ import torch
 from test_gated_delta_gpu import leave_no_memory, make, run      # noqa: F401  (the fixture)
 
 pytestmark = pytest.mark.gpu
-BF = torch.bfloat16
-PATHS = [(128, 128, BF), (64, 64, BF), (20, 37, BF)]
+BF, F32 = torch.bfloat16, torch.float32
+PATHS = [(128, 128, BF), (64, 64, BF), (20, 37, BF), (64, 64, F32), (128, 32, F32)]
 
 
 def poison():
@@ -44,3 +44,29 @@ def test_in_front_and_behind(K, V, dtype, grads):
         assert (got[n][:, 10:170] != 0).any() and torch.isfinite(got[n].float()).all(), n
         if dtype == BF:
             assert torch.equal(got[n][:, 10:60], one[n]), n
+
+
+@pytest.mark.parametrize("K,V,dtype,tr", [(64, 64, BF, False), (128, 128, BF, True), (256, 32, BF, False), (32, 96, F32, False), (64, 32, F32, True)])
+@pytest.mark.parametrize("cu", [[10, 60, 170], [0, 0, 170], [200, 200], [0], [0, 200]])
+def test_token_by_token(K, V, dtype, tr, cu):
+    from kda_b200 import fused_recurrent_gated_delta
+    d = {n: t.cuda() for n, t in make(1, 200, 2, 4, K, V, seed=3, h0=False, dtype=dtype).items() if t is not None}
+    poison()
+    o, _ = fused_recurrent_gated_delta(d["q"], d["k"], d["v"], d["g"], d["beta"], cu_seqlens=torch.tensor(cu, dtype=torch.int32, device="cuda"), transpose_state_layout=tr)
+    assert not o[:, :cu[0]].any() and not o[:, cu[-1]:].any() and (o[:, cu[0]:cu[-1]].any() or cu[0] == cu[-1])
+
+
+def test_a_servers_padded_output():
+    """Decode into a caller's buffer, packed: the rows behind the last sequence become zero too, and a call without one zeroes all."""
+    from kda_b200 import fused_recurrent_gated_delta_fwd
+    d = {n: t.cuda() for n, t in make(1, 12, 2, 2, 128, 128, seed=4, h0=False).items() if t is not None}
+    pool = torch.randn(9, 2, 128, 128, device="cuda")
+    args = [d[n] for n in ("q", "k", "v", "g", "beta")]
+    slots = torch.arange(8, dtype=torch.int32, device="cuda").view(2, 4)
+    out = torch.full_like(d["v"], float("nan"))
+    fused_recurrent_gated_delta_fwd(*args, initial_state=pool, cu_seqlens=torch.tensor([0, 3, 7], dtype=torch.int32, device="cuda"), ssm_state_indices=slots, out=out)
+    assert out[:, :7].isfinite().all() and out[:, :7].any() and not out[:, 7:].any()
+    before = pool.clone()
+    out = torch.full_like(d["v"], float("nan"))
+    fused_recurrent_gated_delta_fwd(*args, initial_state=pool, cu_seqlens=torch.zeros(1, dtype=torch.int32, device="cuda"), ssm_state_indices=slots[:0], out=out)
+    assert not out.any() and torch.equal(pool, before)

@@ -48,9 +48,9 @@ def fused_recurrent_gated_delta(q, k, v, g, beta, A_log=None, dt_bias=None, scal
 
 
 def _float32_packed(q, k, v, g, beta, cu_seqlens, call):
-    """A packed float32 call with gradients.  The kernels behind chunk_kda leave rows of no sequence unwritten; here these rows are cut off on the way in and on the
-    way out, so that they are zero in o and in the gradients."""
-    cu = cu_seqlens.to(q.device)
+    """A packed float32 call with gradients.  The kernels behind chunk_kda take the offsets as they are and leave rows of no sequence unwritten; here offsets stay
+    inside the tensors, and these rows are cut off on the way in and on the way out, so that they are zero in o and in the gradients."""
+    cu = cu_seqlens.to(q.device).clamp(0, q.shape[1]).cummax(0).values
     row = torch.arange(q.shape[1], device=q.device)
     inside = (row >= cu[0]) & (row < cu[-1])
     cut = lambda t: torch.where(inside.view(1, -1, *[1] * (t.dim() - 2)), t, 0)      # noqa: E731

@@ -70,3 +70,17 @@ def test_a_servers_padded_output():
     out = torch.full_like(d["v"], float("nan"))
     fused_recurrent_gated_delta_fwd(*args, initial_state=pool, cu_seqlens=torch.zeros(1, dtype=torch.int32, device="cuda"), ssm_state_indices=slots[:0], out=out)
     assert not out.any() and torch.equal(pool, before)
+
+
+@pytest.mark.parametrize("cu", [[0, 400], [-64, 70], [50, 20, 70], [90, 100]])
+def test_float32_offsets_beyond_the_tensors(cu):
+    """Training in float32 with offsets that do not fit: they are cut to the tensors, and rows outside come out as zeros."""
+    from kda_b200 import chunk_gated_delta
+    d = make(1, 70, 2, 2, 64, 64, seed=5, h0=False, dtype=F32)
+    x = {n: d[n].cuda().requires_grad_() for n in ("q", "k", "v", "g", "beta")}
+    o, _ = chunk_gated_delta(*x.values(), cu_seqlens=torch.tensor(cu, device="cuda"))
+    grads = torch.autograd.grad(o, list(x.values()), torch.ones_like(o))
+    inside = torch.zeros(70, dtype=torch.bool)
+    inside[max(0, cu[0]):max(0, *cu)] = True
+    for t in (o, *grads):
+        assert torch.isfinite(t).all() and not t[:, ~inside.cuda()].any()

@@ -95,13 +95,13 @@ bool chunk_delta(DeltaCall& c, Tensor& o, Tensor& ht) {
   const Sizes s = check_common(c.q, c.k, c.v, c.g, c.beta, c.h0, c.cu, true);
   const at::Device dev = c.q.device();
   require_device(dev, {{"k", &c.k}, {"v", &c.v}, {"g", &c.g}, {"beta", &c.beta}, {"initial_state", &c.h0}});
+  KDA_REQUIRE(!has_tangent({&c.q, &c.k, &c.v, &c.g, &c.beta, &c.h0}), PyExc_NotImplementedError, "kda_b200: chunk_gated_delta has no forward-mode derivative (jvp)");
   const int64_t N = c.cu.defined() ? c.cu.numel() - 1 : s.B;
   const int64_t rows = c.transposed ? s.V : s.K, cols = c.transposed ? s.K : s.V;
   KDA_REQUIRE(!c.cu.defined() || (c.cu.dim() == 1 && c.cu.numel() >= 1), PyExc_ValueError, "cu_seqlens must be [N + 1], got ", c.cu.sizes());
   KDA_REQUIRE(!c.h0.defined() || (c.h0.sizes() == at::IntArrayRef{N, s.H, rows, cols}), PyExc_ValueError, "initial_state must have shape [", N, ", ", s.H, ", ", rows, ", ", cols,
               "], got ", c.h0.sizes());
   if (c.q.scalar_type() != at::kBFloat16 || s.K > 128 || s.V > 128 || s.K % 8 || s.V % 8) return false;
-  KDA_REQUIRE(!has_tangent({&c.q, &c.k, &c.v, &c.g, &c.beta, &c.h0}), PyExc_NotImplementedError, "kda_b200: chunk_gated_delta has no forward-mode derivative (jvp)");
   const DeltaOpts opt{c.scale ? *c.scale : 1.0 / std::sqrt(static_cast<double>(s.K)), c.output_final, c.l2norm, c.slices};
   if (c.transposed && c.h0.defined()) c.h0 = c.h0.transpose(-1, -2);
   const Tensor cu = i32(c.cu, dev);

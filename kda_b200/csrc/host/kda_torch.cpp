@@ -115,6 +115,13 @@ Tensor empty(at::IntArrayRef shape, at::ScalarType dt, const at::Device& dev) {
 Tensor bytes(size_t n, const at::Device& dev) { return empty({static_cast<int64_t>(n)}, at::kByte, dev); }
 cudaStream_t stream_of(const at::Device& dev) { return c10::cuda::getCurrentCUDAStream(dev.index()).stream(); }
 
+// Forward-mode tangents: there is no forward-mode derivative, and a call without gradients passes autograd by, which would drop them.
+bool has_tangent(std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    if (t->defined() && t->_fw_grad(0).defined()) return true;
+  return false;
+}
+
 struct Sizes {
   int64_t B, T, HQ, H, K, V;      // H counts value heads; q and k have HQ
 };
@@ -165,6 +172,8 @@ void check_head_call(const RecurrentCall& c, const Sizes& s) {
   const at::Device dev = c.q.device();
   for (const auto& [name, t] : {std::pair{"k", &c.k}, std::pair{"v", &c.v}, std::pair{"g", &c.g}, std::pair{"beta", &c.beta}, std::pair{"initial_state", &c.h0}, std::pair{"out", &c.out}})
     KDA_REQUIRE(!t->defined() || t->device() == dev, PyExc_ValueError, "kda_b200: `", name, "` is on ", t->device(), ", q on ", dev);
+  KDA_REQUIRE(!has_tangent({&c.q, &c.k, &c.v, &c.g, &c.beta, &c.h0, &c.A_log, &c.dt_bias}), PyExc_NotImplementedError,
+              "kda_b200: fused_recurrent_gated_delta has no forward-mode derivative (jvp)");
   const int64_t N = c.cu.defined() ? c.cu.numel() - 1 : s.B, rows = c.transposed ? s.V : s.K, cols = c.transposed ? s.K : s.V;
   KDA_REQUIRE(s.V % 32 == 0 && (s.K == 32 || s.K == 64 || s.K == 128 || s.K == 256), PyExc_NotImplementedError,
               "kda_b200: the token-recurrent kernels need K in {32, 64, 128, 256} and V a multiple of 32, got K=", s.K, ", V=", s.V);
@@ -445,13 +454,6 @@ struct ChunkCall {
   bool output_final = false, l2norm = false, gate = false, beta_sigmoid = false, safe_gate = false, transposed = false;
   int slices = 0;
 };
-
-// Forward-mode tangents: there is no forward-mode derivative, and a call without gradients passes autograd by, which would drop them.
-bool has_tangent(std::initializer_list<const Tensor*> ts) {
-  for (const Tensor* t : ts)
-    if (t->defined() && t->_fw_grad(0).defined()) return true;
-  return false;
-}
 
 bool wants_grad(std::initializer_list<const Tensor*> ts) {
   if (!at::GradMode::is_enabled()) return false;

@@ -47,6 +47,11 @@ def fused_recurrent_gated_delta(q, k, v, g, beta, A_log=None, dt_bias=None, scal
         use_beta_sigmoid_in_kernel=use_beta_sigmoid_in_kernel, lower_bound=lower_bound, transpose_state_layout=transpose_state_layout)
 
 
+def _no_second_derivative(grads):
+    if torch.is_grad_enabled():      # a backward with create_graph=True: the kernels' gradients carry no graph
+        raise NotImplementedError("kda_b200: chunk_gated_delta has no second derivative (create_graph=True)")
+
+
 def _float32_packed(q, k, v, g, beta, cu_seqlens, call):
     """A packed float32 call with gradients.  The kernels behind chunk_kda take the offsets as they are and leave rows of no sequence unwritten; here offsets stay
     inside the tensors, and these rows are cut off on the way in and on the way out, so that they are zero in o and in the gradients."""
@@ -80,8 +85,10 @@ def chunk_gated_delta(q, k, v, g, beta, scale=None, initial_state=None, output_f
     grads = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, g, beta, initial_state))
     if q.dtype == torch.float32 and grads:
         def per_channel(q, k, v, g, beta, cu):
-            return ops.chunk_kda(q, k, v, g.unsqueeze(-1).expand(*g.shape, K), beta, scale=scale, initial_state=initial_state, output_final_state=output_final_state,
-                                 use_qk_l2norm_in_kernel=use_qk_l2norm_in_kernel, cu_seqlens=cu, transpose_state_layout=transpose_state_layout)
+            o, ht = ops.chunk_kda(q, k, v, g.unsqueeze(-1).expand(*g.shape, K), beta, scale=scale, initial_state=initial_state, output_final_state=output_final_state,
+                                  use_qk_l2norm_in_kernel=use_qk_l2norm_in_kernel, cu_seqlens=cu, transpose_state_layout=transpose_state_layout)
+            o.grad_fn.register_prehook(_no_second_derivative)      # (of the one node that o and ht come from)
+            return o, ht
         return per_channel(q, k, v, g, beta, None) if cu_seqlens is None else _float32_packed(q, k, v, g, beta, cu_seqlens, per_channel)
     if q.dtype == torch.float32 or K > 128 or V > 128:
         if grads or (q.dtype != torch.float32 and K != 256):

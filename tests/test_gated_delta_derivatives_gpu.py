@@ -36,3 +36,18 @@ def test_inference_mode_has_none():
         args = [x[n] for n in NAMES[:5]]
         a, b = chunk_gated_delta(*args, initial_state=x["h0"])[0], fused_recurrent_gated_delta(*args, initial_state=x["h0"])[0]
         assert float((a.double() - b.double()).norm()) <= 2.0 ** -6 * float(a.double().norm())
+@pytest.mark.parametrize("tr", [False, True])
+@pytest.mark.parametrize("K,V,dtype", [(64, 64, BF), (20, 12, BF), (64, 64, F32)])
+@pytest.mark.parametrize("which", ["o", "ht", "both"])
+def test_a_gradients_gradient_is_refused(K, V, dtype, which, tr):
+    from kda_b200 import chunk_gated_delta
+    x = inputs(K, V, dtype)
+    x["v"].requires_grad_()
+    h0 = x["h0"].transpose(-1, -2).contiguous() if tr else x["h0"]
+    o, ht = chunk_gated_delta(*[x[n] for n in NAMES[:5]], initial_state=h0, output_final_state=True, transpose_state_layout=tr)
+    outs = {"o": (o,), "ht": (ht,), "both": (o, ht)}[which]
+    with pytest.raises(NotImplementedError, match="second derivative"):
+        torch.autograd.grad(outs, x["v"], [torch.ones_like(t) for t in outs], create_graph=True)
+    o, ht = chunk_gated_delta(*[x[n] for n in NAMES[:5]], initial_state=h0, output_final_state=True, transpose_state_layout=tr)
+    (dv,) = torch.autograd.grad((o, ht), x["v"], (torch.ones_like(o), torch.ones_like(ht)))      # once it is there
+    assert dv.any()

@@ -39,6 +39,12 @@ def debug_sources() -> list[str]:
     return sorted(os.path.join(d, f) for f in os.listdir(d) if f.endswith(".cu"))
 
 
+def _included(src: str) -> list[str]:
+    """Sources that a development check builds a kernel of its own from."""
+    with open(src) as f:
+        return [os.path.join(os.path.dirname(src), line.split('"')[1]) for line in f if line.startswith('#include "../')]
+
+
 def _host_command() -> list[str]:
     """g++ line of _kda_torch.so: torch's and Python's headers, libkda_b200.so found next to it at run time."""
     import torch
@@ -73,7 +79,7 @@ def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False, 
     for src in sources() + debug_sources():
         obj = os.path.join(OBJ, os.path.basename(src)[:-3] + ".o")
         (dbg_objs if os.path.dirname(src).endswith("debug") else objs).append(obj)
-        if force or _stale(obj, [src] + headers):
+        if force or _stale(obj, [src] + _included(src) + headers):
             cmd = [nvcc] + NVCC_FLAGS + (["-Xptxas", "-v"] if ptxas_info else []) + (["-DKDA_PHASE_CLOCKS"] if phase_clocks else [])
             cmd += ["-c", src, "-o", obj]
             if verbose:

@@ -10,6 +10,11 @@
 
 #include "kda_norm.cuh"
 
+#ifndef KDA_RING_VERDICT      // what a wait of the compute warps says; csrc/debug/kda_norm_ring_test.cu builds the kernel with waits that give up
+#define KDA_RING_VERDICT(ok) (ok)
+#define KDA_RING_ENTRY 1
+#endif
+
 namespace kda {
 
 namespace {
@@ -413,8 +418,9 @@ __global__ void __launch_bounds__(ROOMY ? 288 : 544, 1) norm_ring_kernel(const _
   constexpr int XS = XT == KDA_BF16 ? 2 : 4, ZS = ZT == KDA_BF16 ? 2 : 4;
   int k = 0, s = 0, next = group;      // next: this group's next row of the stage
   bool ok = true;
-  for (long long ch = blockIdx.x; ch < p.chunks; ch += gridDim.x) {
-    if (!(ok = __all_sync(0xffffffffu, mbar_wait(&full[s], k & 1)))) break;
+  long long ch = blockIdx.x;
+  for (; ch < p.chunks; ch += gridDim.x) {
+    if (!(ok = __all_sync(0xffffffffu, KDA_RING_VERDICT(mbar_wait(&full[s], k & 1))))) break;
     unsigned char* const st = smem + s * p.stage_bytes;
     const long long left = a.rows - ch * p.rows;
     int r = next;
@@ -436,7 +442,19 @@ __global__ void __launch_bounds__(ROOMY ? 288 : 544, 1) norm_ring_kernel(const _
       ++k;
     }
   }
-  if (!ok && (threadIdx.x & 31) == 0) atomicOr(&g_norm_status, 1u);
+  if (!ok) {
+    if ((threadIdx.x & 31) == 0) atomicOr(&g_norm_status, 1u);
+    // A wait gave up: this warp frees no stage any more, so that the copies and the other warps' waits come to their end too.  Until then, and beyond, the other warps
+    // of its row meet it in the row's barriers: it goes on taking part in them, once for every sum of every row that is left.
+    const int sums = (BWD ? 2 : 1) * (!GATED && a.post_weight ? 2 : 1);
+    if (p.lanes > 32)
+      for (; ch < p.chunks; ch += gridDim.x) {
+        int r = next;
+        for (; r < p.rows; r += p.groups)
+          for (int i = 0; i < sums; ++i) asm volatile("bar.sync %0, %1;" ::"r"(sum.bar), "r"(p.lanes) : "memory");
+        next = r - p.rows;
+      }
+  }
   if (BWD && p.partial) {
     constexpr int SUMS = GATED ? 1 : 2;
     float* const out = p.partial + static_cast<size_t>(blockIdx.x) * SUMS * a.cols;
@@ -559,6 +577,7 @@ static int launch_ring(const RingParams& p, cudaStream_t st) {
   }
   return launch_ring_nv<GATED, XT, ZT, VEC, BWD, 2, false>(p, st);
 }
+#ifdef KDA_RING_ENTRY
 template <bool GATED, int XT, int ZT>
 static int launch_types(const RingParams& p, bool backward, cudaStream_t st) {
   if (p.a.cols % 8 == 0) return backward ? launch_ring<GATED, XT, ZT, true, true>(p, st) : launch_ring<GATED, XT, ZT, true, false>(p, st);
@@ -579,5 +598,6 @@ int norm_ring(const kda_norm_args& a, bool gated, bool backward, float* partial,
   *partials = static_cast<int>(ring_ctas(p));
   return gated ? launch_norm<true>(p, backward, st) : launch_norm<false>(p, backward, st);
 }
+#endif
 
 }  // namespace kda

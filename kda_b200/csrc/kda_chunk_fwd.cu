@@ -279,8 +279,16 @@ extern "C" int kda_chunk_status(const void* workspace, uint32_t* host_out) {
     if (!base) return KDA_OK;
   }
   const kda::ChunkWs w = kda::carve_ws(const_cast<unsigned char*>(base), nullptr, 0, 0, 1, false);
+  // a copy alone waits for the default stream, not for those of torch: first for everything on the workspace's device
+  cudaPointerAttributes at{};
+  int dev = -1;
+  cudaError_t e = cudaPointerGetAttributes(&at, w.status);
+  if (e == cudaSuccess) e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && at.device != dev) e = cudaSetDevice(at.device);
+  if (e == cudaSuccess) e = cudaDeviceSynchronize();
   unsigned v = 0;
-  const cudaError_t e = cudaMemcpy(&v, w.status, sizeof(v), cudaMemcpyDeviceToHost);
+  if (e == cudaSuccess) e = cudaMemcpy(&v, w.status, sizeof(v), cudaMemcpyDeviceToHost);
+  if (at.device != dev && dev >= 0) cudaSetDevice(dev);
   if (e != cudaSuccess) return static_cast<int>(e);
   *host_out = v;
   return KDA_OK;

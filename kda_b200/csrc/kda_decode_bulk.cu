@@ -530,7 +530,8 @@ int decode_bulk_launch(const HeadArgs& a, bool per_head, cudaStream_t st) {
 extern "C" int kda_recurrent_status(uint32_t* host_out) {
   if (!host_out) return KDA_E_NULL;
   unsigned v = 0, zero = 0;
-  cudaError_t e = cudaMemcpyFromSymbol(&v, kda::g_decode_status, sizeof(v));
+  cudaError_t e = cudaDeviceSynchronize();      // (a copy alone waits for the default stream, not for those of torch)
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&v, kda::g_decode_status, sizeof(v));
   if (e == cudaSuccess && v) e = cudaMemcpyToSymbol(kda::g_decode_status, &zero, sizeof(zero));
   *host_out = v;
   return static_cast<int>(e);

@@ -483,7 +483,8 @@ __global__ void __launch_bounds__(ROOMY ? 288 : 544, 1) norm_ring_kernel(const _
 int norm_ring_status(uint32_t* host_out) {
   if (!host_out) return KDA_E_NULL;
   unsigned v = 0, zero = 0;
-  cudaError_t e = cudaMemcpyFromSymbol(&v, g_norm_status, sizeof(v));
+  cudaError_t e = cudaDeviceSynchronize();      // (a copy alone waits for the default stream, not for those of torch)
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&v, g_norm_status, sizeof(v));
   if (e == cudaSuccess && v) e = cudaMemcpyToSymbol(g_norm_status, &zero, sizeof(zero));
   *host_out = v;
   return static_cast<int>(e);

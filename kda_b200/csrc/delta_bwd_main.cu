@@ -59,10 +59,10 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_main_kernel(const __grid_cons
     mbar_init(&s.fullA[0], 1);
     mbar_init(&s.fullA[1], 1);
     mbar_init(&s.fullB, 1);
-    mbar_init(&s.ready, CW);
+    mbar_init(&s.ready, CW + 1);      // (one is the loading warp's, of done too: see warp_wait)
     mbar_init(&s.eReady, CW);
     mbar_init(&s.used, CW);
-    mbar_init(&s.done, CW);
+    mbar_init(&s.done, CW + 1);
     mbar_init(&s.mS, 1);
     mbar_init(&s.mY, 1);
     mbar_init(&s.mD, 1);
@@ -332,6 +332,8 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_main_kernel(const __grid_cons
     bool ok = true;
     int n = 0;
     if (lane == 0 && static_cast<int>(blockIdx.x) < total) {
+      mbar_arrive(&s.ready);
+      mbar_arrive(&s.done);
       loadA(blockIdx.x, 0);
       loadB(blockIdx.x);
     }
@@ -340,6 +342,7 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_main_kernel(const __grid_cons
       if (__any_sync(0xffffffffu, s.dead != 0)) { ok = false; break; }
       if (!(ok = warp_wait(&s.ready, n & 1))) break;      // everybody is past the tile before
       if (lane == 0) {
+        mbar_arrive(&s.ready);
         if (n > 0) store(tile - gridDim.x, n - 1);
         if (next < total) {
           bulk_wait_read<0>();
@@ -351,6 +354,7 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_main_kernel(const __grid_cons
         if (lane == 0) loadB(next);
       }
       if (!(ok = warp_wait(&s.done, n & 1))) break;
+      if (lane == 0) mbar_arrive(&s.done);
       {      // dg: the sum of dG from a token to the chunk's end, two tokens a lane (these sums are written again behind the load of the tile after the next)
         const ChunkInfo ci = p.map.info(tile / p.H);
         const int h = tile % p.H;

@@ -54,7 +54,7 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_scan_t_kernel(const __grid_co
     mbar_init(&s.dReady, CW);
     mbar_init(&s.xReady, CW);
     mbar_init(&s.yReady, CW);
-    mbar_init(&s.oReady, CW);
+    mbar_init(&s.oReady, CW + 1);      // (one is the loading warp's: see warp_wait)
     mbar_init(&s.m1, 1);
     mbar_init(&s.m2, 1);
     mbar_init(&s.m3, 1);
@@ -263,6 +263,7 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_scan_t_kernel(const __grid_co
           bulk_g2s(s.TP[0], p.TP + tile_of(i) * T_TP, 32768, &s.fullB);
         };
         bool ok = true;
+        mbar_arrive(&s.oReady);
         if (nchunks > 0) {
           loadA(0);
           loadB(0);
@@ -275,6 +276,7 @@ __global__ void __launch_bounds__(NT, 1) delta_bwd_scan_t_kernel(const __grid_co
             loadB(i + 1);
           }
           if (s.dead || !mbar_wait(&s.oReady, i & 1)) { ok = false; break; }
+          mbar_arrive(&s.oReady);
 #pragma unroll
           for (int x = 0; x < 2; ++x) bulk_s2g(p.DF + tile_of(i) * T_VN + x * 8192, s.dO[i & 1][x], 8192);
           if (tok_end - first(i) >= C) {

@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(NT, 1) delta_scan_kernel(const __grid_constant
     mbar_init(&s.hReady, 8);
     mbar_init(&s.rReady, 4);
     mbar_init(&s.uReady, 4);
-    mbar_init(&s.oReady, 4);
+    mbar_init(&s.oReady, BULK ? 5 : 4);      // (one is the loading warp's: see warp_wait)
     mbar_init(&s.m1, 1);
     mbar_init(&s.m2, 1);
     mbar_init(&s.m3, 1);
@@ -278,6 +278,7 @@ __global__ void __launch_bounds__(NT, 1) delta_scan_kernel(const __grid_constant
         bulk_g2s(s.TP[0], p.TP + (static_cast<size_t>(c0 + i) * p.H + h) * T_TP, 32768, &s.fullB);
       };
       bool ok = true;
+      if constexpr (BULK) mbar_arrive(&s.oReady);
       if (nchunks > 0) {
         loadA(0);
         loadB(0);
@@ -308,6 +309,7 @@ __global__ void __launch_bounds__(NT, 1) delta_scan_kernel(const __grid_constant
         }
         if constexpr (BULK) {               // o in q's rows
           if (!mbar_wait(&s.oReady, i & 1)) { ok = false; break; }
+          mbar_arrive(&s.oReady);
           const long long tok0 = tok_begin + static_cast<long long>(i) * C;
           if (tok_end - tok0 >= C) {
             tma_store_rows(&p.tm_o, v0, h, static_cast<int>(tok0), s.KQ[i & 1][0] + 8192);

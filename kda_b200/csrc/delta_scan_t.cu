@@ -267,11 +267,11 @@ __global__ void __launch_bounds__(NT, 1) delta_scan_t_kernel(const __grid_consta
         }
         for (int i = 0; i < nchunks; ++i) {
           if (i + 2 < nchunks) bulk_prefetch(p.TP + tile_of(i + 2) * T_TP, 32768);      // into L2
+          if (s.dead || !mbar_wait(&s.oReady, i & 1)) { ok = false; break; }      // (in front of the next load: see warp_wait)
           if (i + 1 < nchunks) {
-            if (s.dead || !mbar_wait(&s.freeB, i & 1)) { ok = false; break; }
+            if (!mbar_wait(&s.freeB, i & 1)) { ok = false; break; }
             loadB(i + 1);
           }
-          if (s.dead || !mbar_wait(&s.oReady, i & 1)) { ok = false; break; }
           if constexpr (TRAIN) {                 // v_new stands in v's tile
 #pragma unroll
             for (int x = 0; x < 2; ++x) bulk_s2g(p.VN + tile_of(i) * T_VN + x * 8192, s.V[i & 1][x], 8192);

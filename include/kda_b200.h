@@ -365,7 +365,9 @@ int kda_gate_bwd(const kda_gate_args* args, void* stream);
  * zeros; with N = 0 all rows do.
  *
  * kda_delta_chunk_fwd / _bwd: whole sequences in chunks of 64 tokens on the tensor cores, bf16 q, k, v, o.  States, their gradients and every sum are
- * fp32, and operands that are not inputs are bf16 pairs in the two walks over a sequence: final states and dh0 carry about 1e-5 of their norm.  Rules as
+ * fp32, and operands that are not inputs are bf16 pairs in the two walks over a sequence: final states and dh0 carry about 1e-5 of their norm.  The other gradients
+ * take one bf16 per operand (dq, dk, dg, dbeta: about 3e-3 of their norm), and with HQ < H dq and dk are rounded to bf16 for every value head in front of a group's
+ * fp32 sum: about as much of each head's gradient, whatever the sum comes to.  Rules as
  * for kda_chunk_fwd / _bwd: the workspace of a forward with save_for_backward goes to the backward untouched; kda_chunk_status reads its status word.
  * Rows in front of the first sequence of cu_seqlens and behind the last one are zero in o and in the gradients; with N = 0 all rows are.
  * ------------------------------------------------------------------------------------------------ */

@@ -19,7 +19,8 @@
 //
 // Precision.  State and gradient of the state are fp32 in registers.  Every operand that is not an input (h, r, v_new, dh', x, f, Tm, Pt) enters the two
 // scans as two bf16, hi + lo = 17 bits, with the products hi hi, hi lo and lo hi: final states are good to about 1e-5 of their norm, where one
-// bf16 per operand gives 3e-3.  The per-chunk gradients, which end in bf16, take one bf16 per operand.
+// bf16 per operand gives 3e-3.  The per-chunk gradients, which end in bf16, take one bf16 per operand; dq and dk of a group's value heads are rounded per head, in front
+// of their fp32 sum.
 //
 // Tiles in the workspace, per (chunk, head), bf16 rows of 128 bytes, swizzled (umma::sw128), each a tcgen05 operand as it lies in memory:
 //   TP      [128][64] hi, then lo: rows 0..63 Tm, rows 64..127 Pt

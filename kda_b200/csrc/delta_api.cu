@@ -63,7 +63,7 @@ static int launch_tail(const TailParams& p, cudaStream_t st) { return static_cas
 
 // Sums dq, dk of a group's value heads: eight columns per thread.  The sum is fp32 and rounded once; its terms arrive as bf16, like the operands that they were made
 // from (delta.cuh), so what is lost is 2^-8 of each head's gradient, not of the sum's, should the heads cancel.  As fp32 they would be twice the bytes (8 x 4,096 tokens x 32
-// value heads: 1 GB more to write and read again), and the gradients of a head would still be good to some 2^-8 of its own.
+// value heads: 0.5 GB more to write and read again), and the gradients of a head would still be good to some 2^-8 of its own.
 __global__ void __launch_bounds__(256) delta_group_sum_kernel(const __nv_bfloat16* dqh, const __nv_bfloat16* dkh, __nv_bfloat16* dq, __nv_bfloat16* dk, long long pieces,
                                                               int per_row, int grp) {
   chain_point();

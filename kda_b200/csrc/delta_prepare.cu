@@ -53,7 +53,6 @@ __device__ __forceinline__ Two add(const Two& a, const Two& b) {
   const float s = a.hi + b.hi, v = s - a.hi, e = (a.hi - (s - v)) + (b.hi - v) + (a.lo + b.lo), hi = s + e;
   return {hi, e - (hi - s)};
 }
-constexpr float LOG2E_REST = 1.92596299e-8f;      // log2(e) - LOG2E
 // exp(G_i - G_j)
 __device__ __forceinline__ float decay_between(const PrepSmem& s, int i, int j) { return ex2((s.ghi[i] - s.ghi[j]) + (s.glo[i] - s.glo[j])); }
 struct FragPair { uint32_t h[4], l[4]; };

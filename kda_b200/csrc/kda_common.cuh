@@ -12,6 +12,7 @@ namespace kda {
 
 constexpr int C = KDA_CHUNK;              // tokens per chunk
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LOG2E_REST = 1.92596299e-8f;      // log2(e) - LOG2E
 constexpr float L2NORM_EPS = 1e-6f;
 
 // First statement of every kernel that takes part in a chain of launches (launch_chained): waits until the kernels in front have finished

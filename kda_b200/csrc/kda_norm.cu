@@ -96,6 +96,11 @@ __device__ __forceinline__ void my_rows(const NormParams& p, long long& row, lon
   last = (p.a.rows + per - 1) / per * per;      // the same number of turns for a CTA's threads
 }
 
+__device__ __forceinline__ void act_as(bool exact, float z, int activation, float& act, float& slope) {
+  if (exact) act_of<true>(z, activation, act, slope);
+  else act_of<false>(z, activation, act, slope);
+}
+
 // ---- gated -----------------------------------------------------------------------------------------------------------------------------------
 template <bool VEC, int NV, bool WIDE>
 __global__ void gated_fwd_kernel(const __grid_constant__ NormParams p) {
@@ -104,6 +109,7 @@ __global__ void gated_fwd_kernel(const __grid_constant__ NormParams p) {
   const Cols<VEC> c = my_cols<VEC, NV, WIDE>(p);
   RowSum<WIDE> sum{part, p.lanes};
   const float inv = 1.f / a.cols;
+  const bool exact = a.io_dtype == KDA_FP32;
   long long row, step, last;
   my_rows<WIDE>(p, row, step, last);
   float w[NV][8];
@@ -141,7 +147,7 @@ __global__ void gated_fwd_kernel(const __grid_constant__ NormParams p) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         float act, slope;
-        act_of(z[j], a.activation, act, slope);
+        act_as(exact, z[j], a.activation, act, slope);
         z[j] = x[i][j] * rstd * w[i][j] * act;
       }
       store8<VEC>(a.y, row, a.io_dtype, c, i, z);
@@ -156,6 +162,7 @@ __global__ void __launch_bounds__(WIDE ? 512 : NORM_CTA) gated_bwd_kernel(const 
   const Cols<VEC> c = my_cols<VEC, NV, WIDE>(p);
   RowSum<WIDE> sum{part, p.lanes};
   const float inv = 1.f / a.cols;
+  const bool exact = a.io_dtype == KDA_FP32;
   long long row, step, last;
   my_rows<WIDE>(p, row, step, last);
   float w[NV][8], acc[1][NV][8] = {};
@@ -195,7 +202,7 @@ __global__ void __launch_bounds__(WIDE ? 512 : NORM_CTA) gated_bwd_kernel(const 
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         float act, slope;
-        act_of(dz[i][j], a.activation, act, slope);
+        act_as(exact, dz[i][j], a.activation, act, slope);
         x[i][j] *= rstd;
         acc[0][i][j] = there ? fmaf(d[j] * x[i][j], act, acc[0][i][j]) : acc[0][i][j];
         dn[i][j] = d[j] * w[i][j] * act;

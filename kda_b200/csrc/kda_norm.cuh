@@ -99,10 +99,26 @@ __device__ __forceinline__ void store8(void* p, size_t row, int dtype, const Col
   }
 }
 
+// The gate's activation and its slope.  For bf16 results the fast exponential and reciprocal do (their error grows with |z|: 4e-6 at 86).  EXACT, for float32 x: to float32's
+// rounding.  exp(-z) = 2^hi (1 + lo ln 2) with hi + lo the product -z log2(e) in two floats, and 1 - sigmoid(z) is exp(-z) sigmoid(z), which does not cancel for large z.
+// Beyond +-88 either of them is below the normal float32 numbers, and zero; NaN stays.
+template <bool EXACT>
 __device__ __forceinline__ void act_of(float z, int activation, float& act, float& slope) {
-  const float sg = sigmoid_fast(z);
-  act = activation == KDA_ACT_SILU ? z * sg : sg;
-  slope = activation == KDA_ACT_SILU ? sg * fmaf(z, 1.f - sg, 1.f) : sg * (1.f - sg);
+  if constexpr (EXACT) {
+    float zc, e, sg;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(z) : "f"(z), "f"(-88.f));
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(zc) : "f"(z), "f"(88.f));
+    const float hi = -zc * LOG2E, lo = fmaf(-zc, LOG2E_REST, fmaf(-zc, LOG2E, -hi));
+    e = ex2(hi) * fmaf(lo, 0.69314718f, 1.f);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(sg) : "f"(1.f + e));
+    const float rest = e * sg;
+    act = activation == KDA_ACT_SILU ? z * sg : sg;
+    slope = activation == KDA_ACT_SILU ? sg * fmaf(zc, rest, 1.f) : sg * rest;
+  } else {
+    const float sg = sigmoid_fast(z);
+    act = activation == KDA_ACT_SILU ? z * sg : sg;
+    slope = activation == KDA_ACT_SILU ? sg * fmaf(z, 1.f - sg, 1.f) : sg * (1.f - sg);
+  }
 }
 
 // eight columns of a parameter (1 where there is none), of the scale (its one value where it is a number)

@@ -131,7 +131,7 @@ __device__ __forceinline__ void gated_row(const kda_norm_args& a, const float* w
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         float act, slope;
-        act_of(z[j], a.activation, act, slope);
+        act_of<XT == KDA_FP32>(z[j], a.activation, act, slope);
         z[j] = x[i][j] * rstd * w[j] * act;
       }
       put8<XT, VEC>(x_, c, i, z);
@@ -147,7 +147,7 @@ __device__ __forceinline__ void gated_row(const kda_norm_args& a, const float* w
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         float act, slope;
-        act_of(z[j], a.activation, act, slope);
+        act_of<XT == KDA_FP32>(z[j], a.activation, act, slope);
         x[i][j] *= rstd;
         const float da = d[j] * act, dx = d[j] * x[i][j] * w[j];
         if (there) acc[0][i][j] = fmaf(da, x[i][j], acc[0][i][j]);

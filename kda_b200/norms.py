@@ -14,8 +14,8 @@ def _native():
 def gated_rms_norm(x, gate, weight=None, eps=1e-6, activation="sigmoid"):
     """y = x / sqrt(mean(x^2) + eps) * weight * act(gate) over the last dimension (up to 8192 columns), act = "sigmoid", or "silu" ("swish"): z sigmoid(z).
 
-    x and gate [..., D] in bfloat16 or float32 each, weight [D] or None.  y has x's type.  Differentiable with respect to all three; sums over rows are taken in
-    float32 and in a fixed order."""
+    x and gate [..., D] in bfloat16 or float32 each, weight [D] or None.  y has x's type; with float32 x the activation is good to float32's rounding, with bfloat16 x
+    fast exponentials are taken (4e-6 at most).  Differentiable with respect to all three; sums over rows are taken in float32 and in a fixed order."""
     if activation not in _ACTIVATIONS:
         raise ValueError(f"kda_b200: activation must be one of {sorted(_ACTIVATIONS)}, got {activation!r}")
     return _native().gated_norm(x, gate, weight, eps, _ACTIVATIONS[activation])

@@ -86,14 +86,31 @@ struct RowBits {
   }
 };
 
-// One decay per head, packed: rows of o in front of the first sequence and behind the last one become zeros, by the warps of these sequences.
-// (bos, eos: of sequence n, inside the call's tokens if cu_seqlens is in order; otherwise the rows are cut to them.)
-template <class Z>
-__device__ __forceinline__ void rows_of_none(const HeadArgs& a, int n, long long bos, long long eos, Z&& zeros) {
-  if (!a.cu_seqlens) return;
-  if (n == 0) zeros(0, bos < a.tokens ? bos : a.tokens);
-  if (n == a.N - 1) zeros(eos > 0 ? eos : 0, a.tokens);
-}
+// One decay per head, packed: rows of o in front of the first sequence and behind the last one become zeros.  All sequences' warps share them, so that a server's padded
+// buffer costs no more than its bytes.  Asked for in front of the tokens, used behind them; cut to the call's tokens.
+struct RowsOfNone {
+  long long first, last;
+  __device__ __forceinline__ explicit RowsOfNone(const HeadArgs& a) : first(0), last(a.tokens) {
+    if (!a.cu_seqlens) return;
+    first = a.cu_seqlens[0];
+    last = a.cu_seqlens[a.N];
+  }
+  __device__ __forceinline__ explicit RowsOfNone(const kda_recurrent_args&) {}
+  // a warp's part: four columns from `col` on in every RG-th row, rg the lane's first
+  template <typename IO, int RG>
+  __device__ __forceinline__ void clear(const HeadArgs& a, long long n, int h, int col, int rg) const {
+    const size_t row = static_cast<size_t>(a.H) * a.V, step = static_cast<size_t>(a.N) * RG * row;
+    auto zeros = [&](long long from, long long to) {
+      long long t = from + n * RG + rg;
+      IO* p = static_cast<IO*>(a.o) + static_cast<size_t>(t) * row + static_cast<size_t>(h) * a.V + col;
+#pragma unroll 4
+      for (; t < to; t += static_cast<long long>(a.N) * RG, p += step) IoTraits<IO>::st4(p, make_float4(0.f, 0.f, 0.f, 0.f));
+    };
+    zeros(0, first < a.tokens ? first : a.tokens);
+    const long long from = last > 0 ? last : 0;
+    zeros(first > from ? first : from, a.tokens);
+  }
+};
 
 // A token's vectors are fetched while the token before is worked on: with one warp per slice there is nobody else to hide
 // their latency (one sequence of four draft tokens: 14.2 us when each token fetched its own, 8.0 us so).
@@ -153,15 +170,13 @@ __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_kernel(const Rec
   };
   // continuous batching: the sequence's row of slot numbers; it starts from the slot of the last accepted token
   const int32_t* slots = a.state_indices ? a.state_indices + static_cast<size_t>(n) * a.state_indices_stride : nullptr;
+  const RowsOfNone none(a);
   long long slot = n;
   if constexpr (HEAD) {
-    auto zeros = [&](long long from, long long to) {
-      if (rg == 0)
-        for (long long t = from; t < to; ++t) IoTraits<IO>::st4(static_cast<IO*>(a.o) + (static_cast<size_t>(t) * a.H + h) * a.V + col, make_float4(0.f, 0.f, 0.f, 0.f));
-    };
-    rows_of_none(a, n, bos, eos, zeros);
     if (slots && !a.holds(slot = a.start_slot(n))) {
-      zeros(bos, eos);
+      if (rg == 0)
+        for (long long t = bos; t < eos; ++t) IoTraits<IO>::st4(static_cast<IO*>(a.o) + (static_cast<size_t>(t) * a.H + h) * a.V + col, make_float4(0.f, 0.f, 0.f, 0.f));
+      none.clear<IO, RG>(a, n, h, col, rg);
       return;
     }
   } else if (slots) {
@@ -273,6 +288,7 @@ __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_kernel(const Rec
     for (int i = 0; i < R; ++i)
       __stcs(reinterpret_cast<float4*>(a.ht + sbase + static_cast<size_t>(rg + RG * i) * a.V), S[i]);
   }
+  if constexpr (HEAD) none.clear<IO, RG>(a, n, h, col, rg);
 }
 
 // E (2 or 4) consecutive floats of a state row, streaming loads / stores of 8 or 16 bytes
@@ -322,14 +338,12 @@ __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_t_kernel(const R
     eos = bos + a.T;
   }
   const int32_t* slots = a.state_indices ? a.state_indices + static_cast<size_t>(n) * a.state_indices_stride : nullptr;
+  const RowsOfNone none(a);
   long long slot = n;
   if constexpr (HEAD) {
-    auto zeros = [&](long long from, long long to) {
-      for (long long t = from; t < to; ++t) static_cast<IO*>(a.o)[(static_cast<size_t>(t) * a.H + h) * a.V + vs * 32 + lane] = IO(0.f);
-    };
-    rows_of_none(a, n, bos, eos, zeros);
     if (slots && !a.holds(slot = a.start_slot(n))) {
-      zeros(bos, eos);
+      for (long long t = bos; t < eos; ++t) static_cast<IO*>(a.o)[(static_cast<size_t>(t) * a.H + h) * a.V + vs * 32 + lane] = IO(0.f);
+      none.clear<IO, 4>(a, n, h, vs * 32 + 4 * (lane & 7), lane >> 3);
       return;
     }
   } else if (slots) {
@@ -420,6 +434,7 @@ __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_t_kernel(const R
 #pragma unroll
     for (int r = 0; r < 32; ++r) st_row<E>(pt + static_cast<size_t>(r) * K, S[r]);
   }
+  if constexpr (HEAD) none.clear<IO, 4>(a, n, h, vs * 32 + 4 * (lane & 7), lane >> 3);
 }
 
 template <typename IO, int K, bool HEAD>

@@ -47,7 +47,7 @@ def test_in_front_and_behind(K, V, dtype, grads):
 
 
 @pytest.mark.parametrize("K,V,dtype,tr", [(64, 64, BF, False), (128, 128, BF, True), (256, 32, BF, False), (32, 96, F32, False), (64, 32, F32, True)])
-@pytest.mark.parametrize("cu", [[10, 60, 170], [0, 0, 170], [200, 200], [0], [0, 200]])
+@pytest.mark.parametrize("cu", [[10, 60, 170], [0, 0, 170], [200, 200], [0], [0, 200], [3, 50, 51, 51, 90, 137]])
 def test_token_by_token(K, V, dtype, tr, cu):
     from kda_b200 import fused_recurrent_gated_delta
     d = {n: t.cuda() for n, t in make(1, 200, 2, 4, K, V, seed=3, h0=False, dtype=dtype).items() if t is not None}
@@ -70,6 +70,20 @@ def test_a_servers_padded_output():
     out = torch.full_like(d["v"], float("nan"))
     fused_recurrent_gated_delta_fwd(*args, initial_state=pool, cu_seqlens=torch.zeros(1, dtype=torch.int32, device="cuda"), ssm_state_indices=slots[:0], out=out)
     assert not out.any() and torch.equal(pool, before)
+
+
+@pytest.mark.parametrize("tr", [False, True])
+def test_a_padded_entry_and_padded_rows(tr):
+    """A packed decode call of four sequences, two of them padded entries, in a buffer that is much larger than their tokens."""
+    from kda_b200 import fused_recurrent_gated_delta_fwd
+    d = {n: t.cuda() for n, t in make(1, 1000, 2, 2, 64, 64, seed=6, h0=False).items() if t is not None}
+    cu, slots = torch.tensor([5, 8, 10, 13, 14], dtype=torch.int32, device="cuda"), torch.tensor([[0, 1, 2], [-1, 3, 3], [4, 5, 6], [9, 9, 9]], dtype=torch.int32, device="cuda")
+    pool = torch.randn(8, 2, 64, 64, device="cuda")
+    out = torch.full_like(d["v"], float("nan"))
+    fused_recurrent_gated_delta_fwd(*[d[n] for n in ("q", "k", "v", "g", "beta")], initial_state=pool, cu_seqlens=cu, ssm_state_indices=slots, out=out, transpose_state_layout=tr)
+    there = torch.zeros(1000, dtype=torch.bool, device="cuda")
+    there[5:8] = there[10:13] = True
+    assert out[:, there].isfinite().all() and out[:, there].abs().sum((0, 2, 3)).all() and not out[:, ~there].any()
 
 
 @pytest.mark.parametrize("cu", [[0, 400], [-64, 70], [50, 20, 70], [90, 100]])

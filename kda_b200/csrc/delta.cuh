@@ -182,6 +182,17 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) {
   __syncwarp();
   if (lane == 0) mbar_arrive(bar);
 }
+// eight columns (col a multiple of 8) of a row of an operand of VC columns as bf16 pairs: 32 + 32 side by side in one tile, 64 in two
+template <int VC>
+__device__ __forceinline__ void put(unsigned char* tile, int rows, int row, int col, const Split& x) {
+  if constexpr (VC == 32) {
+    *reinterpret_cast<uint4*>(piece(tile, row, col >> 3)) = x.hi;
+    *reinterpret_cast<uint4*>(piece(tile, row, 4 + (col >> 3))) = x.lo;
+  } else {
+    *reinterpret_cast<uint4*>(piece(tile, row, col >> 3)) = x.hi;
+    *reinterpret_cast<uint4*>(piece(tile + rows * 128, row, col >> 3)) = x.lo;
+  }
+}
 // One value column of a [64 t][64 v] tile in shared memory, two bytes a row: `at` from column_at for a first row that is a multiple of eight, `j` rows further.
 __device__ __forceinline__ uint32_t column_at(const unsigned char* tile, int row, int v) { return smem_u32(tile) + umma::sw128(row, v); }
 __device__ __forceinline__ uint32_t column_get(uint32_t at, int j) {

@@ -33,17 +33,6 @@ struct RSmem {
 };
 static_assert(sizeof(RSmem<64>) + 1024 <= 227 * 1024, "RSmem too large");
 
-template <int VC>
-__device__ __forceinline__ void put(unsigned char* tile, int rows, int row, int col, const Split& x) {
-  if constexpr (VC == 32) {
-    *reinterpret_cast<uint4*>(piece(tile, row, col >> 3)) = x.hi;
-    *reinterpret_cast<uint4*>(piece(tile, row, 4 + (col >> 3))) = x.lo;
-  } else {
-    *reinterpret_cast<uint4*>(piece(tile, row, col >> 3)) = x.hi;
-    *reinterpret_cast<uint4*>(piece(tile + rows * 128, row, col >> 3)) = x.lo;
-  }
-}
-
 }  // namespace
 
 template <int VC>

@@ -47,7 +47,7 @@ __device__ __forceinline__ void frag_a(uint32_t (&f)[4], const unsigned char* ti
 __device__ __forceinline__ void frag_b(uint32_t (&f)[4], const unsigned char* tile, int row, int col, int lane) {
   ldsm_x4_t(f, smem_u32(tile) + umma::sw128(row + (lane & 15), col + 8 * (lane >> 4)));
 }
-// the sum of two numbers as two floats each, to the last bit but a few of 48
+// the sum of two numbers as two floats each, to the last bit but a few of 48 (Knuth's sum with its rounding error, of the high parts)
 struct Two { float hi, lo; };
 __device__ __forceinline__ Two add(const Two& a, const Two& b) {
   const float s = a.hi + b.hi, v = s - a.hi, e = (a.hi - (s - v)) + (b.hi - v) + (a.lo + b.lo), hi = s + e;

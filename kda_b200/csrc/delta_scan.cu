@@ -36,18 +36,6 @@ struct ScanSmem {
 };
 static_assert(sizeof(ScanSmem<64>) + 1024 <= 227 * 1024, "ScanSmem too large");
 
-// where eight columns (col a multiple of 8) of a row stand in an operand of VC columns as bf16 pairs
-template <int VC>
-__device__ __forceinline__ void put(unsigned char* tile, int rows, int row, int col, const Split& x) {
-  if constexpr (VC == 32) {
-    *reinterpret_cast<uint4*>(piece(tile, row, col >> 3)) = x.hi;
-    *reinterpret_cast<uint4*>(piece(tile, row, 4 + (col >> 3))) = x.lo;
-  } else {
-    *reinterpret_cast<uint4*>(piece(tile, row, col >> 3)) = x.hi;
-    *reinterpret_cast<uint4*>(piece(tile + rows * 128, row, col >> 3)) = x.lo;
-  }
-}
-
 }  // namespace
 
 template <int VC, bool TRAIN>

@@ -90,15 +90,14 @@ struct RowBits {
 // buffer costs no more than its bytes.  Asked for in front of the tokens, used behind them; cut to the call's tokens.
 struct RowsOfNone {
   long long first, last;
-  __device__ __forceinline__ explicit RowsOfNone(const HeadArgs& a) : first(0), last(a.tokens) {
-    if (!a.cu_seqlens) return;
-    first = a.cu_seqlens[0];
-    last = a.cu_seqlens[a.N];
+  template <bool CLEAR>
+  __device__ __forceinline__ static RowsOfNone of(const kda_recurrent_args& a) {
+    if constexpr (CLEAR) return {a.cu_seqlens[0], a.cu_seqlens[a.N]};
+    else return {0, 0};
   }
-  __device__ __forceinline__ explicit RowsOfNone(const kda_recurrent_args&) {}
   // a warp's part: four columns from `col` on in every RG-th row, rg the lane's first
   template <typename IO, int RG>
-  __device__ __forceinline__ void clear(const HeadArgs& a, long long n, int h, int col, int rg) const {
+  __device__ __forceinline__ void clear(const kda_recurrent_args& a, long long n, int h, int col, int rg) const {
     const size_t row = static_cast<size_t>(a.H) * a.V, step = static_cast<size_t>(a.N) * RG * row;
     auto zeros = [&](long long from, long long to) {
       long long t = from + n * RG + rg;
@@ -115,7 +114,8 @@ struct RowsOfNone {
 // A token's vectors are fetched while the token before is worked on: with one warp per slice there is nobody else to hide
 // their latency (one sequence of four draft tokens: 14.2 us when each token fetched its own, 8.0 us so).
 // HEAD: one decay per token and head (kda_delta_recurrent_fwd).
-template <typename IO, int K, int VS, bool HEAD>
+// CLEAR (with HEAD): packed, so that there may be rows of no sequence (a variant of its own: with the rows' few instructions in it one token of one sequence takes 4.1 us, 3.6 without).
+template <typename IO, int K, int VS, bool HEAD, bool CLEAR>
 __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_kernel(const RecArgs<HEAD> a) {
   chain_point();
   constexpr int CL = VS / 4;      // lanes across the V slice (4 columns each)
@@ -170,13 +170,13 @@ __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_kernel(const Rec
   };
   // continuous batching: the sequence's row of slot numbers; it starts from the slot of the last accepted token
   const int32_t* slots = a.state_indices ? a.state_indices + static_cast<size_t>(n) * a.state_indices_stride : nullptr;
-  const RowsOfNone none(a);
+  [[maybe_unused]] const RowsOfNone none = RowsOfNone::of<CLEAR>(a);
   long long slot = n;
   if constexpr (HEAD) {
     if (slots && !a.holds(slot = a.start_slot(n))) {
       if (rg == 0)
         for (long long t = bos; t < eos; ++t) IoTraits<IO>::st4(static_cast<IO*>(a.o) + (static_cast<size_t>(t) * a.H + h) * a.V + col, make_float4(0.f, 0.f, 0.f, 0.f));
-      none.clear<IO, RG>(a, n, h, col, rg);
+      if constexpr (CLEAR) none.clear<IO, RG>(a, n, h, col, rg);
       return;
     }
   } else if (slots) {
@@ -288,7 +288,7 @@ __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_kernel(const Rec
     for (int i = 0; i < R; ++i)
       __stcs(reinterpret_cast<float4*>(a.ht + sbase + static_cast<size_t>(rg + RG * i) * a.V), S[i]);
   }
-  if constexpr (HEAD) none.clear<IO, RG>(a, n, h, col, rg);
+  if constexpr (CLEAR) none.clear<IO, RG>(a, n, h, col, rg);
 }
 
 // E (2 or 4) consecutive floats of a state row, streaming loads / stores of 8 or 16 bytes
@@ -313,7 +313,7 @@ __device__ __forceinline__ void st_row(float* p, const float (&d)[E]) {
 // lane*(K/32) .. of those rows, so every state access is again contiguous over the warp.  The two reductions over K
 // are per-lane partial dot products summed over the lanes 32 values at a time by a butterfly (lane L ends up with
 // the total of value row L); the delta-rule update needs every row's dv in every lane: one shuffle per row.
-template <typename IO, int K, bool HEAD>
+template <typename IO, int K, bool HEAD, bool CLEAR>
 __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_t_kernel(const RecArgs<HEAD> a) {
   constexpr int E = K / 32;       // key columns per lane
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -338,12 +338,12 @@ __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_t_kernel(const R
     eos = bos + a.T;
   }
   const int32_t* slots = a.state_indices ? a.state_indices + static_cast<size_t>(n) * a.state_indices_stride : nullptr;
-  const RowsOfNone none(a);
+  [[maybe_unused]] const RowsOfNone none = RowsOfNone::of<CLEAR>(a);
   long long slot = n;
   if constexpr (HEAD) {
     if (slots && !a.holds(slot = a.start_slot(n))) {
       for (long long t = bos; t < eos; ++t) static_cast<IO*>(a.o)[(static_cast<size_t>(t) * a.H + h) * a.V + vs * 32 + lane] = IO(0.f);
-      none.clear<IO, 4>(a, n, h, vs * 32 + 4 * (lane & 7), lane >> 3);
+      if constexpr (CLEAR) none.clear<IO, 4>(a, n, h, vs * 32 + 4 * (lane & 7), lane >> 3);
       return;
     }
   } else if (slots) {
@@ -434,7 +434,7 @@ __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_t_kernel(const R
 #pragma unroll
     for (int r = 0; r < 32; ++r) st_row<E>(pt + static_cast<size_t>(r) * K, S[r]);
   }
-  if constexpr (HEAD) none.clear<IO, 4>(a, n, h, vs * 32 + 4 * (lane & 7), lane >> 3);
+  if constexpr (CLEAR) none.clear<IO, 4>(a, n, h, vs * 32 + 4 * (lane & 7), lane >> 3);
 }
 
 template <typename IO, int K, bool HEAD>
@@ -443,7 +443,13 @@ static int launch_rec_t(const RecArgs<HEAD>& a, cudaStream_t st) {
   const long long blocks = (total + REC_WARPS - 1) / REC_WARPS;
   if (blocks <= 0) return KDA_OK;
   if (blocks > 0x7fffffffLL) return KDA_E_SHAPE;
-  kda_recurrent_t_kernel<IO, K, HEAD><<<static_cast<unsigned>(blocks), REC_WARPS * 32, 0, st>>>(a);
+  if constexpr (HEAD) {
+    if (a.cu_seqlens) {
+      kda_recurrent_t_kernel<IO, K, HEAD, true><<<static_cast<unsigned>(blocks), REC_WARPS * 32, 0, st>>>(a);
+      return static_cast<int>(cudaGetLastError());
+    }
+  }
+  kda_recurrent_t_kernel<IO, K, HEAD, false><<<static_cast<unsigned>(blocks), REC_WARPS * 32, 0, st>>>(a);
   return static_cast<int>(cudaGetLastError());
 }
 
@@ -453,7 +459,10 @@ static int launch_rec(const RecArgs<HEAD>& a, cudaStream_t st) {
   const long long blocks = (total + REC_WARPS - 1) / REC_WARPS;
   if (blocks <= 0) return KDA_OK;
   if (blocks > 0x7fffffffLL) return KDA_E_SHAPE;
-  return static_cast<int>(launch_chained(kda_recurrent_kernel<IO, K, VS, HEAD>, static_cast<unsigned>(blocks), REC_WARPS * 32, 0, st, a));
+  if constexpr (HEAD) {
+    if (a.cu_seqlens) return static_cast<int>(launch_chained(kda_recurrent_kernel<IO, K, VS, HEAD, true>, static_cast<unsigned>(blocks), REC_WARPS * 32, 0, st, a));
+  }
+  return static_cast<int>(launch_chained(kda_recurrent_kernel<IO, K, VS, HEAD, false>, static_cast<unsigned>(blocks), REC_WARPS * 32, 0, st, a));
 }
 
 template <typename IO, bool HEAD>

@@ -67,6 +67,27 @@ __device__ __forceinline__ float softplus_fast(float x) {
   const float e = __expf(fminf(x, 20.f));
   return x > 20.f ? x : (x < -15.f ? e : __logf(1.f + e));
 }
+// ---- the same to float32's rounding (the decode call with one decay per head, the gated norm on float32) -------------
+__device__ __forceinline__ float clamp_nan(float x, float low, float high) {      // NaN stays
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(low));
+  asm("min.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(high));
+  return x;
+}
+// exp(x) = 2^hi (1 + lo ln 2), hi + lo the product x log2(e) in two floats; zero below -88 (no normal float32), infinite above 89
+__device__ __forceinline__ float exp_full(float x) {
+  x = clamp_nan(x, -89.f, 90.f);
+  const float hi = x * LOG2E, lo = fmaf(x, LOG2E_REST, fmaf(x, LOG2E, -hi));
+  return ex2(hi) * fmaf(lo, 0.69314718f, 1.f);
+}
+// sigmoid(z) = 1 / (1 + exp(-z)); rest: 1 - sigmoid(z) as exp(-z) sigmoid(z), which does not cancel for large z
+__device__ __forceinline__ float sigmoid_full(float z, float& rest) {
+  const float e = exp_full(-clamp_nan(z, -88.f, 88.f));
+  float sg;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(sg) : "f"(1.f + e));
+  rest = e * sg;
+  return sg;
+}
+__device__ __forceinline__ float softplus_full(float x) { return fmaxf(x, 0.f) + log1pf(exp_full(-fabsf(x))); }
 // ---- gate front end of the recurrent kernels: activated log-decay and beta from the raw layer outputs -------------
 __device__ __forceinline__ float load_raw(const void* p, size_t i, int dtype) {      // dtype: KDA_BF16 or KDA_FP32
   return dtype == KDA_BF16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]) : static_cast<const float*>(p)[i];
@@ -83,17 +104,26 @@ __device__ __forceinline__ float recurrent_beta(const kda_recurrent_args& a, siz
   return a.beta_sigmoid ? sigmoid_fast(load_raw(a.beta, row, a.beta_raw_dtype)) : a.beta[row];
 }
 
-// the same with one decay per token and head
+// The same with one decay per token and head.  To float32's rounding: with dt_bias around -7, as layers have it, softplus_fast is 7e-5 of itself off, and A times that is in every
+// decay of the state (states behind a few tokens: 1e-6 of their norm, 1e-7 so); one value per token and head costs nothing.
+__device__ __forceinline__ float head_gate(float x, float A_log, const kda_recurrent_args& a) {
+  const float al = exp_full(A_log);
+  float rest;
+  return a.use_lower_bound ? a.lower_bound * sigmoid_full(al * x, rest) : -al * softplus_full(x);
+}
+__device__ __forceinline__ float head_sigmoid(float x) {
+  float rest;
+  return sigmoid_full(x, rest);
+}
 __device__ __forceinline__ float recurrent_head_decay(const kda_recurrent_args& a, size_t row, int h) {
   float x = load_raw(a.g, row, a.g_raw_dtype);
   if (!a.A_log) return x;
   if (a.dt_bias) x += a.dt_bias[h];
-  const float al = __expf(a.A_log[h]);
-  return a.use_lower_bound ? a.lower_bound * sigmoid_fast(al * x) : -al * softplus_fast(x);
+  return head_gate(x, a.A_log[h], a);
 }
 __device__ __forceinline__ float recurrent_head_beta(const kda_recurrent_args& a, size_t row) {
   const float x = load_raw(a.beta, row, a.beta_raw_dtype);
-  return a.beta_sigmoid ? sigmoid_fast(x) : x;
+  return a.beta_sigmoid ? head_sigmoid(x) : x;
 }
 
 // ---- tensor-core primitives (warp-level, bf16 in / fp32 accumulate) ------------------------------

@@ -275,17 +275,21 @@ __global__ void __launch_bounds__(HV * 2 + 32, 128 / HV) kda_decode_bulk_kernel(
       if constexpr (GATE) {
         if (a.A_log) {
           const float x = to_float(r.x[RG], a.g_raw_dtype == KDA_BF16) + __uint_as_float(r.x[RBIAS]);
-          const float al = __expf(__uint_as_float(r.x[RA]));
-          g = a.use_lower_bound ? a.lower_bound * sigmoid_fast(al * x) : -al * softplus_fast(x);
+          if constexpr (HEAD) {
+            g = head_gate(x, __uint_as_float(r.x[RA]), a);
+          } else {
+            const float al = __expf(__uint_as_float(r.x[RA]));
+            g = a.use_lower_bound ? a.lower_bound * sigmoid_fast(al * x) : -al * softplus_fast(x);
+          }
         }
       }
-      s.eg[buf][e] = __expf(g);
+      s.eg[buf][e] = HEAD ? exp_full(g) : __expf(g);
       if (e < HV) s.vv[buf][e] = to_float(r.x[RV], IO16);
     }
     if (tid == 0) {
       float b = to_float(r.x[RB], HEAD && a.beta_raw_dtype == KDA_BF16);
       if constexpr (GATE) {
-        if (a.beta_sigmoid) b = sigmoid_fast(to_float(r.x[RB], a.beta_raw_dtype == KDA_BF16));
+        if (a.beta_sigmoid) b = HEAD ? head_sigmoid(to_float(r.x[RB], a.beta_raw_dtype == KDA_BF16)) : sigmoid_fast(to_float(r.x[RB], a.beta_raw_dtype == KDA_BF16));
       }
       s.beta[buf] = b;
     }

@@ -100,20 +100,15 @@ __device__ __forceinline__ void store8(void* p, size_t row, int dtype, const Col
 }
 
 // The gate's activation and its slope.  For bf16 results the fast exponential and reciprocal do (their error grows with |z|: 4e-6 at 86).  EXACT, for float32 x: to float32's
-// rounding.  exp(-z) = 2^hi (1 + lo ln 2) with hi + lo the product -z log2(e) in two floats, and 1 - sigmoid(z) is exp(-z) sigmoid(z), which does not cancel for large z.
-// Beyond +-88 either of them is below the normal float32 numbers, and zero; NaN stays.
+// rounding.  Beyond +-88 sigmoid or what is left of it is below the normal float32 numbers, and zero; NaN stays.
 template <bool EXACT>
 __device__ __forceinline__ void act_of(float z, int activation, float& act, float& slope) {
   if constexpr (EXACT) {
-    float zc, e, sg;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(z) : "f"(z), "f"(-88.f));
-    asm("min.NaN.f32 %0, %1, %2;" : "=f"(zc) : "f"(z), "f"(88.f));
-    const float hi = -zc * LOG2E, lo = fmaf(-zc, LOG2E_REST, fmaf(-zc, LOG2E, -hi));
-    e = ex2(hi) * fmaf(lo, 0.69314718f, 1.f);
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(sg) : "f"(1.f + e));
-    const float rest = e * sg;
+    float rest;
+    const float sg = sigmoid_full(z, rest);
+    z = clamp_nan(z, -88.f, INFINITY);
     act = activation == KDA_ACT_SILU ? z * sg : sg;
-    slope = activation == KDA_ACT_SILU ? sg * fmaf(zc, rest, 1.f) : sg * rest;
+    slope = activation == KDA_ACT_SILU ? sg * fmaf(clamp_nan(z, -88.f, 88.f), rest, 1.f) : sg * rest;
   } else {
     const float sg = sigmoid_fast(z);
     act = activation == KDA_ACT_SILU ? z * sg : sg;

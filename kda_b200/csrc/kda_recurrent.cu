@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_kernel(const Rec
   float bias[EG], al = 0.f, decay = 1.f;
 #pragma unroll
   for (int e = 0; e < EG; ++e) bias[e] = a.dt_bias ? a.dt_bias[HEAD ? h : static_cast<size_t>(h) * K + lane * E + e] : 0.f;
-  if (a.A_log) al = __expf(a.A_log[h]);
+  if (a.A_log) al = HEAD ? a.A_log[h] : __expf(a.A_log[h]);      // (HEAD: head_gate's argument)
   const size_t sbase = (static_cast<size_t>(slot) * a.H + h) * K * a.V + col;
 
   float4 S[R];
@@ -212,9 +212,10 @@ __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_kernel(const Rec
       float g = cur.g.get(HEAD ? 0 : e, g16);
       if (a.A_log) {
         g += bias[HEAD ? 0 : e];
-        g = a.use_lower_bound ? a.lower_bound * sigmoid_fast(al * g) : -al * softplus_fast(g);
+        if constexpr (HEAD) g = head_gate(g, al, a);
+        else g = a.use_lower_bound ? a.lower_bound * sigmoid_fast(al * g) : -al * softplus_fast(g);
       }
-      if constexpr (HEAD) decay = expf(g);
+      if constexpr (HEAD) decay = exp_full(g);
       else s_eg[warp][lane * E + e] = expf(g);
     }
     float qs = a.scale;
@@ -238,7 +239,7 @@ __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_kernel(const Rec
       s_q[warp][lane * E + e] = qf[e] * qs;
     }
     float beta = cur.b.get(0, b16);
-    if (a.beta_sigmoid) beta = sigmoid_fast(beta);
+    if (a.beta_sigmoid) beta = HEAD ? head_sigmoid(beta) : sigmoid_fast(beta);
     const float4 vt = make_float4(cur.v.get(0, IO16), cur.v.get(1, IO16), cur.v.get(2, IO16), cur.v.get(3, IO16));
     __syncwarp();
 
@@ -374,7 +375,7 @@ __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_t_kernel(const R
     for (int e = 0; e < E; ++e) {
       qf[e] = IoTraits<IO>::ld(qp + rowq + e);
       kf[e] = IoTraits<IO>::ld(kp + rowq + e);
-      if constexpr (HEAD) eg[e] = e == 0 ? expf(recurrent_head_decay(a, static_cast<size_t>(t) * a.H + h, h)) : eg[0];
+      if constexpr (HEAD) eg[e] = e == 0 ? exp_full(recurrent_head_decay(a, static_cast<size_t>(t) * a.H + h, h)) : eg[0];
       else eg[e] = expf(recurrent_log_decay(a, static_cast<size_t>(t) * a.H + h, h, lane * E + e, K));
     }
     float qs = a.scale;

@@ -68,24 +68,33 @@ __device__ __forceinline__ float softplus_fast(float x) {
   return x > 20.f ? x : (x < -15.f ? e : __logf(1.f + e));
 }
 // ---- the same to float32's rounding (the decode call with one decay per head, the gated norm on float32) -------------
-__device__ __forceinline__ float clamp_nan(float x, float low, float high) {      // NaN stays
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(low));
-  asm("min.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(high));
-  return x;
+__device__ __forceinline__ float at_least(float x, float low) {      // NaN stays, as in the next one
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(low));
+  return y;
 }
-// exp(x) = 2^hi (1 + lo ln 2), hi + lo the product x log2(e) in two floats; zero below -88 (no normal float32), infinite above 89
-__device__ __forceinline__ float exp_full(float x) {
-  x = clamp_nan(x, -89.f, 90.f);
+__device__ __forceinline__ float at_most(float x, float high) {
+  float y;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(high));
+  return y;
+}
+// exp(x) for x from -90 to 90, zero below -88 (no normal float32), infinite above 89: 2^hi (1 + lo ln 2), hi + lo the product x log2(e) in two floats
+__device__ __forceinline__ float exp_within(float x) {
   const float hi = x * LOG2E, lo = fmaf(x, LOG2E_REST, fmaf(x, LOG2E, -hi));
   return ex2(hi) * fmaf(lo, 0.69314718f, 1.f);
 }
-// sigmoid(z) = 1 / (1 + exp(-z)); rest: 1 - sigmoid(z) as exp(-z) sigmoid(z), which does not cancel for large z
-__device__ __forceinline__ float sigmoid_full(float z, float& rest) {
-  const float e = exp_full(-clamp_nan(z, -88.f, 88.f));
+__device__ __forceinline__ float exp_full(float x) { return exp_within(at_most(at_least(x, -90.f), 90.f)); }
+// sigmoid(z) = 1 / (1 + exp(-z)) for z from -88 to 88; rest: 1 - sigmoid(z) as exp(-z) sigmoid(z), which does not cancel for large z
+__device__ __forceinline__ float sigmoid_within(float z, float& rest) {
+  const float e = exp_within(-z);
   float sg;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(sg) : "f"(1.f + e));
   rest = e * sg;
   return sg;
+}
+__device__ __forceinline__ float sigmoid_full(float z) {
+  float rest;
+  return sigmoid_within(at_most(at_least(z, -88.f), 88.f), rest);
 }
 __device__ __forceinline__ float softplus_full(float x) { return fmaxf(x, 0.f) + log1pf(exp_full(-fabsf(x))); }
 // ---- gate front end of the recurrent kernels: activated log-decay and beta from the raw layer outputs -------------
@@ -108,12 +117,7 @@ __device__ __forceinline__ float recurrent_beta(const kda_recurrent_args& a, siz
 // decay of the state (states behind a few tokens: 1e-6 of their norm, 1e-7 so); one value per token and head costs nothing.
 __device__ __forceinline__ float head_gate(float x, float A_log, const kda_recurrent_args& a) {
   const float al = exp_full(A_log);
-  float rest;
-  return a.use_lower_bound ? a.lower_bound * sigmoid_full(al * x, rest) : -al * softplus_full(x);
-}
-__device__ __forceinline__ float head_sigmoid(float x) {
-  float rest;
-  return sigmoid_full(x, rest);
+  return a.use_lower_bound ? a.lower_bound * sigmoid_full(al * x) : -al * softplus_full(x);
 }
 __device__ __forceinline__ float recurrent_head_decay(const kda_recurrent_args& a, size_t row, int h) {
   float x = load_raw(a.g, row, a.g_raw_dtype);
@@ -123,7 +127,7 @@ __device__ __forceinline__ float recurrent_head_decay(const kda_recurrent_args& 
 }
 __device__ __forceinline__ float recurrent_head_beta(const kda_recurrent_args& a, size_t row) {
   const float x = load_raw(a.beta, row, a.beta_raw_dtype);
-  return a.beta_sigmoid ? head_sigmoid(x) : x;
+  return a.beta_sigmoid ? sigmoid_full(x) : x;
 }
 
 // ---- tensor-core primitives (warp-level, bf16 in / fp32 accumulate) ------------------------------

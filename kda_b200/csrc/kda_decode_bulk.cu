@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(HV * 2 + 32, 128 / HV) kda_decode_bulk_kernel(
     if (tid == 0) {
       float b = to_float(r.x[RB], HEAD && a.beta_raw_dtype == KDA_BF16);
       if constexpr (GATE) {
-        if (a.beta_sigmoid) b = HEAD ? head_sigmoid(to_float(r.x[RB], a.beta_raw_dtype == KDA_BF16)) : sigmoid_fast(to_float(r.x[RB], a.beta_raw_dtype == KDA_BF16));
+        if (a.beta_sigmoid) b = HEAD ? sigmoid_full(to_float(r.x[RB], a.beta_raw_dtype == KDA_BF16)) : sigmoid_fast(to_float(r.x[RB], a.beta_raw_dtype == KDA_BF16));
       }
       s.beta[buf] = b;
     }

@@ -104,11 +104,12 @@ __device__ __forceinline__ void store8(void* p, size_t row, int dtype, const Col
 template <bool EXACT>
 __device__ __forceinline__ void act_of(float z, int activation, float& act, float& slope) {
   if constexpr (EXACT) {
+    z = at_least(z, -88.f);
+    const float zc = at_most(z, 88.f);
     float rest;
-    const float sg = sigmoid_full(z, rest);
-    z = clamp_nan(z, -88.f, INFINITY);
+    const float sg = sigmoid_within(zc, rest);
     act = activation == KDA_ACT_SILU ? z * sg : sg;
-    slope = activation == KDA_ACT_SILU ? sg * fmaf(clamp_nan(z, -88.f, 88.f), rest, 1.f) : sg * rest;
+    slope = activation == KDA_ACT_SILU ? sg * fmaf(zc, rest, 1.f) : sg * rest;
   } else {
     const float sg = sigmoid_fast(z);
     act = activation == KDA_ACT_SILU ? z * sg : sg;

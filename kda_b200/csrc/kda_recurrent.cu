@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_kernel(const Rec
       s_q[warp][lane * E + e] = qf[e] * qs;
     }
     float beta = cur.b.get(0, b16);
-    if (a.beta_sigmoid) beta = HEAD ? head_sigmoid(beta) : sigmoid_fast(beta);
+    if (a.beta_sigmoid) beta = HEAD ? sigmoid_full(beta) : sigmoid_fast(beta);
     const float4 vt = make_float4(cur.v.get(0, IO16), cur.v.get(1, IO16), cur.v.get(2, IO16), cur.v.get(3, IO16));
     __syncwarp();
 

@@ -4,7 +4,7 @@
 // Bound by HBM.  A thread that loads its columns, waits for the row's sums and stores keeps too few bytes under way: 32,768 x 4096 backward 904 us, 1,048,576 x 128
 // backward 389, with half of HBM's rate.  Here one warp keeps 100 to 200 KB per SM coming and going whatever the others wait for.  Rows are copied as runs
 // of bytes, so columns need not be a multiple of anything: a stage holds as many rows as make 16 bytes even.
-//   us, forward + backward: gated 1,048,576 x 128 125 + 207 (6.4 TB/s); residual 32,768 x 4096 with an fp32 residual and post weight 247 + 472 (6.5, 5.1 TB/s: the
+//   us, forward + backward: gated 1,048,576 x 128 124 + 207 (6.4 TB/s); residual 32,768 x 4096 with an fp32 residual and post weight 248 + 470 (6.5, 5.1 TB/s: the
 //   backward's copies alone take 392, and the four sums of a row one after the other are not quite hidden behind them)
 #include <algorithm>
 

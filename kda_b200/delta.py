@@ -2,7 +2,8 @@
 
     S_t = exp(g_t) (I - beta_t k_t k_t^T) S_{t-1} + beta_t k_t v_t^T,      o_t = scale S_t^T q_t
 
-The operators keep the arguments, checks and errors of those two; only g is [B, T, HV] and with it `dt_bias` [HV].  As there, everything below the Python
+g is [B, T, HV], and with it `dt_bias` [HV].  The token-by-token operators otherwise take what theirs of the per-channel rule take; the chunked one takes a log-decay
+and a beta that are activated already (no raw gate and logits, no intermediate states), and checks its arguments as `chunk_kda` does.  Everything below the Python
 signature runs in hand-written sm_100a kernels (`csrc/delta*.cu`, `csrc/kda_recurrent.cu`, `csrc/kda_decode_bulk.cu`), and there is no fallback."""
 from __future__ import annotations
 
@@ -23,7 +24,8 @@ def fused_recurrent_gated_delta_fwd(q, k, v, g, beta, A_log=None, dt_bias=None, 
     """Decode step, forward only: `fused_recurrent_kda_fwd` with one decay per token and head.
 
     q, k [B,T,H,K]; v [B,T,HV,V]; g, beta [B,T,HV] in bfloat16 or float32 (raw layer outputs with `use_gate_in_kernel`, `use_beta_sigmoid_in_kernel`; then
-    g = -exp(A_log) softplus(g + dt_bias) with A_log, dt_bias [HV], or lower_bound sigmoid(exp(A_log) (g + dt_bias))).  K in {32, 64, 128, 256}, V a multiple of 32.
+    g = -exp(A_log) softplus(g + dt_bias) with A_log, dt_bias [HV], or lower_bound sigmoid(exp(A_log) (g + dt_bias)); to float32's rounding: states carry about 1e-7 of
+    their norm).  K in {32, 64, 128, 256}, V a multiple of 32.
     With `inplace_final_state` states are written over `initial_state`, a float32 [slots, HV, K, V] pool where `ssm_state_indices` [N] or [N, T] names the slot of
     every token: a sequence starts from the slot of its first token (with `num_accepted_tokens` [N] of its last accepted one) and the state behind token t lands
     in that token's slot.  Slots are read as 32-bit numbers; no two sequences may name the same one.  A sequence whose starting slot lies outside the pool (-1: a padded entry) or whose accepted count
@@ -71,10 +73,10 @@ def chunk_gated_delta(q, k, v, g, beta, scale=None, initial_state=None, output_f
     q, k [B,T,H,K]; v [B,T,HV,V]; g [B,T,HV] log-space decay (<= 0; -inf forgets the state) and beta [B,T,HV], in bfloat16 or float32; initial_state [N,HV,K,V]
     float32; cu_seqlens [N+1] with B == 1.  HV is a multiple of H (value head h reads q/k head h // (HV // H)).  Returns (o, final_state or None), differentiable
     with respect to q, k, v, g, beta and initial_state; gradients come in the types of their tensors.  Rows in front of the first sequence of cu_seqlens and behind
-    the last one are zero, in o and in the gradients.  `transpose_state_layout`: states are [.., V, K].
+    the last one are zero, in o and in the gradients.  `transpose_state_layout`: states are [.., V, K] (turned by a copy in front of and behind the kernels).
 
     bfloat16 with K, V up to 128 takes the chunked tensor-core kernels (columns in multiples of 8 as they are, others zero-padded); final states and dh0 carry about
-    1e-5 of their norm, which single bfloat16 operands would not give.  bfloat16 with K = 256 runs forward only, token by token.  float32 runs token by
+    1e-5 of their norm, which single bfloat16 operands would not give; the other gradients 3e-3, those of q and k per value head where heads are grouped.  bfloat16 with K = 256 runs forward only, token by token.  float32 runs token by
     token: forward for K in {32, 64, 128, 256}; with gradients (K, V in {32, 64, 128}) through `chunk_kda`, the decay spread over the key channels."""
     r = _native().chunk_delta(q, k, v, g, beta, initial_state, scale, output_final_state, cu_seqlens, use_qk_l2norm_in_kernel, transpose_state_layout, SCAN_SLICES)
     if r is not None:

@@ -512,6 +512,7 @@ static int recurrent_fwd(const kda_recurrent_args* args, bool per_head, int32_t 
     }
     if (per_head && a.N == 0 && a.tokens > 0) {      // rows of no sequence
       if (!a.o) return KDA_E_NULL;
+      if (a.io_dtype != KDA_BF16 && a.io_dtype != KDA_FP32) return KDA_E_DTYPE;
       return static_cast<int>(cudaMemsetAsync(a.o, 0, static_cast<size_t>(a.tokens) * a.H * a.V * (a.io_dtype == KDA_BF16 ? 2 : 4), static_cast<cudaStream_t>(stream)));
     }
     return KDA_OK;

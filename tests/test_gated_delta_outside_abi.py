@@ -22,4 +22,4 @@ def test_backward_without_sequences(lib, missing):      # noqa: F811
 def test_decode_without_sequences(lib):      # noqa: F811
     from kda_b200 import _lib
     call = lambda **kw: lib.kda_delta_recurrent_fwd(C.byref(_lib.RecurrentArgs(**{**dict(N=0, T=4, tokens=4, H=2, K=64, V=64, io_dtype=_lib.KDA_BF16, cu_seqlens=512), **kw})), 0, 0, None)      # noqa: E731
-    assert call(o=0) == -1 and call(tokens=0) == 0
+    assert call(o=0) == -1 and call(tokens=0) == 0 and call(o=512, io_dtype=7) == -3

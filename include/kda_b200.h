@@ -259,7 +259,7 @@ int kda_chunk_bwd(const kda_chunk_args* args, void* stream);
  * times; a wait that runs out makes its CTA stop and sets a bit, and the outputs of that call are then incomplete.
  * kda_chunk_fwd clears the word at its start and also reports an inconsistent cu_seqlens there; kda_chunk_bwd adds
  * its bits to the word of the forward whose workspace it is given.  This call copies the word to *host_out; it waits
- * for the device (cudaMemcpy), so it is a check to make after a step, not part of one.  workspace == NULL reads the
+ * for the workspace's device, every stream of it, so it is a check to make after a step, not part of one.  workspace == NULL reads the
  * word of the fixed array kda_chunk_fwd_noalloc uses on the current device.  0: nothing to report. */
 #define KDA_STATUS_SCAN_LOAD_WAIT 0x1u      /* forward scan: operand tiles of a chunk did not arrive */
 #define KDA_STATUS_SCAN_MMA_WAIT 0x2u       /* forward scan: a product did not complete */

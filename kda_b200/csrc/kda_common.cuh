@@ -78,7 +78,8 @@ __device__ __forceinline__ float at_most(float x, float high) {
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(high));
   return y;
 }
-// exp(x) for x from -90 to 90, zero below -88 (no normal float32), infinite above 89: 2^hi (1 + lo ln 2), hi + lo the product x log2(e) in two floats
+// exp(x) for x from -90 to 90, zero below -88 (no normal float32), infinite above 89: 2^hi (1 + lo ln 2), hi + lo the product x log2(e): its
+// rounding error by fma, and log2(e)'s own rest
 __device__ __forceinline__ float exp_within(float x) {
   const float hi = x * LOG2E, lo = fmaf(x, LOG2E_REST, fmaf(x, LOG2E, -hi));
   return ex2(hi) * fmaf(lo, 0.69314718f, 1.f);

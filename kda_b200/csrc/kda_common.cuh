@@ -1,7 +1,5 @@
 // Device-side helpers shared by the KDA kernels (sm_100a only).
 #pragma once
-#include <type_traits>
-
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -54,11 +52,8 @@ struct HeadArgs : kda_recurrent_args {
     const int c = num_accepted_tokens ? num_accepted_tokens[n] - 1 : 0;
     return c >= 0 && c < columns ? state_indices[static_cast<size_t>(n) * state_indices_stride + c] : -1;
   }
+  __device__ __forceinline__ bool keeps(const int32_t* slots, long long t) const { return t < columns && holds(slots[t]); }      // the state behind token t
 };
-template <bool HEAD>
-using RecArgs = std::conditional_t<HEAD, HeadArgs, kda_recurrent_args>;
-__device__ __forceinline__ bool token_slot_there(const HeadArgs& a, const int32_t* slots, long long t) { return t < a.columns && a.holds(slots[t]); }
-__device__ __forceinline__ bool token_slot_there(const kda_recurrent_args&, const int32_t*, long long) { return true; }
 
 // ---- the gate's activations (gate kernels, preparation, recurrent kernels: the same values from each) --------------
 __device__ __forceinline__ float sigmoid_fast(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }

@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(HV * 2 + 32, 128 / HV) kda_decode_bulk_kernel(
   // ================= the compute warps =================
   // A thread fetches its elements of a step's vectors (HV = 64: one of each; 128: of q and k, or of g and v) two steps ahead of its use and keeps the untouched bits in registers until
   // stash(): an instruction that depends on a load makes the thread wait for it right there, and a small load takes longer than
-  // a unit's update when the memory system is saturated.  Plain loads, no read-only ones (__ldg): see kda_recurrent.cu.
+  // a unit's update when the memory system is saturated.  Plain loads, no read-only ones (__ldg): see kda_recurrent.cuh.
   // Four registers a step, not seven: with gates the rest made the compiler touch loads still in flight (1,000 x 32, the layer's call: 682 -> 649 us)
   // (HV = 128: the threads of q, k and those of g, v use the same registers; beta waits in thread 0's slot for A_log, which it has no use for)
   constexpr int RQ = 0, RK = 1, RG = HV == 64 ? 2 : 0, RV = HV == 64 ? 3 : 1, RA = HV == 64 ? 4 : 2, RBIAS = HV == 64 ? 5 : 3, RB = HV == 64 ? 6 : 2;

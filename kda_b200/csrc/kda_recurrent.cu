@@ -8,115 +8,14 @@
 // reduction, no block barrier, warps are independent.
 // Per token (order as in fla/ops/kda/fused_recurrent.py:146-192): S *= exp(g); v' = beta (v - S^T k);
 // S += k v'^T; o = scale S^T q.
-#include "kda_common.cuh"
-#include "kda_device.cuh"
+#include "kda_recurrent.cuh"
 
 namespace kda {
 
-template <typename IO> struct IoTraits;
-template <> struct IoTraits<float> {
-  static __device__ __forceinline__ float ld(const float* p) { return *p; }
-  static __device__ __forceinline__ void st4(float* p, float4 x) { *reinterpret_cast<float4*>(p) = x; }
-  static __device__ __forceinline__ float4 ld4(const float* p) { return *reinterpret_cast<const float4*>(p); }
-};
-template <> struct IoTraits<__nv_bfloat16> {
-  static __device__ __forceinline__ float ld(const __nv_bfloat16* p) { return __bfloat162float(*p); }
-  static __device__ __forceinline__ void st4(__nv_bfloat16* p, float4 x) {
-    uint2 u = make_uint2(pack_bf16(x.x, x.y), pack_bf16(x.z, x.w));
-    *reinterpret_cast<uint2*>(p) = u;
-  }
-  static __device__ __forceinline__ float4 ld4(const __nv_bfloat16* p) {
-    uint2 u = *reinterpret_cast<const uint2*>(p);
-    float2 a = unpack_bf16(u.x), b = unpack_bf16(u.y);
-    return make_float4(a.x, a.y, b.x, b.y);
-  }
-};
-
-constexpr int REC_WARPS = 4;
-
-// Sum over the 32 lanes of 32 per-lane values at once: lane L returns the total of v[L] (31 shuffles).
-__device__ __forceinline__ float butterfly_sum32(float (&v)[32], int lane) {
-#pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) {
-    const bool up = (lane & o) != 0;
-#pragma unroll
-    for (int i = 0; i < o; ++i) {
-      const float mine = up ? v[i + o] : v[i];
-      const float other = up ? v[i] : v[i + o];
-      v[i] = mine + __shfl_xor_sync(0xffffffffu, other, o);
-    }
-  }
-  return v[0];
-}
-
-// E consecutive elements of a row as untouched bits: a conversion right behind the load would make the warp wait for it there.
-// Plain loads, no read-only ones (__ldg) in this file: a chained kernel's lifetime overlaps that of the kernel in front, which may be writing
-// these tensors, and read-only loads are defined only for data that nobody writes meanwhile (nor are they held behind chain_point()).
-template <int E>
-struct RowBits {
-  uint32_t w[E];
-  __device__ __forceinline__ void load(const void* base, size_t i, bool bf16) {
-    if (bf16) {
-      const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(base) + i;
-      if constexpr (E == 1) w[0] = *reinterpret_cast<const unsigned short*>(p);
-      else if constexpr (E == 2) w[0] = *reinterpret_cast<const uint32_t*>(p);
-      else {
-#pragma unroll
-        for (int e = 0; e < E / 4; ++e) {
-          const uint2 u = reinterpret_cast<const uint2*>(p)[e];
-          w[2 * e] = u.x; w[2 * e + 1] = u.y;
-        }
-      }
-    } else {
-      const uint32_t* p = static_cast<const uint32_t*>(base) + i;
-      if constexpr (E == 1) w[0] = *p;
-      else {
-#pragma unroll
-        for (int e = 0; e < E / 2; ++e) {
-          const uint2 u = reinterpret_cast<const uint2*>(p)[e];
-          w[2 * e] = u.x; w[2 * e + 1] = u.y;
-        }
-      }
-    }
-  }
-  __device__ __forceinline__ float get(int e, bool bf16) const {
-    if (!bf16) return __uint_as_float(w[e]);
-    const uint32_t u = w[e >> 1];
-    return __uint_as_float((e & 1) ? u & 0xffff0000u : u << 16);
-  }
-};
-
-// One decay per head, packed: rows of o in front of the first sequence and behind the last one become zeros.  All sequences' warps share them, so that a server's padded
-// buffer costs no more than its bytes.  Asked for in front of the tokens, used behind them; cut to the call's tokens.
-struct RowsOfNone {
-  long long first, last;
-  template <bool CLEAR>
-  __device__ __forceinline__ static RowsOfNone of(const kda_recurrent_args& a) {
-    if constexpr (CLEAR) return {a.cu_seqlens[0], a.cu_seqlens[a.N]};
-    else return {0, 0};
-  }
-  // a warp's part: four columns from `col` on in every RG-th row, rg the lane's first
-  template <typename IO, int RG>
-  __device__ __forceinline__ void clear(const kda_recurrent_args& a, long long n, int h, int col, int rg) const {
-    const size_t row = static_cast<size_t>(a.H) * a.V, step = static_cast<size_t>(a.N) * RG * row;
-    auto zeros = [&](long long from, long long to) {
-      long long t = from + n * RG + rg;
-      IO* p = static_cast<IO*>(a.o) + static_cast<size_t>(t) * row + static_cast<size_t>(h) * a.V + col;
-#pragma unroll 4
-      for (; t < to; t += static_cast<long long>(a.N) * RG, p += step) IoTraits<IO>::st4(p, make_float4(0.f, 0.f, 0.f, 0.f));
-    };
-    zeros(0, first < a.tokens ? first : a.tokens);
-    const long long from = last > 0 ? last : 0;
-    zeros(first > from ? first : from, a.tokens);
-  }
-};
-
 // A token's vectors are fetched while the token before is worked on: with one warp per slice there is nobody else to hide
 // their latency (one sequence of four draft tokens: 14.2 us when each token fetched its own, 8.0 us so).
-// HEAD: one decay per token and head (kda_delta_recurrent_fwd).
-// CLEAR (with HEAD): packed, so that there may be rows of no sequence (a variant of its own: with the rows' few instructions in it one token of one sequence takes 4.1 us, 3.6 without).
-template <typename IO, int K, int VS, bool HEAD, bool CLEAR>
-__global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_kernel(const RecArgs<HEAD> a) {
+template <typename IO, int K, int VS>
+__global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_kernel(const kda_recurrent_args a) {
   chain_point();
   constexpr int CL = VS / 4;      // lanes across the V slice (4 columns each)
   constexpr int RG = 32 / CL;     // row groups
@@ -125,7 +24,7 @@ __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_kernel(const Rec
   constexpr bool IO16 = sizeof(IO) == 2;
   static_assert(K % RG == 0 && K % 32 == 0, "unsupported K");
 
-  __shared__ float s_k[REC_WARPS][K], s_q[REC_WARPS][K], s_eg[REC_WARPS][HEAD ? 1 : K];
+  __shared__ float s_k[REC_WARPS][K], s_q[REC_WARPS][K], s_eg[REC_WARPS][K];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int nvs = a.V / VS;
@@ -143,19 +42,13 @@ __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_kernel(const Rec
   if (a.cu_seqlens) {
     bos = a.cu_seqlens[n];
     eos = a.cu_seqlens[n + 1];
-    if constexpr (HEAD) {      // (offsets outside the call's tokens are not followed either)
-      bos = bos < 0 ? 0 : bos;
-      eos = eos < a.tokens ? eos : a.tokens;
-    }
   } else {
     bos = static_cast<long long>(n) * a.T;
     eos = bos + a.T;
   }
-  const bool g16 = (HEAD || a.A_log) && a.g_raw_dtype == KDA_BF16, b16 = (HEAD || a.beta_sigmoid) && a.beta_raw_dtype == KDA_BF16;
-  constexpr int EG = HEAD ? 1 : E;      // g elements per lane
+  const bool g16 = a.A_log && a.g_raw_dtype == KDA_BF16, b16 = a.beta_sigmoid && a.beta_raw_dtype == KDA_BF16;
   struct Token {
-    RowBits<E> q, k;
-    RowBits<EG> g;
+    RowBits<E> q, k, g;
     RowBits<4> v;
     RowBits<1> b;
   };
@@ -164,30 +57,19 @@ __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_kernel(const Rec
     const size_t row = static_cast<size_t>(t) * a.H + h;
     x.q.load(a.q, rowq, IO16);
     x.k.load(a.k, rowq, IO16);
-    x.g.load(a.g, HEAD ? row : row * K + lane * E, g16);
+    x.g.load(a.g, row * K + lane * E, g16);
     x.b.load(a.beta, row, b16);
     x.v.load(a.v, row * a.V + col, IO16);
   };
   // continuous batching: the sequence's row of slot numbers; it starts from the slot of the last accepted token
   const int32_t* slots = a.state_indices ? a.state_indices + static_cast<size_t>(n) * a.state_indices_stride : nullptr;
-  [[maybe_unused]] const RowsOfNone none = RowsOfNone::of<CLEAR>(a);
-  long long slot = n;
-  if constexpr (HEAD) {
-    if (slots && !a.holds(slot = a.start_slot(n))) {
-      if (rg == 0)
-        for (long long t = bos; t < eos; ++t) IoTraits<IO>::st4(static_cast<IO*>(a.o) + (static_cast<size_t>(t) * a.H + h) * a.V + col, make_float4(0.f, 0.f, 0.f, 0.f));
-      if constexpr (CLEAR) none.clear<IO, RG>(a, n, h, col, rg);
-      return;
-    }
-  } else if (slots) {
-    slot = slots[a.num_accepted_tokens ? a.num_accepted_tokens[n] - 1 : 0];
-  }
+  const long long slot = slots ? slots[a.num_accepted_tokens ? a.num_accepted_tokens[n] - 1 : 0] : n;
   Token cur, nxt;
   if (bos < eos) fetch(bos, cur);
-  float bias[EG], al = 0.f, decay = 1.f;
+  float bias[E], al = 0.f;
 #pragma unroll
-  for (int e = 0; e < EG; ++e) bias[e] = a.dt_bias ? a.dt_bias[HEAD ? h : static_cast<size_t>(h) * K + lane * E + e] : 0.f;
-  if (a.A_log) al = HEAD ? a.A_log[h] : __expf(a.A_log[h]);      // (HEAD: head_gate's argument)
+  for (int e = 0; e < E; ++e) bias[e] = a.dt_bias ? a.dt_bias[static_cast<size_t>(h) * K + lane * E + e] : 0.f;
+  if (a.A_log) al = __expf(a.A_log[h]);
   const size_t sbase = (static_cast<size_t>(slot) * a.H + h) * K * a.V + col;
 
   float4 S[R];
@@ -208,15 +90,12 @@ __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_kernel(const Rec
     for (int e = 0; e < E; ++e) {
       qf[e] = cur.q.get(e, IO16);
       kf[e] = cur.k.get(e, IO16);
-      if (HEAD && e > 0) continue;
-      float g = cur.g.get(HEAD ? 0 : e, g16);
+      float g = cur.g.get(e, g16);
       if (a.A_log) {
-        g += bias[HEAD ? 0 : e];
-        if constexpr (HEAD) g = head_gate(g, al, a);
-        else g = a.use_lower_bound ? a.lower_bound * sigmoid_fast(al * g) : -al * softplus_fast(g);
+        g += bias[e];
+        g = a.use_lower_bound ? a.lower_bound * sigmoid_fast(al * g) : -al * softplus_fast(g);
       }
-      if constexpr (HEAD) decay = exp_full(g);
-      else s_eg[warp][lane * E + e] = expf(g);
+      s_eg[warp][lane * E + e] = expf(g);
     }
     float qs = a.scale;
     if (a.use_qk_l2norm) {
@@ -239,7 +118,7 @@ __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_kernel(const Rec
       s_q[warp][lane * E + e] = qf[e] * qs;
     }
     float beta = cur.b.get(0, b16);
-    if (a.beta_sigmoid) beta = HEAD ? sigmoid_full(beta) : sigmoid_fast(beta);
+    if (a.beta_sigmoid) beta = sigmoid_fast(beta);
     const float4 vt = make_float4(cur.v.get(0, IO16), cur.v.get(1, IO16), cur.v.get(2, IO16), cur.v.get(3, IO16));
     __syncwarp();
 
@@ -247,7 +126,7 @@ __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_kernel(const Rec
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       const int r = rg + RG * i;
-      const float eg = HEAD ? decay : s_eg[warp][r], kk = s_k[warp][r];
+      const float eg = s_eg[warp][r], kk = s_k[warp][r];
       S[i].x *= eg; S[i].y *= eg; S[i].z *= eg; S[i].w *= eg;
       hk.x += kk * S[i].x; hk.y += kk * S[i].y; hk.z += kk * S[i].z; hk.w += kk * S[i].w;
     }
@@ -275,7 +154,7 @@ __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_kernel(const Rec
       oa.w += __shfl_xor_sync(0xffffffffu, oa.w, off);
     }
     if (rg == 0) IoTraits<IO>::st4(op + (static_cast<size_t>(t) * a.H + h) * a.V + col, oa);
-    if (slots && a.ht && token_slot_there(a, slots, t - bos)) {      // the state after every token goes to that token's slot
+    if (slots && a.ht) {      // the state after every token goes to that token's slot
       const size_t tb = (static_cast<size_t>(slots[t - bos]) * a.H + h) * K * a.V + col;
 #pragma unroll
       for (int i = 0; i < R; ++i) __stcs(reinterpret_cast<float4*>(a.ht + tb + static_cast<size_t>(rg + RG * i) * a.V), S[i]);
@@ -289,24 +168,6 @@ __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_kernel(const Rec
     for (int i = 0; i < R; ++i)
       __stcs(reinterpret_cast<float4*>(a.ht + sbase + static_cast<size_t>(rg + RG * i) * a.V), S[i]);
   }
-  if constexpr (CLEAR) none.clear<IO, RG>(a, n, h, col, rg);
-}
-
-// E (2 or 4) consecutive floats of a state row, streaming loads / stores of 8 or 16 bytes
-template <int E>
-__device__ __forceinline__ void ld_row(float (&d)[E], const float* p) {
-  if constexpr (E == 4) {
-    const float4 x = __ldcs(reinterpret_cast<const float4*>(p));
-    d[0] = x.x; d[1] = x.y; d[2] = x.z; d[3] = x.w;
-  } else {
-    const float2 x = __ldcs(reinterpret_cast<const float2*>(p));
-    d[0] = x.x; d[1] = x.y;
-  }
-}
-template <int E>
-__device__ __forceinline__ void st_row(float* p, const float (&d)[E]) {
-  if constexpr (E == 4) __stcs(reinterpret_cast<float4*>(p), make_float4(d[0], d[1], d[2], d[3]));
-  else __stcs(reinterpret_cast<float2*>(p), make_float2(d[0], d[1]));
 }
 
 // ---- transposed state layout [slots, H, V, K] (K contiguous) ------------------------------------------------------
@@ -314,8 +175,8 @@ __device__ __forceinline__ void st_row(float* p, const float (&d)[E]) {
 // lane*(K/32) .. of those rows, so every state access is again contiguous over the warp.  The two reductions over K
 // are per-lane partial dot products summed over the lanes 32 values at a time by a butterfly (lane L ends up with
 // the total of value row L); the delta-rule update needs every row's dv in every lane: one shuffle per row.
-template <typename IO, int K, bool HEAD, bool CLEAR>
-__global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_t_kernel(const RecArgs<HEAD> a) {
+template <typename IO, int K>
+__global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_t_kernel(const kda_recurrent_args a) {
   constexpr int E = K / 32;       // key columns per lane
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int nvs = a.V / 32;
@@ -330,26 +191,12 @@ __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_t_kernel(const R
   if (a.cu_seqlens) {
     bos = a.cu_seqlens[n];
     eos = a.cu_seqlens[n + 1];
-    if constexpr (HEAD) {      // (offsets outside the call's tokens are not followed either)
-      bos = bos < 0 ? 0 : bos;
-      eos = eos < a.tokens ? eos : a.tokens;
-    }
   } else {
     bos = static_cast<long long>(n) * a.T;
     eos = bos + a.T;
   }
   const int32_t* slots = a.state_indices ? a.state_indices + static_cast<size_t>(n) * a.state_indices_stride : nullptr;
-  [[maybe_unused]] const RowsOfNone none = RowsOfNone::of<CLEAR>(a);
-  long long slot = n;
-  if constexpr (HEAD) {
-    if (slots && !a.holds(slot = a.start_slot(n))) {
-      for (long long t = bos; t < eos; ++t) static_cast<IO*>(a.o)[(static_cast<size_t>(t) * a.H + h) * a.V + vs * 32 + lane] = IO(0.f);
-      if constexpr (CLEAR) none.clear<IO, 4>(a, n, h, vs * 32 + 4 * (lane & 7), lane >> 3);
-      return;
-    }
-  } else if (slots) {
-    slot = slots[a.num_accepted_tokens ? a.num_accepted_tokens[n] - 1 : 0];
-  }
+  const long long slot = slots ? slots[a.num_accepted_tokens ? a.num_accepted_tokens[n] - 1 : 0] : n;
   auto state_ptr = [&](const float* base, long long sl) {
     return base + ((static_cast<size_t>(sl) * a.H + h) * a.V + vs * 32) * K + lane * E;
   };
@@ -375,8 +222,7 @@ __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_t_kernel(const R
     for (int e = 0; e < E; ++e) {
       qf[e] = IoTraits<IO>::ld(qp + rowq + e);
       kf[e] = IoTraits<IO>::ld(kp + rowq + e);
-      if constexpr (HEAD) eg[e] = e == 0 ? exp_full(recurrent_head_decay(a, static_cast<size_t>(t) * a.H + h, h)) : eg[0];
-      else eg[e] = expf(recurrent_log_decay(a, static_cast<size_t>(t) * a.H + h, h, lane * E + e, K));
+      eg[e] = expf(recurrent_log_decay(a, static_cast<size_t>(t) * a.H + h, h, lane * E + e, K));
     }
     float qs = a.scale;
     if (a.use_qk_l2norm) {
@@ -395,7 +241,7 @@ __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_t_kernel(const R
     }
 #pragma unroll
     for (int e = 0; e < E; ++e) qf[e] *= qs;
-    const float beta = HEAD ? recurrent_head_beta(a, static_cast<size_t>(t) * a.H + h) : recurrent_beta(a, static_cast<size_t>(t) * a.H + h);
+    const float beta = recurrent_beta(a, static_cast<size_t>(t) * a.H + h);
     const float vt = IoTraits<IO>::ld(vp + (static_cast<size_t>(t) * a.H + h) * a.V + vs * 32 + lane);      // value row `lane`
     float part[32];
 #pragma unroll
@@ -424,7 +270,7 @@ __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_t_kernel(const R
     const float o = butterfly_sum32(part, lane);
     if (sizeof(IO) == 2) reinterpret_cast<__nv_bfloat16*>(op)[(static_cast<size_t>(t) * a.H + h) * a.V + vs * 32 + lane] = __float2bfloat16_rn(o);
     else reinterpret_cast<float*>(op)[(static_cast<size_t>(t) * a.H + h) * a.V + vs * 32 + lane] = o;
-    if (slots && a.ht && token_slot_there(a, slots, t - bos)) {
+    if (slots && a.ht) {
       float* pt = const_cast<float*>(state_ptr(a.ht, slots[t - bos]));
 #pragma unroll
       for (int r = 0; r < 32; ++r) st_row<E>(pt + static_cast<size_t>(r) * K, S[r]);
@@ -435,53 +281,43 @@ __global__ void __launch_bounds__(REC_WARPS * 32) kda_recurrent_t_kernel(const R
 #pragma unroll
     for (int r = 0; r < 32; ++r) st_row<E>(pt + static_cast<size_t>(r) * K, S[r]);
   }
-  if constexpr (CLEAR) none.clear<IO, 4>(a, n, h, vs * 32 + 4 * (lane & 7), lane >> 3);
 }
 
-template <typename IO, int K, bool HEAD>
-static int launch_rec_t(const RecArgs<HEAD>& a, cudaStream_t st) {
+template <typename IO, int K>
+static int launch_rec_t(const kda_recurrent_args& a, cudaStream_t st) {
   const long long total = static_cast<long long>(a.N) * a.H * (a.V / 32);
   const long long blocks = (total + REC_WARPS - 1) / REC_WARPS;
   if (blocks <= 0) return KDA_OK;
   if (blocks > 0x7fffffffLL) return KDA_E_SHAPE;
-  if constexpr (HEAD) {
-    if (a.cu_seqlens) {
-      kda_recurrent_t_kernel<IO, K, HEAD, true><<<static_cast<unsigned>(blocks), REC_WARPS * 32, 0, st>>>(a);
-      return static_cast<int>(cudaGetLastError());
-    }
-  }
-  kda_recurrent_t_kernel<IO, K, HEAD, false><<<static_cast<unsigned>(blocks), REC_WARPS * 32, 0, st>>>(a);
+  kda_recurrent_t_kernel<IO, K><<<static_cast<unsigned>(blocks), REC_WARPS * 32, 0, st>>>(a);
   return static_cast<int>(cudaGetLastError());
 }
 
-template <typename IO, int K, int VS, bool HEAD>
-static int launch_rec(const RecArgs<HEAD>& a, cudaStream_t st) {
+template <typename IO, int K, int VS>
+static int launch_rec(const kda_recurrent_args& a, cudaStream_t st) {
   const long long total = static_cast<long long>(a.N) * a.H * (a.V / VS);
   const long long blocks = (total + REC_WARPS - 1) / REC_WARPS;
   if (blocks <= 0) return KDA_OK;
   if (blocks > 0x7fffffffLL) return KDA_E_SHAPE;
-  if constexpr (HEAD) {
-    if (a.cu_seqlens) return static_cast<int>(launch_chained(kda_recurrent_kernel<IO, K, VS, HEAD, true>, static_cast<unsigned>(blocks), REC_WARPS * 32, 0, st, a));
-  }
-  return static_cast<int>(launch_chained(kda_recurrent_kernel<IO, K, VS, HEAD, false>, static_cast<unsigned>(blocks), REC_WARPS * 32, 0, st, a));
+  return static_cast<int>(launch_chained(kda_recurrent_kernel<IO, K, VS>, static_cast<unsigned>(blocks), REC_WARPS * 32, 0, st, a));
 }
 
-template <typename IO, bool HEAD>
-static int dispatch_rec(const RecArgs<HEAD>& a, cudaStream_t st) {
+template <typename IO>
+static int dispatch_rec(const kda_recurrent_args& a, cudaStream_t st) {
   if (a.transpose_state) {
     switch (a.K) {
-      case 64: return launch_rec_t<IO, 64, HEAD>(a, st);
-      case 128: return launch_rec_t<IO, 128, HEAD>(a, st);
+      case 64: return launch_rec_t<IO, 64>(a, st);
+      case 128: return launch_rec_t<IO, 128>(a, st);
       default: return KDA_E_SHAPE;
     }
   }
   switch (a.K) {
-    case 32: return launch_rec<IO, 32, 32, HEAD>(a, st);
-    case 64: return launch_rec<IO, 64, 32, HEAD>(a, st);
+    case 32: return launch_rec<IO, 32, 32>(a, st);
+    case 64: return launch_rec<IO, 64, 32>(a, st);
     // one or two sequences leave most SMs idle: twice as many warps with half the columns each (one sequence x 32 heads, one token: 3.4
     // instead of 4.3 us; from half a state per SM on the wider slices win: 96 states 4.3 against 4.5 us)
-    case 128: return 2LL * a.N * a.H <= sm_count() ? launch_rec<IO, 128, 16, HEAD>(a, st) : launch_rec<IO, 128, 32, HEAD>(a, st);
-    case 256: return (a.V % 32 == 0) ? launch_rec<IO, 256, 16, HEAD>(a, st) : KDA_E_SHAPE;
+    case 128: return 2LL * a.N * a.H <= sm_count() ? launch_rec<IO, 128, 16>(a, st) : launch_rec<IO, 128, 32>(a, st);
+    case 256: return (a.V % 32 == 0) ? launch_rec<IO, 256, 16>(a, st) : KDA_E_SHAPE;
     default: return KDA_E_SHAPE;
   }
 }
@@ -526,8 +362,9 @@ static int recurrent_fwd(const kda_recurrent_args* args, bool per_head, int32_t 
   if (bits & 15u) return KDA_E_ALIGN;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (kda::decode_bulk_covers(a)) return kda::decode_bulk_launch(a, per_head, st);
-  if (a.io_dtype == KDA_BF16) return per_head ? kda::dispatch_rec<__nv_bfloat16, true>(a, st) : kda::dispatch_rec<__nv_bfloat16, false>(a, st);
-  if (a.io_dtype == KDA_FP32) return per_head ? kda::dispatch_rec<float, true>(a, st) : kda::dispatch_rec<float, false>(a, st);
+  if (per_head) return kda::recurrent_head_launch(a, st);
+  if (a.io_dtype == KDA_BF16) return kda::dispatch_rec<__nv_bfloat16>(a, st);
+  if (a.io_dtype == KDA_FP32) return kda::dispatch_rec<float>(a, st);
   return KDA_E_DTYPE;
 }
 

@@ -4,7 +4,7 @@
 
 g is [B, T, HV], and with it `dt_bias` [HV].  The token-by-token operators otherwise take what theirs of the per-channel rule take; the chunked one takes a log-decay
 and a beta that are activated already (no raw gate and logits, no intermediate states), and checks its arguments as `chunk_kda` does.  Everything below the Python
-signature runs in hand-written sm_100a kernels (`csrc/delta*.cu`, `csrc/kda_recurrent.cu`, `csrc/kda_decode_bulk.cu`), and there is no fallback."""
+signature runs in hand-written sm_100a kernels (`csrc/delta*.cu`, `csrc/kda_decode_bulk.cu`), and there is no fallback."""
 from __future__ import annotations
 
 import torch
